@@ -45,6 +45,16 @@ void attention_forward(at::Tensor qkv, at::Tensor out, at::Tensor lse, int64_t H
                        int64_t q_begin, int64_t q_len);
 void attention_backward(at::Tensor qkv, at::Tensor out, at::Tensor dout, at::Tensor lse, at::Tensor delta, at::Tensor dqkv,
                         int64_t H, int64_t HKV, int64_t D, bool causal, double scale, int64_t q_begin, int64_t q_len);
+void kv_cache_write(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale, c10::optional<at::Tensor> v_scale,
+                    at::Tensor k, at::Tensor v, at::Tensor slots);
+void kv_cache_read(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale, c10::optional<at::Tensor> v_scale,
+                   at::Tensor slots, at::Tensor k, at::Tensor v);
+void paged_attention(at::Tensor q, at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale,
+                     c10::optional<at::Tensor> v_scale, at::Tensor block_table, at::Tensor lengths, at::Tensor out,
+                     c10::optional<at::Tensor> lse, double scale);
+void sample_tokens(at::Tensor logits, at::Tensor noise, c10::optional<at::Tensor> temperature_rows, double temperature,
+                   c10::optional<at::Tensor> top_k_rows, int64_t top_k, c10::optional<at::Tensor> top_p_rows, double top_p,
+                   c10::optional<at::Tensor> min_p_rows, double min_p, at::Tensor token, at::Tensor logprob);
 void bucket_all_reduce(at::Tensor flat, std::vector<int64_t> buffer_ptrs, std::vector<int64_t> pad_ptrs, int64_t multicast_ptr,
                        int64_t start, int64_t numel, double scale, int64_t rank, int64_t slot_base, int64_t max_blocks,
                        at::Tensor status, double timeout_s, bool wide, int64_t min_peer_slots);
@@ -95,6 +105,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_backward", &ht::attention_backward, py::arg("qkv"), py::arg("out"), py::arg("dout"), py::arg("lse"),
         py::arg("delta"), py::arg("dqkv"), py::arg("H"), py::arg("HKV"), py::arg("D"), py::arg("causal"), py::arg("scale"),
         py::arg("q_begin") = 0, py::arg("q_len") = -1);
+  m.def("kv_cache_write", &ht::kv_cache_write, "write keys and values into a paged pool (bf16, or 8 bits with a scale per row)");
+  m.def("kv_cache_read", &ht::kv_cache_read, "read rows of a paged pool back as bf16");
+  m.def("paged_attention", &ht::paged_attention, "attention of one new token per sequence over a paged pool");
+  m.def("sample_tokens", &ht::sample_tokens, "next tokens from logits and given random numbers (temperature, top-k, top-p, min-p)");
   m.def("bucket_all_reduce", &ht::bucket_all_reduce, "in-kernel NVLink all-reduce of one DDP bucket");
   m.def("fsdp_reduce_scatter_adamw", &ht::fsdp_reduce_scatter_adamw,
         "FSDP gradient reduce-scatter fused with the cast and the sharded AdamW update (NVLink peer memory)");

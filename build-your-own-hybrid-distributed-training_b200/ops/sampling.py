@@ -1,0 +1,94 @@
+"""Choosing the next token from logits and given random numbers (temperature, top-k, top-p, min-p).
+
+``sample_tokens`` draws by an exponential race: with ``noise`` independent and exponentially
+distributed (``torch.empty(B, V).exponential_()``), the token with the largest ``weight / noise`` among
+those that the filters leave is a draw from their softmax.  The random numbers are the caller's, so a
+draw can be repeated, and no rounding of a long cumulative sum decides it.  The kernel is
+``csrc/sampling.cu``; the reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from ..errors import ConfigurationError, format_error
+from ._ext import extension
+
+__all__ = ["reference_sample_tokens", "sample_tokens"]
+
+Number = float | int | torch.Tensor
+
+
+def _refuse(problem: str, expected: object, observed: object, resolution: str) -> ConfigurationError:
+    return ConfigurationError(format_error("ops.sample_tokens", problem, expected=expected, observed=observed, resolution=resolution))
+
+
+def _checked(name: str, value: Number, logits: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor | None, float | int]:
+    if isinstance(value, torch.Tensor):
+        if value.shape != logits.shape[:1] or value.dtype != dtype or value.device != logits.device:
+            raise _refuse(f"{name} does not fit the logits", f"a number or a {dtype} tensor [{logits.shape[0]}] on {logits.device}",
+                          f"{value.dtype} {tuple(value.shape)} on {value.device}", "pass one value per row, or one number")
+        return value.contiguous(), 0
+    if math.isnan(value) or value < 0 or (name == "top_p" and value > 1) or (name == "min_p" and value > 1):
+        raise _refuse(f"{name} is out of range", "0 to 1" if name in ("top_p", "min_p") else "0 or more", value, "choose a value in range")
+    return None, value
+
+
+def reference_sample_tokens(logits: torch.Tensor, noise: torch.Tensor, temperature: Number = 1.0, top_k: Number = 0, top_p: Number = 1.0,
+                            min_p: Number = 0.0, *, compute_dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+    """Plain PyTorch statement of :func:`sample_tokens` (the CPU path)."""
+    b, v = logits.shape
+    col = lambda x: (x if isinstance(x, torch.Tensor) else torch.full((b,), x, device=logits.device))[:, None]  # noqa: E731
+    temperature, top_k, top_p, min_p = (col(x) for x in (temperature, top_k, top_p, min_p))
+    z = logits.to(compute_dtype)
+    z = torch.where(torch.isnan(z), -math.inf, z)
+    best = z.amax(-1, keepdim=True)
+    empty = best[:, 0] == -math.inf
+    greedy = ~(temperature > 0)
+    x = torch.where(z == best, 0.0, torch.where(z == -math.inf, -math.inf, (z - best) / torch.where(greedy, 1.0, temperature.to(compute_dtype))))
+    w = torch.exp(x)
+    ranked, order = torch.sort(z, dim=-1, descending=True, stable=True)
+    rank = torch.arange(v, device=logits.device)[None]
+    keep = (rank < top_k) | (top_k <= 0)
+    ws = torch.gather(w, 1, order)
+    mass = torch.where(keep, ws, 0.0)
+    before = torch.cumsum(mass, -1) - mass
+    keep &= (before < top_p.to(compute_dtype) * mass.sum(-1, keepdim=True)) | (top_p >= 1)
+    keep &= (ws >= min_p) & ~greedy & (ranked > -math.inf)
+    keep |= rank == 0
+    score = torch.where(keep, ws / torch.gather(noise.to(compute_dtype), 1, order), -1.0)
+    token = torch.where(score == score.amax(-1, keepdim=True), order, v).amin(-1)
+    logprob = torch.gather(x, 1, token.clamp(max=v - 1)[:, None])[:, 0] - torch.log(w.sum(-1))
+    return torch.where(empty, -1, token), torch.where(empty, -math.inf, logprob)
+
+
+def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, *, temperature: Number = 1.0, top_k: Number = 0, top_p: Number = 1.0,
+                  min_p: Number = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """One token per row of ``logits`` ``[B, V]`` (bf16 or fp32), drawn with ``noise`` ``[B, V]`` (fp32, positive, Exp(1)).
+
+    The filters apply in this order: ``top_k`` keeps that many tokens of the largest logits (0: all), ``top_p`` the
+    smallest prefix of those that holds this share of their probability (1: all), ``min_p`` drops tokens less
+    probable than this share of the most probable one.  The most probable token always stays, the lower index wins
+    ties, and ``temperature`` 0 takes it without drawing.  Each of the four is a number or one value per row
+    (fp32; ``top_k`` int32).  Returns ``(tokens int64 [B], logprobs fp32 [B])``; the log-probability is that of the whole
+    row at this temperature (at 1 where the temperature is 0), before any filter.  Logits of ``-inf`` or NaN cannot
+    be drawn; a row without any other gives ``-1`` and ``-inf``.
+    """
+    if logits.dim() != 2 or logits.shape[1] == 0 or noise.shape != logits.shape or noise.dtype != torch.float32 or noise.device != logits.device:
+        raise _refuse("logits and noise must be alike", "[B, V] logits and fp32 noise of the same shape and device",
+                      f"{tuple(logits.shape)} and {noise.dtype} {tuple(noise.shape)} on {noise.device}", "draw one Exp(1) number per logit")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise _refuse("unsupported logit type", "bfloat16 or float32", logits.dtype, "cast the logits")
+    t_rows, t = _checked("temperature", temperature, logits, torch.float32)
+    k_rows, k = _checked("top_k", top_k, logits, torch.int32)
+    p_rows, p = _checked("top_p", top_p, logits, torch.float32)
+    m_rows, m = _checked("min_p", min_p, logits, torch.float32)
+    logits = logits.detach()
+    if not logits.is_cuda:
+        return reference_sample_tokens(logits, noise, temperature, top_k, top_p, min_p)
+    token = torch.empty(logits.shape[0], dtype=torch.int64, device=logits.device)
+    logprob = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+    extension().sample_tokens(logits, noise, t_rows, t, k_rows, k, p_rows, p, m_rows, m, token, logprob)
+    return token, logprob
