@@ -12,9 +12,7 @@
 //
 // Bound: memory.  Both kernels touch every byte once, 16 bytes of bf16 per lane and D / 8 lanes per
 // row.
-#include "common.cuh"
-
-#include "kv_cache.cuh"
+#include "generation.cuh"
 
 namespace ht {
 namespace kv {
@@ -47,16 +45,6 @@ __device__ __forceinline__ float value_of(uint32_t byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
 }
 
-struct WriteArgs {
-  const __nv_bfloat16* src[2];  // k, v: [T, Hkv, D]
-  long long tok[2], head[2];    // strides in elements
-  void* dst[2];                 // pools
-  float* scale[2];
-  const void* slots;
-  long long T, capacity;
-  int Hkv, page_shift, wide;  // wide: int64 slots
-};
-
 __device__ __forceinline__ long long slot_of(const void* slots, int wide, long long t) {
   return wide ? static_cast<const long long*>(slots)[t] : (long long)static_cast<const int*>(slots)[t];
 }
@@ -70,23 +58,27 @@ __device__ __forceinline__ long long pool_row(long long slot, int h, int Hkv, in
 template <int F, int D>
 __global__ void __launch_bounds__(THREADS) write_kernel(WriteArgs a) {
   constexpr int LANES = D / 8;
-  const long long rows = a.T * a.Hkv;
+  const long long rows = a.T * a.pool.Hkv;
   const int lane = threadIdx.x % LANES;
-  const int which = blockIdx.y;
+  const int which = blockIdx.y;  // 0: keys, 1: values
+  const __nv_bfloat16* const src = which ? a.src[1] : a.src[0];
+  const long long tok = which ? a.tok[1] : a.tok[0], head = which ? a.head[1] : a.head[0];
+  void* const pool = which ? a.pool.v : a.pool.k;
+  float* const scales = which ? a.pool.v_scale : a.pool.k_scale;
   const long long step = (long long)gridDim.x * (THREADS / LANES);
   const long long first = (long long)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
   // every lane of a warp makes the same number of turns, so the shuffles below always see a full warp
   for (long long base = first; base - threadIdx.x / LANES < rows; base += step) {
     const bool on = base < rows;
-    const long long t = on ? base / a.Hkv : 0;
-    const int h = on ? (int)(base - t * a.Hkv) : 0;
+    const long long t = on ? base / a.pool.Hkv : 0;
+    const int h = on ? (int)(base - t * a.pool.Hkv) : 0;
     const long long slot = on ? slot_of(a.slots, a.wide, t) : -1;
-    const bool stored = slot >= 0 && slot < a.capacity;
+    const bool stored = slot >= 0 && slot < a.pool.pages << a.pool.page_shift;
     uint4 raw = make_uint4(0, 0, 0, 0);
-    if (stored) raw = *reinterpret_cast<const uint4*>(a.src[which] + t * a.tok[which] + h * a.head[which] + lane * 8);
-    const long long row = stored ? pool_row(slot, h, a.Hkv, a.page_shift) : 0;
+    if (stored) raw = *reinterpret_cast<const uint4*>(src + t * tok + h * head + lane * 8);
+    const long long row = stored ? pool_row(slot, h, a.pool.Hkv, a.pool.page_shift) : 0;
     if constexpr (F == kBf16) {
-      if (stored) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.dst[which]) + row * D + lane * 8) = raw;
+      if (stored) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(pool) + row * D + lane * 8) = raw;
     } else {
       const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
       float x[8];
@@ -104,42 +96,36 @@ __global__ void __launch_bounds__(THREADS) write_kernel(WriteArgs a) {
                                  : __int_as_float(0x7fc00000);
       const uint2 q = finite ? quantise8<F>(x, __frcp_rn(scale)) : make_uint2(0, 0);
       if (stored) {
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.dst[which]) + row * D + lane * 8) = q;
-        if (lane == 0) a.scale[which][row] = scale;
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + row * D + lane * 8) = q;
+        if (lane == 0) scales[row] = scale;
       }
     }
   }
 }
 
-struct ReadArgs {
-  const void* src[2];
-  const float* scale[2];
-  __nv_bfloat16* dst[2];  // [T, Hkv, D]
-  long long tok[2], head[2];
-  const void* slots;
-  long long T, capacity;
-  int Hkv, page_shift, wide;
-};
-
 template <int F, int D>
 __global__ void __launch_bounds__(THREADS) read_kernel(ReadArgs a) {
   constexpr int LANES = D / 8;
-  const long long rows = a.T * a.Hkv;
+  const long long rows = a.T * a.pool.Hkv;
   const int lane = threadIdx.x % LANES;
-  const int which = blockIdx.y;
+  const int which = blockIdx.y;  // 0: keys, 1: values
+  __nv_bfloat16* const dst = which ? a.dst[1] : a.dst[0];
+  const long long tok = which ? a.tok[1] : a.tok[0], head = which ? a.head[1] : a.head[0];
+  void* const pool = which ? a.pool.v : a.pool.k;
+  float* const scales = which ? a.pool.v_scale : a.pool.k_scale;
   const long long step = (long long)gridDim.x * (THREADS / LANES);
   for (long long r = (long long)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES; r < rows; r += step) {
-    const long long t = r / a.Hkv;
-    const int h = (int)(r - t * a.Hkv);
+    const long long t = r / a.pool.Hkv;
+    const int h = (int)(r - t * a.pool.Hkv);
     const long long slot = slot_of(a.slots, a.wide, t);
     uint4 out = make_uint4(0, 0, 0, 0);
-    if (slot >= 0 && slot < a.capacity) {
-      const long long row = pool_row(slot, h, a.Hkv, a.page_shift);
+    if (slot >= 0 && slot < a.pool.pages << a.pool.page_shift) {
+      const long long row = pool_row(slot, h, a.pool.Hkv, a.pool.page_shift);
       if constexpr (F == kBf16) {
-        out = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.src[which]) + row * D + lane * 8);
+        out = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(pool) + row * D + lane * 8);
       } else {
-        const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.src[which]) + row * D + lane * 8);
-        const float scale = a.scale[which][row];
+        const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pool) + row * D + lane * 8);
+        const float scale = scales[row];
         uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -151,88 +137,26 @@ __global__ void __launch_bounds__(THREADS) read_kernel(ReadArgs a) {
         out = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    *reinterpret_cast<uint4*>(a.dst[which] + t * a.tok[which] + h * a.head[which] + lane * 8) = out;
+    *reinterpret_cast<uint4*>(dst + t * tok + h * head + lane * 8) = out;
   }
 }
 
+static dim3 row_grid(long long rows, int D, int sms) {
+  const long long per_block = THREADS / (D / 8), blocks = (rows + per_block - 1) / per_block;
+  return dim3((unsigned)(blocks < sms * 8ll ? blocks : sms * 8ll), 2);
+}
+
+cudaError_t launch_write(const WriteArgs& a, int sms, cudaStream_t stream) {
+  const dim3 grid = row_grid(a.T * a.pool.Hkv, a.pool.D, sms);
+  by_format(a.pool, [&](auto f, auto d) { write_kernel<decltype(f)::value, decltype(d)::value><<<grid, THREADS, 0, stream>>>(a); });
+  return cudaGetLastError();
+}
+
+cudaError_t launch_read(const ReadArgs& a, int sms, cudaStream_t stream) {
+  const dim3 grid = row_grid(a.T * a.pool.Hkv, a.pool.D, sms);
+  by_format(a.pool, [&](auto f, auto d) { read_kernel<decltype(f)::value, decltype(d)::value><<<grid, THREADS, 0, stream>>>(a); });
+  return cudaGetLastError();
+}
+
 }  // namespace kv
-
-static void check_rows(const at::Tensor& x, const char* name, int64_t heads, int64_t dim) {
-  HT_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() == 3 && x.size(1) == heads && x.size(2) == dim, name,
-           " must be a CUDA bf16 tensor [T, ", heads, ", ", dim, "]");
-}
-
-static void check_slots(const at::Tensor& slots, const at::Tensor& rows) {
-  HT_CHECK(slots.is_cuda() && slots.device() == rows.device() && (slots.scalar_type() == at::kLong || slots.scalar_type() == at::kInt) &&
-               slots.dim() == 1 && slots.size(0) == rows.size(0),
-           "slots must be an int32 or int64 tensor of one slot per token, on the rows' device");
-}
-
-static bool vector_rows(const at::Tensor& x) {
-  return x.stride(2) == 1 && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
-}
-
-static dim3 row_grid(long long rows, int D) {
-  const int per_block = kv::THREADS / (D / 8);
-  return dim3((unsigned)std::max(1ll, std::min((rows + per_block - 1) / per_block, (long long)num_sms() * 8)), 2);
-}
-
-void kv_cache_write(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale, c10::optional<at::Tensor> v_scale,
-                    at::Tensor k, at::Tensor v, at::Tensor slots) {
-  const c10::cuda::CUDAGuard guard(k_pool.device());
-  const kv::Pool p = kv::checked_pool(k_pool, v_pool, k_scale, v_scale);
-  check_rows(k, "k", p.Hkv, p.D);
-  check_rows(v, "v", p.Hkv, p.D);
-  HT_CHECK(k.size(0) == v.size(0) && k.device() == k_pool.device() && v.device() == k_pool.device(),
-           "k and v must hold the same tokens, on the pool's device");
-  check_slots(slots, k);
-  if (k.size(0) == 0) return;
-  // rows that a 16-byte load cannot take (another order or alignment) are copied first
-  if (!vector_rows(k)) k = k.clone(at::MemoryFormat::Contiguous);
-  if (!vector_rows(v)) v = v.clone(at::MemoryFormat::Contiguous);
-  slots = slots.contiguous();
-  kv::WriteArgs a{{reinterpret_cast<const __nv_bfloat16*>(k.data_ptr()), reinterpret_cast<const __nv_bfloat16*>(v.data_ptr())},
-                  {k.stride(0), v.stride(0)},
-                  {k.stride(1), v.stride(1)},
-                  {p.k, p.v},
-                  {p.k_scale, p.v_scale},
-                  slots.data_ptr(),
-                  k.size(0),
-                  (long long)p.pages << p.page_shift,
-                  p.Hkv,
-                  p.page_shift,
-                  slots.scalar_type() == at::kLong};
-  const dim3 grid = row_grid(a.T * a.Hkv, p.D);
-  kv::by_format(p, [&](auto f, auto d) { kv::write_kernel<decltype(f)::value, decltype(d)::value><<<grid, kv::THREADS, 0, stream()>>>(a); });
-  HT_CUDA_CHECK(cudaGetLastError());
-}
-
-void kv_cache_read(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale, c10::optional<at::Tensor> v_scale,
-                   at::Tensor slots, at::Tensor k, at::Tensor v) {
-  const c10::cuda::CUDAGuard guard(k_pool.device());
-  const kv::Pool p = kv::checked_pool(k_pool, v_pool, k_scale, v_scale);
-  check_rows(k, "k", p.Hkv, p.D);
-  check_rows(v, "v", p.Hkv, p.D);
-  HT_CHECK(k.size(0) == v.size(0) && k.device() == k_pool.device() && v.device() == k_pool.device(),
-           "k and v must hold the same tokens, on the pool's device");
-  check_slots(slots, k);
-  if (k.size(0) == 0) return;
-  HT_CHECK(vector_rows(k) && vector_rows(v), "k and v must have unit inner stride and rows on 16-byte boundaries");
-  slots = slots.contiguous();
-  kv::ReadArgs a{{p.k, p.v},
-                 {p.k_scale, p.v_scale},
-                 {reinterpret_cast<__nv_bfloat16*>(k.data_ptr()), reinterpret_cast<__nv_bfloat16*>(v.data_ptr())},
-                 {k.stride(0), v.stride(0)},
-                 {k.stride(1), v.stride(1)},
-                 slots.data_ptr(),
-                 k.size(0),
-                 (long long)p.pages << p.page_shift,
-                 p.Hkv,
-                 p.page_shift,
-                 slots.scalar_type() == at::kLong};
-  const dim3 grid = row_grid(a.T * a.Hkv, p.D);
-  kv::by_format(p, [&](auto f, auto d) { kv::read_kernel<decltype(f)::value, decltype(d)::value><<<grid, kv::THREADS, 0, stream()>>>(a); });
-  HT_CUDA_CHECK(cudaGetLastError());
-}
-
 }  // namespace ht

@@ -6,104 +6,712 @@
 // A sequence without tokens gives o = 0 and lse = -inf.  Tokens in pages that lie outside the pool
 // count as masked, lengths beyond the table are cut to it.
 //
-// One warp per (sequence, query head), the head's dimensions spread over the lanes, one pass over
-// the tokens with the running maximum and sum of the softmax in fp32.
-#include "common.cuh"
+// Bound: memory.  Every cached byte is needed once and meets 2 * (heads per key/value head) flops per
+// element, so the kernel is built around keeping loads in flight:
+//
+// * Work.  A *row* is one sequence and one key/value head with up to 8 of its query heads (a larger
+//   group makes further rows, which read the same keys and values again).  All rows' tiles of TOK tokens
+//   form one line, cut into equal ranges per block and, inside a block, per warp, whatever the lengths:
+//   one persistent block per SM, no idle SM for ragged batches, long rows split without a plan on the
+//   host.  Every warp streams its range through a ring of its own in shared memory with 16-byte
+//   cp.async; warps never wait for one another before their range is done.
+// * Matrix instructions.  S = Q K^T and O += P V are m16n8k16 with the 8 heads as rows 0-7: at these
+//   intensities the tensor pipe is far from its limit, and a tile of 16 rows is the smallest there is.
+//   Rows 8-15 are not wasted: in the second product they carry what rounding P to 16 bits left over, so
+//   P enters with 16 (bf16) or 22 (fp16) significant bits at no extra instruction.  The dimensions of q and
+//   k are summed in the order in which 16-byte loads deliver them (the order of a dot product is free),
+//   so 8-bit keys go from shared memory to the instruction's fragments with byte permutes alone.
+// * 8 bits.  int8 and e4m3 values are exact in fp16, and q is scaled by a power of two per head so that
+//   its bf16 values are exact there too (down to 2^-24 of the head's largest).  A token's key scale
+//   multiplies its score.  Its value scale sv joins the exponent: with s'_t = s_t + log2(sv_t), the running
+//   maximum m of s' and p_t = 2^(s'_t - m) <= 1, the output is sum p_t v_t / sum (p_t / sv_t): p fits fp16
+//   whatever the scales are.
+// * Joining.  A row inside one warp's range is finished by that warp.  Otherwise warps leave (o, m, sum)
+//   in shared memory, the block merges neighbours, and rows that cross blocks go through a workspace:
+//   the block that arrives last merges the pieces in the order of the tokens, so results do not depend
+//   on timing.  One launch, no second kernel.
+#include <algorithm>
 
-#include "kv_cache.cuh"
+#include "generation.cuh"
 
 namespace ht {
 namespace paged {
 
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
+constexpr int HEADS = 8;  // query heads of one row
 
-struct Args {
-  const __nv_bfloat16* q;  // [B, H, D]
-  long long q_seq, q_head;
-  kv::Pool pool;
-  const int* table;  // [B, width]
-  long long table_row;
-  int width;
-  const int* lengths;
-  __nv_bfloat16* out;  // [B, H, D]
-  float* lse;          // [B, H] or null
-  int B, H;
-  float scale_log2;
+template <int F, int D>
+struct Shape {
+  static constexpr int ROW = D * (F == kv::kBf16 ? 2 : 1);  // bytes of one key
+  static constexpr int TOK = ROW == 256 ? 16 : 32;          // tokens of one tile
+  static constexpr int WARPS = 8;
+  static constexpr int DATA = TOK * ROW, SCALES = F == kv::kBf16 ? 0 : TOK * 4;
+  static constexpr int STAGE = 2 * (DATA + SCALES);
+  static constexpr int STAGES = STAGE > 8192 ? 2 : STAGE == 8192 ? 3 : 4;
+  static constexpr int PIECE = HEADS * (D + 2) * 4;  // o, m and sum of one row's piece
+  static constexpr int THREADS = WARPS * 32;
+  static constexpr int SMEM = WARPS * (STAGES * STAGE + PIECE) + 1024;
 };
 
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// 16 bytes, or zeros without reading `src`.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void ldmatrix4t(uint32_t* r, uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+
 template <int F>
-__device__ __forceinline__ float element(const void* pool, long long i) {
-  if constexpr (F == kv::kBf16) return __bfloat162float(static_cast<const __nv_bfloat16*>(pool)[i]);
-  if constexpr (F == kv::kInt8) return (float)static_cast<const int8_t*>(pool)[i];
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const __nv_fp8_storage_t*>(pool)[i], __NV_E4M3)));
+__device__ __forceinline__ void mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (F == kv::kBf16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Two 8-bit values (the bytes `SEL` of x) as a pair of fp16.  int8: x holds value + 128 as a byte u, and the fp16 with
+// bits 0x6400 | u is 1024 + u, so one subtraction gives the value exactly.
+template <int F, int PAIR>
+__device__ __forceinline__ uint32_t half_pair(uint32_t x) {
+  if constexpr (F == kv::kInt8) {
+    const uint32_t biased = __byte_perm(x, 0x64646464u, PAIR == 0 ? 0x4140 : 0x4342);
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2_raw v = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(PAIR == 0 ? x & 0xffffu : x >> 16), __NV_E4M3);
+    return (uint32_t)v.x | ((uint32_t)v.y << 16);
+  }
+}
+template <int F>
+__device__ __forceinline__ uint32_t unsign(uint32_t x) {
+  return F == kv::kInt8 ? x ^ 0x80808080u : x;
+}
+
+template <int F>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  if constexpr (F == kv::kBf16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <int F>
+__device__ __forceinline__ float2 unpack(uint32_t x) {
+  if constexpr (F == kv::kBf16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A place on the line of tiles.  `rows` counts the rows of one sequence.
+struct Cursor {
+  int b, row, tile, tiles, n;
+};
+
+// Tokens of sequence b that the kernel attends to.
+__device__ __forceinline__ int tokens_of(const Args& a, int b) {
+  const long long most = (long long)a.width << a.pool.page_shift;
+  const int n = max(a.lengths[b], 0);
+  return n < most ? n : (int)most;
+}
+
+template <int TOK>
+__device__ __forceinline__ void open_row(const Args& a, Cursor& c) {
+  c.n = tokens_of(a, c.b);
+  c.tiles = (c.n + TOK - 1) / TOK;
+}
+
+template <int TOK>
+__device__ __forceinline__ void advance(const Args& a, Cursor& c, int rows) {
+  if (++c.tile < c.tiles) return;
+  c.tile = 0;
+  if (++c.row < rows) return;
+  c.row = 0;
+  do {
+    if (++c.b >= a.B) return;
+    open_row<TOK>(a, c);
+  } while (c.tiles == 0);
 }
 
 template <int F, int D>
-__global__ void __launch_bounds__(128) decode_kernel(Args a) {
-  constexpr int E = D / 32;
-  const int item = blockIdx.x * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (item >= a.B * a.H) return;
-  const int b = item / a.H, h = item % a.H, g = h / (a.H / a.pool.Hkv);
-  const long long n = min((long long)max(a.lengths[b], 0), (long long)a.width << a.pool.page_shift);
-  float q[E], o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = bf2f(a.q[b * a.q_seq + h * a.q_head + e * 32 + lane]);
-    o[e] = 0.f;
+__global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const Args a) {
+  using S = Shape<F, D>;
+  constexpr int TOK = S::TOK, GROUPS = TOK / 16, NT = D / 8, WARPS = S::WARPS;
+  extern __shared__ __align__(16) unsigned char smem[];
+  struct Meta {
+    long long item;  // first tile of the row on the line
+    int b, row, tile, count, tiles;
+  };
+  struct Shared {
+    Meta meta[WARPS][2];
+    long long scan[WARPS];
+    Cursor start[WARPS];
+    int head_of[2 * WARPS + 1];
+    int groups;
+    int join_first[2], join_count[2], join_b[2], join_row[2];
+  };
+  static_assert(sizeof(Shared) <= 1024, "shared bookkeeping");
+  unsigned char* const rings = smem;
+  unsigned char* const pieces = smem + WARPS * S::STAGES * S::STAGE;
+  Shared& sh = *reinterpret_cast<Shared*>(pieces + WARPS * S::PIECE);
+
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int g = lane / 4, c4 = lane % 4;
+  const int group = a.H / a.pool.Hkv;               // query heads per key/value head
+  const int chunks = (group + HEADS - 1) / HEADS;  // rows per key/value head
+  const int rows = a.pool.Hkv * chunks;
+
+  // ---- sequences without tokens
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    if (tokens_of(a, b) > 0) continue;
+    for (int i = tid; i < a.H * D; i += S::THREADS) a.out[(long long)b * a.H * D + i] = __float2bfloat16_rn(0.f);
+    if (a.lse != nullptr)
+      for (int i = tid; i < a.H; i += S::THREADS) a.lse[(long long)b * a.H + i] = -INFINITY;
   }
-  float m = -INFINITY, l = 0.f;
-  for (long long t = 0; t < n; ++t) {
-    const int page = a.table[b * a.table_row + (t >> a.pool.page_shift)];
-    if (page < 0 || page >= a.pool.pages) continue;
-    const long long row = (((long long)page * a.pool.Hkv + g) << a.pool.page_shift) + (t & ((1 << a.pool.page_shift) - 1));
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s += q[e] * element<F>(a.pool.k, row * D + e * 32 + lane);
-    s = warp_sum(s) * a.scale_log2 * (F == kv::kBf16 ? 1.f : a.pool.k_scale[row]);
-    const float top = fmaxf(m, s);
-    const float keep = top == -INFINITY ? 1.f : exp2f(m - top), p = top == -INFINITY ? 0.f : exp2f(s - top);
-    const float pv = p * (F == kv::kBf16 ? 1.f : a.pool.v_scale[row]);
-    m = top;
-    l = l * keep + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * keep + pv * element<F>(a.pool.v, row * D + e * 32 + lane);
+
+  // ---- this block's and its warps' ranges of the line
+  const auto block_sum = [&](long long v) {
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if (lane == 0) sh.scan[warp] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < WARPS; ++w) v += sh.scan[w];
+    return v;
+  };
+  long long mine = 0;
+  for (int b = tid; b < a.B; b += S::THREADS) mine += (tokens_of(a, b) + TOK - 1) / TOK;
+  const long long line = block_sum(mine) * rows;
+  // at least one tile for each warp of a block: fewer, fuller blocks have fewer pieces to join
+  const long long per_block = max((line + gridDim.x - 1) / gridDim.x, (long long)WARPS);
+  const long long block_from = min(line, per_block * blockIdx.x), block_to = min(line, block_from + per_block);
+  if (block_from >= block_to) return;
+  const long long per_warp = (block_to - block_from + WARPS - 1) / WARPS;
+  if (tid < 2 * WARPS) sh.meta[tid / 2][tid % 2].count = 0;
+  {
+    long long base = 0;  // tiles of the sequences before this chunk of them
+    for (int b0 = 0; b0 < a.B && base < block_to; b0 += S::THREADS) {
+      const int b = b0 + tid;
+      const int n = b < a.B ? tokens_of(a, b) : 0;
+      const long long tiles = (long long)((n + TOK - 1) / TOK) * rows;
+      long long upto = tiles;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long other = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += other;
+      }
+      __syncthreads();
+      if (lane == 31) sh.scan[warp] = upto;
+      __syncthreads();
+      long long total = 0;
+      for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) upto += sh.scan[w];
+        total += sh.scan[w];
+      }
+      const long long from = base + upto - tiles, to = base + upto;
+      for (int w = 0; w < WARPS; ++w) {
+        const long long at = block_from + w * per_warp;
+        if (at >= from && at < to) {
+          const int per_row = (n + TOK - 1) / TOK;
+          const long long in = at - from;
+          sh.start[w] = Cursor{b, (int)(in / per_row), (int)(in % per_row), per_row, n};
+        }
+      }
+      base += total;
+    }
   }
+  __syncthreads();
+
+  const long long from = block_from + warp * per_warp;
+  const int count = (int)max(0ll, min(per_warp, block_to - from));
+  unsigned char* const ring = rings + warp * S::STAGES * S::STAGE;
+  const uint32_t ring_addr = smem_addr(ring);
+
+  if (count > 0) {
+    Cursor load = sh.start[warp], use = load;
+    int to_load = count;
+    uint32_t held = 0;  // per stage: which groups of 16 tokens are in the pool
+    int page = -1;      // lane i < GROUPS: page of the tile's group i
+    const auto look_up = [&] {
+      const int token = load.tile * TOK + lane * 16;
+      page = -1;
+      if (to_load > 0 && lane < GROUPS && token < load.n) page = a.table[load.b * a.table_row + (token >> a.pool.page_shift)];
+    };
+    const auto issue = [&](int stage) {
+      if (to_load > 0) {
+        const uint32_t base = ring_addr + stage * S::STAGE;
+        uint32_t bits = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) a.out[(long long)item * D + e * 32 + lane] = f2bf(l > 0.f ? o[e] / l : (l == 0.f ? 0.f : l));
-  if (lane == 0 && a.lse != nullptr) a.lse[item] = l > 0.f ? m * LN2 + logf(l) : (l == 0.f ? -INFINITY : l);
+        for (int i = 0; i < GROUPS; ++i) {
+          const int p = __shfl_sync(0xffffffffu, page, i);
+          const int token = load.tile * TOK + i * 16;
+          const bool in_pool = p >= 0 && p < a.pool.pages;
+          bits |= (uint32_t)in_pool << i;
+          const long long first =
+              in_pool ? (((long long)p * a.pool.Hkv + load.row / chunks) << a.pool.page_shift) + (token & ((1 << a.pool.page_shift) - 1)) : 0;
+          const int real = in_pool ? load.n - token : 0;  // rows behind the sequence become zeros: 0 * NaN would not be 0
+          const unsigned char* ks = static_cast<const unsigned char*>(a.pool.k) + first * S::ROW;
+          const unsigned char* vs = static_cast<const unsigned char*>(a.pool.v) + first * S::ROW;
+#pragma unroll
+          for (int j = 0; j < S::ROW / 32; ++j) {
+            constexpr int PER = S::ROW / 16;  // 16-byte pieces of a row
+            const int q = j * 32 + lane, r = q / PER, ch = q % PER;
+            const int kch = PER >= 8 ? ch ^ ((r & 1) << 2) : ch;
+            const int vch = F == kv::kBf16 ? ch ^ (r & 7) : PER >= 8 ? ch ^ (((r >> 1) & 3) << 1) : ch;
+            copy16(base + (i * 16 + r) * S::ROW + kch * 16, ks + q * 16, r < real);
+            copy16(base + S::DATA + (i * 16 + r) * S::ROW + vch * 16, vs + q * 16, r < real);
+          }
+          if (F != kv::kBf16 && lane < 8) {
+            const float* scales = (lane < 4 ? a.pool.k_scale : a.pool.v_scale) + first;
+            copy16(base + 2 * S::DATA + (lane < 4 ? 0 : S::SCALES) + i * 64 + (lane & 3) * 16, scales + (lane & 3) * 4, in_pool);
+          }
+        }
+        held = (held & ~(0xfu << (4 * stage))) | (bits << (4 * stage));
+        advance<TOK>(a, load, rows);
+        --to_load;
+        look_up();
+      }
+      copies_commit();
+    };
+
+    look_up();
+#pragma unroll
+    for (int s = 0; s < S::STAGES - 1; ++s) issue(s);
+
+    // Per row: q as fragments of the first operand, the output's accumulators, and the softmax's state.
+    constexpr int QR = D / 8;  // registers of q
+    uint32_t q[QR];
+    float o[NT][4], m = -INFINITY, sum = 0.f, factor = 0.f;
+    int row_tile = 0;          // the row's first tile in this warp
+    bool opened = false, first_row = true;
+    int stage = 0;
+    long long row_start = from - use.tile;  // first tile of the row on the line
+
+    for (int i = 0; i < count; ++i) {
+      if (!opened) {
+        opened = true;
+        row_tile = use.tile;
+        m = -INFINITY;
+        sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+        const int in_group = (use.row % chunks) * HEADS + g;
+        const bool real = in_group < group;
+        const __nv_bfloat16* src = a.q + use.b * a.q_seq + ((long long)(use.row / chunks) * group + in_group) * a.q_head;
+        // lane (g, c4) holds, of head g, the 16-byte pieces of a key row that it will load: piece 4 j + c4
+        if constexpr (F == kv::kBf16) {
+          factor = a.scale_log2;
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            const uint4 x = real ? *reinterpret_cast<const uint4*>(src + (j * 4 + c4) * 8) : make_uint4(0, 0, 0, 0);
+            q[4 * j] = x.x, q[4 * j + 1] = x.y, q[4 * j + 2] = x.z, q[4 * j + 3] = x.w;
+          }
+        } else {
+          float top = 0.f;
+#pragma unroll
+          for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint4 x = real ? *reinterpret_cast<const uint4*>(src + (j * 4 + c4) * 16 + h * 8) : make_uint4(0, 0, 0, 0);
+              uint32_t* to = q + 8 * j + 4 * h;
+              to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float2 f = unpack<kv::kBf16>(to[r]);
+                top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+              }
+            }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          // the power of two that brings the largest magnitude into [1, 2): exact both ways
+          const int exponent = max(-126, min(126, (int)(__float_as_uint(top) >> 23) - 127));
+          const float down = __uint_as_float((uint32_t)(127 - exponent) << 23), up = __uint_as_float((uint32_t)(127 + exponent) << 23);
+#pragma unroll
+          for (int r = 0; r < QR; ++r) {
+            const float2 f = unpack<kv::kBf16>(q[r]);
+            q[r] = pack<F>(f.x * down, f.y * down);
+          }
+          factor = a.scale_log2 * up;
+        }
+      }
+
+      copies_wait<S::STAGES - 2>();
+      __syncwarp();
+      {
+        int next = stage + S::STAGES - 1;
+        if (next >= S::STAGES) next -= S::STAGES;
+        issue(next);
+      }
+      const uint32_t kb = ring_addr + stage * S::STAGE, vb = kb + S::DATA, sb = kb + 2 * S::DATA;
+      const uint32_t in_pool = held >> (4 * stage);
+
+      // scores, in the accumulator's layout: head g, tokens 8 t + 2 c4 and + 1
+      float s[TOK / 8][2], inv[TOK / 8][2];
+      float top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < TOK / 8; ++t) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint32_t row = kb + (t * 8 + g) * S::ROW;
+        if constexpr (F == kv::kBf16) {
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            const uint4 k = lds128(row + (((j * 4 + c4) ^ ((g & 1) << 2)) * 16));
+            mma<F>(acc, q[4 * j], 0u, q[4 * j + 1], 0u, k.x, k.y);
+            mma<F>(acc, q[4 * j + 2], 0u, q[4 * j + 3], 0u, k.z, k.w);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < D / 64; ++j) {
+            const uint4 k = lds128(row + ((D == 128 ? (j * 4 + c4) ^ ((g & 1) << 2) : c4) * 16));
+            const uint32_t w[4] = {unsign<F>(k.x), unsign<F>(k.y), unsign<F>(k.z), unsign<F>(k.w)};
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              mma<F>(acc, q[8 * j + 2 * r], 0u, q[8 * j + 2 * r + 1], 0u, half_pair<F, 0>(w[r]), half_pair<F, 1>(w[r]));
+          }
+        }
+        float2 ks = make_float2(1.f, 1.f), shift = make_float2(0.f, 0.f);
+        inv[t][0] = inv[t][1] = 1.f;
+        if constexpr (F != kv::kBf16) {
+          const uint2 kw = lds64(sb + (t * 8 + 2 * c4) * 4), vw = lds64(sb + S::SCALES + (t * 8 + 2 * c4) * 4);
+          ks = make_float2(__uint_as_float(kw.x), __uint_as_float(kw.y));
+          // a scale of zero (none that kv_cache_write leaves) counts as the smallest one; NaN stays NaN
+          const float v0 = __uint_as_float(vw.x), v1 = __uint_as_float(vw.y);
+          const float s0 = v0 < kv::kMinScale ? kv::kMinScale : v0, s1 = v1 < kv::kMinScale ? kv::kMinScale : v1;
+          shift = make_float2(fast_log2(s0), fast_log2(s1));
+          inv[t][0] = __frcp_rn(s0);
+          inv[t][1] = __frcp_rn(s1);
+        }
+        const int token = use.tile * TOK + t * 8 + 2 * c4;
+        const bool pool_ok = (in_pool >> (t / 2)) & 1u;
+        s[t][0] = pool_ok && token < use.n ? acc[0] * factor * ks.x + shift.x : -INFINITY;
+        s[t][1] = pool_ok && token + 1 < use.n ? acc[1] * factor * ks.y + shift.y : -INFINITY;
+        top = fmaxf(top, fmaxf(s[t][0], s[t][1]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float higher = fmaxf(m, top);
+      const float at = higher == -INFINITY ? 0.f : higher;  // nothing but masked tokens so far
+      if (__any_sync(0xffffffffu, higher > m)) {
+        const float keep = fast_exp2(m - at);
+        sum *= keep;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          o[t][0] *= keep, o[t][1] *= keep, o[t][2] *= keep, o[t][3] *= keep;
+        }
+        m = higher;
+      }
+#pragma unroll
+      for (int t = 0; t < TOK / 8; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bool masked = s[t][e] == -INFINITY;
+          const float p = masked ? 0.f : fast_exp2(s[t][e] - at);
+          sum += F == kv::kBf16 ? p : masked ? 0.f : p * inv[t][e];
+          s[t][e] = p;
+        }
+
+      // o += p v, the rounding's remainder of p in rows 8 to 15
+#pragma unroll
+      for (int kk = 0; kk < GROUPS; ++kk) {
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float x = s[2 * kk + h][0], y = s[2 * kk + h][1];
+          hi[h] = pack<F>(x, y);
+          const float2 back = unpack<F>(hi[h]);
+          lo[h] = pack<F>(x - back.x, y - back.y);
+        }
+        if constexpr (F == kv::kBf16) {
+          const int mat = lane / 8, r = kk * 16 + (mat & 1) * 8 + (lane & 7);
+          const uint32_t row = vb + r * S::ROW;
+#pragma unroll
+          for (int np = 0; np < NT / 2; ++np) {
+            uint32_t v[4];
+            ldmatrix4t(v, row + (((2 * np + (mat >> 1)) ^ (r & 7)) * 16));
+            mma<F>(o[2 * np], hi[0], lo[0], hi[1], lo[1], v[0], v[1]);
+            mma<F>(o[2 * np + 1], hi[0], lo[0], hi[1], lo[1], v[2], v[3]);
+          }
+        } else {
+          // lane (g, c4) takes dimensions g * NT ... + NT - 1 of the tokens 2 c4, 2 c4 + 1, 2 c4 + 8, 2 c4 + 9
+          constexpr int WORDS = NT / 4;
+          uint32_t w[4][WORDS];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int r = kk * 16 + 2 * c4 + (x & 1) + (x >> 1) * 8;
+            if constexpr (D == 128) {
+              const uint4 v = lds128(vb + r * S::ROW + ((g ^ (((r >> 1) & 3) << 1)) * 16));
+              w[x][0] = unsign<F>(v.x), w[x][1] = unsign<F>(v.y), w[x][2] = unsign<F>(v.z), w[x][3] = unsign<F>(v.w);
+            } else {
+              const uint2 v = lds64(vb + r * S::ROW + g * 8);
+              w[x][0] = unsign<F>(v.x), w[x][1] = unsign<F>(v.y);
+            }
+          }
+#pragma unroll
+          for (int y = 0; y < WORDS; ++y) {
+            const uint32_t a01 = __byte_perm(w[0][y], w[1][y], 0x5140), a23 = __byte_perm(w[0][y], w[1][y], 0x7362);
+            const uint32_t b01 = __byte_perm(w[2][y], w[3][y], 0x5140), b23 = __byte_perm(w[2][y], w[3][y], 0x7362);
+            mma<F>(o[4 * y], hi[0], lo[0], hi[1], lo[1], half_pair<F, 0>(a01), half_pair<F, 0>(b01));
+            mma<F>(o[4 * y + 1], hi[0], lo[0], hi[1], lo[1], half_pair<F, 1>(a01), half_pair<F, 1>(b01));
+            mma<F>(o[4 * y + 2], hi[0], lo[0], hi[1], lo[1], half_pair<F, 0>(a23), half_pair<F, 0>(b23));
+            mma<F>(o[4 * y + 3], hi[0], lo[0], hi[1], lo[1], half_pair<F, 1>(a23), half_pair<F, 1>(b23));
+          }
+        }
+      }
+      __syncwarp();  // the stage may be refilled
+      if (++stage == S::STAGES) stage = 0;
+
+      const bool row_ends = use.tile + 1 == use.tiles, last = i + 1 == count;
+      if (row_ends || last) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        // where accumulator column n of tile t lies in the head's dimensions
+        const auto dim = [&](int t, int e) { return F == kv::kBf16 ? t * 8 + 2 * c4 + e : (2 * c4 + e) * NT + t; };
+        if (row_ends && row_tile == 0) {
+          const int in_group = (use.row % chunks) * HEADS + g;
+          if (in_group < group) {
+            const long long head = (long long)use.b * a.H + (use.row / chunks) * group + in_group;
+            const float norm = sum == 0.f ? 0.f : 1.f / sum;
+            __nv_bfloat16* dst = a.out + head * D;
+            if constexpr (F == kv::kBf16) {
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+                *reinterpret_cast<uint32_t*>(dst + dim(t, 0)) = pack<kv::kBf16>((o[t][0] + o[t][2]) * norm, (o[t][1] + o[t][3]) * norm);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int t = 0; t < NT; t += 8) {
+                  uint32_t x[4];
+#pragma unroll
+                  for (int y = 0; y < 4; ++y)
+                    x[y] = pack<kv::kBf16>((o[t + 2 * y][e] + o[t + 2 * y][e + 2]) * norm, (o[t + 2 * y + 1][e] + o[t + 2 * y + 1][e + 2]) * norm);
+                  *reinterpret_cast<uint4*>(dst + dim(t, e)) = make_uint4(x[0], x[1], x[2], x[3]);
+                }
+            }
+            if (a.lse != nullptr && c4 == 0) a.lse[head] = sum == 0.f ? -INFINITY : (m + fast_log2(sum)) * LN2;
+          }
+        } else {
+          // A piece of a row.  One of the warp's first row goes to a place of its own, one of a later row ends the
+          // range, so that the ring is free for it.
+          const int which = first_row ? 0 : 1;
+          if (which == 1) {
+            copies_wait<0>();
+            __syncwarp();
+          }
+          float* const piece = reinterpret_cast<float*>(which == 0 ? pieces + warp * S::PIECE : ring);
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) piece[g * D + dim(t, e)] = o[t][e] + o[t][e + 2];
+          if (c4 == 0) {
+            piece[HEADS * D + g] = m;
+            piece[HEADS * D + HEADS + g] = sum;
+          }
+          if (lane == 0) sh.meta[warp][which] = Meta{row_start, use.b, use.row, row_tile, use.tile + 1 - row_tile, use.tiles};
+          __syncwarp();
+        }
+        opened = first_row = false;
+        row_start = from + i + 1;
+      }
+      advance<TOK>(a, use, rows);
+    }
+    copies_wait<0>();
+  }
+  __syncthreads();
+
+  // ---- pieces of the same row are neighbours: merge them
+  if (warp == 0) {
+    const bool some = lane < 2 * WARPS && sh.meta[lane / 2 % WARPS][lane % 2].count > 0;
+    const long long item = some ? sh.meta[lane / 2][lane % 2].item : -1;
+    const uint32_t have = __ballot_sync(0xffffffffu, some), before = have & ((1u << lane) - 1);
+    const long long previous = __shfl_sync(0xffffffffu, item, before ? 31 - __clz(before) : 0);
+    const bool head = some && (before == 0 || previous != item);
+    const uint32_t heads = __ballot_sync(0xffffffffu, head);
+    if (head) sh.head_of[__popc(heads & ((1u << lane) - 1))] = lane;
+    if (lane == 0) {
+      sh.groups = __popc(heads);
+      sh.head_of[__popc(heads)] = 2 * WARPS;
+      sh.join_count[0] = sh.join_count[1] = 0;
+    }
+  }
+  __syncthreads();
+  const int real_heads = min(group, HEADS), columns = real_heads * D;
+  const auto piece_of = [&](int i) {
+    return reinterpret_cast<const float*>(i % 2 == 0 ? pieces + i / 2 * S::PIECE : rings + i / 2 * S::STAGES * S::STAGE);
+  };
+  const auto ends_of = [&](int gi, Meta& first, Meta& last) {  // the group's first and last piece
+    first = sh.meta[sh.head_of[gi] / 2][sh.head_of[gi] % 2];
+    last = first;
+    for (int i = sh.head_of[gi] + 1; i < sh.head_of[gi + 1]; ++i)
+      if (sh.meta[i / 2][i % 2].count > 0) last = sh.meta[i / 2][i % 2];
+  };
+  const auto finish = [&](const Meta& row, int h, int d, float value, float top, float total) {
+    const int in_group = row.row % chunks * HEADS + h;
+    if (in_group >= group) return;
+    const long long head = (long long)row.b * a.H + (long long)(row.row / chunks) * group + in_group;
+    a.out[head * D + d] = __float2bfloat16_rn(total == 0.f ? 0.f : value / total);
+    if (d == 0 && a.lse != nullptr) a.lse[head] = total == 0.f ? -INFINITY : (top + fast_log2(total)) * LN2;
+  };
+  for (int x = tid; x < sh.groups * columns; x += S::THREADS) {
+    const int gi = x / columns, h = x % columns / D, d = x % D;
+    float top = -INFINITY, value = 0.f, total = 0.f;
+    for (int i = sh.head_of[gi]; i < sh.head_of[gi + 1]; ++i)
+      if (sh.meta[i / 2][i % 2].count > 0) top = fmaxf(top, piece_of(i)[HEADS * D + h]);
+    const float at = top == -INFINITY ? 0.f : top;
+    for (int i = sh.head_of[gi]; i < sh.head_of[gi + 1]; ++i)
+      if (sh.meta[i / 2][i % 2].count > 0) {
+        const float* p = piece_of(i);
+        const float w = fast_exp2(p[HEADS * D + h] - at);
+        value += w * p[h * D + d];
+        total += w * p[HEADS * D + HEADS + h];
+      }
+    Meta first, last;
+    ends_of(gi, first, last);
+    if (first.tile == 0 && last.tile + last.count == last.tiles) {
+      finish(first, h, d, value, top, total);
+    } else {
+      float* out = a.partial + ((long long)blockIdx.x * 2 + (first.tile > 0 ? 0 : 1)) * (HEADS * (D + 2));
+      out[h * D + d] = value;
+      if (d == 0) {
+        out[HEADS * D + h] = top;
+        out[HEADS * D + HEADS + h] = total;
+      }
+    }
+  }
+
+  // ---- rows that cross blocks: the last block to arrive joins them.  A row that goes on behind its first block is that
+  // block's last one, so the block's number names the counter.
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    int joins = 0;
+    for (int gi = 0; gi < sh.groups; gi += max(1, sh.groups - 1)) {
+      Meta first, last;
+      ends_of(gi, first, last);
+      if (first.tile == 0 && last.tile + last.count == last.tiles) continue;
+      const int b0 = (int)(first.item / per_block), b1 = (int)((first.item + first.tiles - 1) / per_block);
+      if (atomicAdd(a.arrived + b0, 1u) == (unsigned)(b1 - b0)) {
+        a.arrived[b0] = 0;
+        sh.join_first[joins] = b0;
+        sh.join_count[joins] = b1 - b0 + 1;
+        sh.join_b[joins] = first.b;
+        sh.join_row[joins++] = first.row;
+      }
+    }
+  }
+  __syncthreads();
+  for (int join = 0; join < 2; ++join) {
+    const int n = sh.join_count[join];
+    if (n == 0) break;
+    __threadfence();
+    const auto part = [&](int j) {
+      return a.partial + ((long long)(sh.join_first[join] + j) * 2 + (j == 0 ? 1 : 0)) * (HEADS * (D + 2));
+    };
+    float* const weights = reinterpret_cast<float*>(rings);  // [n][HEADS], then the heads' tops and totals, then the columns
+    float* const tops = weights + n * HEADS;
+    float* const sums = tops + 2 * HEADS;
+    if (warp < real_heads) {  // one warp per head
+      float top = -INFINITY, total = 0.f;
+      for (int j = lane; j < n; j += 32) top = fmaxf(top, __ldcg(part(j) + HEADS * D + warp));
+      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float at = top == -INFINITY ? 0.f : top;
+      for (int j = lane; j < n; j += 32) {
+        const float w = fast_exp2(__ldcg(part(j) + HEADS * D + warp) - at);
+        weights[j * HEADS + warp] = w;
+        total += w * __ldcg(part(j) + HEADS * D + HEADS + warp);
+      }
+      for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+      if (lane == 0) {
+        tops[warp] = top;
+        tops[HEADS + warp] = total;
+      }
+    }
+    __syncthreads();
+    const int quads = columns / 4, copies = S::THREADS / quads;  // 8 heads of 128 make 256 quads: one per thread
+    const int quad = tid % quads, copy = tid / quads;
+    if (copy < copies) {
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      const int h = quad * 4 / D;
+#pragma unroll 4
+      for (int j = copy; j < n; j += copies) {
+        const float w = weights[j * HEADS + h];
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(part(j)) + quad);
+        acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
+      }
+      reinterpret_cast<float4*>(sums)[copy * quads + quad] = acc;
+    }
+    __syncthreads();
+    const Meta row{0, sh.join_b[join], sh.join_row[join], 0, 0, 0};
+    for (int x = tid; x < columns; x += S::THREADS) {
+      float value = 0.f;
+      for (int y = 0; y < copies; ++y) value += sums[y * columns + x];
+      finish(row, x / D, x % D, value, tops[x / D], tops[HEADS + x / D]);
+    }
+    __syncthreads();
+  }
+}
+
+long long workspace_floats(int sms) { return (long long)sms * 2 * HEADS * (128 + 2); }
+int workspace_counters(int sms) { return sms; }
+
+template <int F, int D>
+static cudaError_t launch_as(const Args& a, int sms, cudaStream_t stream) {
+  using S = Shape<F, D>;
+  // dynamic shared memory beyond 48 KB is opted into once per device
+  static unsigned long long opted = 0;
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  const unsigned long long bit = 1ull << (device & 63);
+  if (!(__atomic_load_n(&opted, __ATOMIC_ACQUIRE) & bit)) {
+    err = cudaFuncSetAttribute(decode_kernel<F, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (err != cudaSuccess) return err;
+    __atomic_fetch_or(&opted, bit, __ATOMIC_RELEASE);
+  }
+  decode_kernel<F, D><<<sms, S::THREADS, S::SMEM, stream>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t launch(const Args& a, int sms, cudaStream_t stream) {
+  cudaError_t err = cudaSuccess;
+  kv::by_format(a.pool, [&](auto f, auto d) { err = launch_as<decltype(f)::value, decltype(d)::value>(a, sms, stream); });
+  return err;
 }
 
 }  // namespace paged
-
-void paged_attention(at::Tensor q, at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale,
-                     c10::optional<at::Tensor> v_scale, at::Tensor block_table, at::Tensor lengths, at::Tensor out,
-                     c10::optional<at::Tensor> lse, double scale) {
-  const c10::cuda::CUDAGuard guard(k_pool.device());
-  const kv::Pool p = kv::checked_pool(k_pool, v_pool, k_scale, v_scale);
-  HT_CHECK(q.is_cuda() && q.device() == k_pool.device() && q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.size(2) == p.D &&
-               q.size(1) % p.Hkv == 0 && q.size(1) > 0,
-           "q must be a CUDA bf16 tensor [B, H, ", p.D, "] with H a multiple of the pool's ", p.Hkv, " heads");
-  const int64_t B = q.size(0), H = q.size(1);
-  HT_CHECK(block_table.is_cuda() && block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == B &&
-               (block_table.size(1) <= 1 || block_table.stride(1) == 1),
-           "block_table must be a CUDA int32 tensor [B, pages per sequence] with unit inner stride");
-  HT_CHECK(lengths.is_cuda() && lengths.scalar_type() == at::kInt && lengths.is_contiguous() && lengths.dim() == 1 && lengths.size(0) == B,
-           "lengths must be a contiguous CUDA int32 tensor [B]");
-  HT_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.sizes() == q.sizes(), "out must be contiguous bf16 [B, H, D]");
-  if (B == 0) return;
-  if (q.stride(2) != 1) q = q.contiguous();
-  paged::Args a{reinterpret_cast<const __nv_bfloat16*>(q.data_ptr()), q.stride(0), q.stride(1), p, block_table.data_ptr<int>(),
-                block_table.stride(0), (int)block_table.size(1), lengths.data_ptr<int>(),
-                reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), nullptr, (int)B, (int)H, (float)(scale * 1.4426950408889634)};
-  if (lse.has_value() && lse->defined()) {
-    HT_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->numel() == B * H, "lse must be contiguous fp32 [B, H]");
-    a.lse = lse->data_ptr<float>();
-  }
-  kv::by_format(p, [&](auto f, auto d) {
-    paged::decode_kernel<decltype(f)::value, decltype(d)::value><<<(unsigned)((B * H + 3) / 4), 128, 0, stream()>>>(a);
-  });
-  HT_CUDA_CHECK(cudaGetLastError());
-}
-
 }  // namespace ht

@@ -12,32 +12,13 @@
 //
 // Each cut is found by bisection over the bits of the ordered logit: 32 passes over the row that count
 // the tokens, or sum the weights, at or above a pivot.
-#include "common.cuh"
+#include "generation.cuh"
 
 namespace ht {
 namespace sampling {
 
 constexpr int THREADS = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
-
-// One value per row, or one for all of them.
-template <typename T>
-struct PerRow {
-  const T* rows;
-  T same;
-  __device__ __forceinline__ T operator[](int row) const { return rows != nullptr ? rows[row] : same; }
-};
-
-struct Args {
-  const void* logits;
-  long long row_stride, noise_stride;
-  const float* noise;
-  PerRow<float> temperature, top_p, min_p;
-  PerRow<int> top_k;
-  long long* token;
-  float* logprob;
-  int B, V;
-};
 
 // Unsigned keys in the order of the floats; NaN and -inf share the lowest key.
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -198,48 +179,11 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
   }
 }
 
+cudaError_t launch(const Args& a, int sms, cudaStream_t stream) {
+  if (a.wide) sample_kernel<float><<<(unsigned)a.B, THREADS, 0, stream>>>(a);
+  else sample_kernel<__nv_bfloat16><<<(unsigned)a.B, THREADS, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
 }  // namespace sampling
-
-template <typename T>
-static sampling::PerRow<T> per_row(const c10::optional<at::Tensor>& t, double same, const at::Tensor& logits, at::ScalarType type,
-                                   const char* name) {
-  if (!t.has_value() || !t->defined()) return {nullptr, (T)same};
-  HT_CHECK(t->device() == logits.device() && t->scalar_type() == type && t->is_contiguous() && t->dim() == 1 && t->size(0) == logits.size(0),
-           name, " must be a number or a contiguous ", type, " tensor [B] on the logits' device");
-  return {t->data_ptr<T>(), (T)same};
-}
-
-void sample_tokens(at::Tensor logits, at::Tensor noise, c10::optional<at::Tensor> temperature_rows, double temperature,
-                   c10::optional<at::Tensor> top_k_rows, int64_t top_k, c10::optional<at::Tensor> top_p_rows, double top_p,
-                   c10::optional<at::Tensor> min_p_rows, double min_p, at::Tensor token, at::Tensor logprob) {
-  const c10::cuda::CUDAGuard guard(logits.device());
-  HT_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat),
-           "logits must be a CUDA bf16 or fp32 tensor [B, V]");
-  const int64_t B = logits.size(0), V = logits.size(1);
-  HT_CHECK(V >= 1 && V < (1ll << 30), "the vocabulary must have 1 to 2^30 - 1 tokens, got ", V);
-  HT_CHECK(noise.device() == logits.device() && noise.scalar_type() == at::kFloat && noise.sizes() == logits.sizes(),
-           "noise must be an fp32 tensor of the logits' shape and device");
-  HT_CHECK(token.scalar_type() == at::kLong && token.is_contiguous() && token.numel() == B && logprob.scalar_type() == at::kFloat &&
-               logprob.is_contiguous() && logprob.numel() == B,
-           "results must be contiguous int64 and fp32 [B]");
-  if (B == 0) return;
-  if (V > 1 && logits.stride(1) != 1) logits = logits.contiguous();
-  if (V > 1 && noise.stride(1) != 1) noise = noise.contiguous();
-  sampling::Args a{logits.data_ptr(),
-                   logits.stride(0),
-                   noise.stride(0),
-                   noise.data_ptr<float>(),
-                   per_row<float>(temperature_rows, temperature, logits, at::kFloat, "temperature"),
-                   per_row<float>(top_p_rows, top_p, logits, at::kFloat, "top_p"),
-                   per_row<float>(min_p_rows, min_p, logits, at::kFloat, "min_p"),
-                   per_row<int>(top_k_rows, (double)std::min<int64_t>(std::max<int64_t>(top_k, 0), V), logits, at::kInt, "top_k"),
-                   reinterpret_cast<long long*>(token.data_ptr<int64_t>()),
-                   logprob.data_ptr<float>(),
-                   (int)B,
-                   (int)V};
-  if (logits.scalar_type() == at::kFloat) sampling::sample_kernel<float><<<(unsigned)B, sampling::THREADS, 0, stream()>>>(a);
-  else sampling::sample_kernel<__nv_bfloat16><<<(unsigned)B, sampling::THREADS, 0, stream()>>>(a);
-  HT_CUDA_CHECK(cudaGetLastError());
-}
-
 }  // namespace ht
