@@ -150,6 +150,8 @@ void paged_attention(at::Tensor q, at::Tensor k_pool, at::Tensor v_pool, c10::op
   HT_CHECK(block_table.device() == q.device() && block_table.scalar_type() == at::kInt && block_table.dim() == 2 &&
                block_table.size(0) == B && (block_table.size(1) <= 1 || block_table.stride(1) == 1) && block_table.size(1) * k_pool.size(2) <= INT32_MAX - 256,
            "block_table must be int32 [B, pages per sequence] with unit inner stride, on the pool's device");
+  HT_CHECK(B * ((block_table.size(1) * k_pool.size(2) + 15) / 16) < (1ll << 31) / H,
+           "block_table spans too many tokens for one call (sequences x heads x tokens / 16 beyond 2^31): split the batch");
   HT_CHECK(lengths.device() == q.device() && lengths.scalar_type() == at::kInt && lengths.is_contiguous() && lengths.dim() == 1 &&
                lengths.size(0) == B,
            "lengths must be a contiguous int32 tensor [B] on the pool's device");
@@ -179,7 +181,8 @@ void sample_tokens(at::Tensor logits, at::Tensor noise, c10::optional<at::Tensor
   HT_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat),
            "logits must be a CUDA bf16 or fp32 tensor [B, V]");
   const int64_t B = logits.size(0), V = logits.size(1);
-  HT_CHECK(V >= 1 && V < (1ll << 30) && B <= INT32_MAX, "the vocabulary must have 1 to 2^30 - 1 tokens, got ", V);
+  HT_CHECK(V >= 1 && V <= sampling::kMaxVocabulary && B <= (1 << 24), "sample_tokens supports 1 to ", sampling::kMaxVocabulary,
+           " tokens and up to 2^24 rows, got ", V, " and ", B);
   HT_CHECK(noise.device() == logits.device() && noise.scalar_type() == at::kFloat && noise.sizes() == logits.sizes(),
            "noise must be an fp32 tensor of the logits' shape and device");
   HT_CHECK(token.device() == logits.device() && token.scalar_type() == at::kLong && token.is_contiguous() && token.numel() == B &&

@@ -89,6 +89,8 @@ cudaError_t launch(const Args& a, int sms, cudaStream_t stream);
 
 namespace sampling {
 
+constexpr int kMaxVocabulary = 1 << 18;
+
 // One value per row, or one for all of them.
 template <typename T>
 struct PerRow {

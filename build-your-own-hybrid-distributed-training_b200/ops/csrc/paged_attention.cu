@@ -43,14 +43,16 @@ constexpr int HEADS = 8;  // query heads of one row
 template <int F, int D>
 struct Shape {
   static constexpr int ROW = D * (F == kv::kBf16 ? 2 : 1);  // bytes of one key
-  static constexpr int TOK = ROW == 256 ? 16 : 32;          // tokens of one tile
+  static constexpr int TOK = ROW == 256 ? 16 : ROW == 64 ? 64 : 32;  // tokens of one tile: 8 KB of keys and values
   static constexpr int WARPS = 8;
   static constexpr int DATA = TOK * ROW, SCALES = F == kv::kBf16 ? 0 : TOK * 4;
   static constexpr int STAGE = 2 * (DATA + SCALES);
-  static constexpr int STAGES = STAGE > 8192 ? 2 : STAGE == 8192 ? 3 : 4;
+  static constexpr int STAGES = F == kv::kBf16 ? 3 : 2;
   static constexpr int PIECE = HEADS * (D + 2) * 4;  // o, m and sum of one row's piece
   static constexpr int THREADS = WARPS * 32;
-  static constexpr int SMEM = WARPS * (STAGES * STAGE + PIECE) + 1024;
+  static constexpr int FACTORS = F == kv::kBf16 ? 0 : TOK * 16;  // per token: what its scales do to score and weight
+  static constexpr int BOOK = 224;  // bookkeeping per warp
+  static constexpr int SMEM = WARPS * (STAGES * STAGE + PIECE + FACTORS + BOOK);
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -85,11 +87,11 @@ __device__ __forceinline__ void ldmatrix4t(uint32_t* r, uint32_t a) {
 template <int F>
 __device__ __forceinline__ void mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (F == kv::kBf16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -175,21 +177,28 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
   constexpr int TOK = S::TOK, GROUPS = TOK / 16, NT = D / 8, WARPS = S::WARPS;
   extern __shared__ __align__(16) unsigned char smem[];
   struct Meta {
-    long long item;  // first tile of the row on the line
+    int item;  // first tile of the row on the line
     int b, row, tile, count, tiles;
   };
+  struct Group {
+    Meta first;
+    int end_tile, from, to;  // pieces [from, to) of the list of all
+    bool whole;
+  };
   struct Shared {
-    Meta meta[WARPS][2];
-    long long scan[WARPS];
+    Meta meta[2 * WARPS];
+    Group groups[WARPS + 1];
+    int count;
+    uint32_t have;
+    float weight[2 * WARPS][HEADS];
+    int scan[WARPS];
     Cursor start[WARPS];
-    int head_of[2 * WARPS + 1];
-    int groups;
     int join_first[2], join_count[2], join_b[2], join_row[2];
   };
-  static_assert(sizeof(Shared) <= 1024, "shared bookkeeping");
+  static_assert(sizeof(Shared) <= WARPS * S::BOOK, "shared bookkeeping");
   unsigned char* const rings = smem;
   unsigned char* const pieces = smem + WARPS * S::STAGES * S::STAGE;
-  Shared& sh = *reinterpret_cast<Shared*>(pieces + WARPS * S::PIECE);
+  Shared& sh = *reinterpret_cast<Shared*>(pieces + WARPS * (S::PIECE + S::FACTORS));
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int g = lane / 4, c4 = lane % 4;
@@ -197,88 +206,108 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
   const int chunks = (group + HEADS - 1) / HEADS;  // rows per key/value head
   const int rows = a.pool.Hkv * chunks;
 
-  // ---- sequences without tokens
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    if (tokens_of(a, b) > 0) continue;
-    for (int i = tid; i < a.H * D; i += S::THREADS) a.out[(long long)b * a.H * D + i] = __float2bfloat16_rn(0.f);
-    if (a.lse != nullptr)
-      for (int i = tid; i < a.H; i += S::THREADS) a.lse[(long long)b * a.H + i] = -INFINITY;
-  }
-
-  // ---- this block's and its warps' ranges of the line
-  const auto block_sum = [&](long long v) {
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  // ---- this block's and its warps' ranges of the line, from one scan of the lengths (in chunks of a block's threads)
+  int per_block = 0, block_from = 0, block_to = 0, per_warp = 0;
+  if (tid < 2 * WARPS) sh.meta[tid].count = 0;
+  const auto scan_chunk = [&](int tiles, int& total) {  // inclusive
+    int upto = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
     __syncthreads();
-    if (lane == 0) sh.scan[warp] = v;
+    if (lane == 31) sh.scan[warp] = upto;
     __syncthreads();
-    v = 0;
-    for (int w = 0; w < WARPS; ++w) v += sh.scan[w];
-    return v;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const int of_warp = sh.scan[w];
+      if (w < warp) upto += of_warp;
+      total += of_warp;
+    }
+    return upto;
   };
-  long long mine = 0;
-  for (int b = tid; b < a.B; b += S::THREADS) mine += (tokens_of(a, b) + TOK - 1) / TOK;
-  const long long line = block_sum(mine) * rows;
-  // at least one tile for each warp of a block: fewer, fuller blocks have fewer pieces to join
-  const long long per_block = max((line + gridDim.x - 1) / gridDim.x, (long long)WARPS);
-  const long long block_from = min(line, per_block * blockIdx.x), block_to = min(line, block_from + per_block);
-  if (block_from >= block_to) return;
-  const long long per_warp = (block_to - block_from + WARPS - 1) / WARPS;
-  if (tid < 2 * WARPS) sh.meta[tid / 2][tid % 2].count = 0;
   {
-    long long base = 0;  // tiles of the sequences before this chunk of them
-    for (int b0 = 0; b0 < a.B && base < block_to; b0 += S::THREADS) {
+    const int my_n = tid < a.B ? tokens_of(a, tid) : 0;
+    const int my_tiles = (my_n + TOK - 1) / TOK * rows;
+    int total = 0;
+    const int my_upto = scan_chunk(my_tiles, total);
+    int line = total;
+    for (int b0 = S::THREADS; b0 < a.B; b0 += S::THREADS) {
+      int more = 0;
+      scan_chunk(b0 + tid < a.B ? (tokens_of(a, b0 + tid) + TOK - 1) / TOK * rows : 0, more);
+      line += more;
+    }
+    // at least one tile for each warp of a block: fewer, fuller blocks have fewer pieces to join
+    per_block = max((int)((line + gridDim.x - 1) / gridDim.x), WARPS);
+    block_from = min((long long)line, (long long)per_block * blockIdx.x);
+    block_to = min(line - block_from, per_block) + block_from;
+    per_warp = (block_to - block_from + WARPS - 1) / WARPS;
+    int base = 0;  // tiles of the sequences before this chunk of them
+    for (int b0 = 0; b0 < a.B; b0 += S::THREADS) {
       const int b = b0 + tid;
-      const int n = b < a.B ? tokens_of(a, b) : 0;
-      const long long tiles = (long long)((n + TOK - 1) / TOK) * rows;
-      long long upto = tiles;
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long other = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += other;
+      int n = my_n, upto = my_upto;
+      if (b0 > 0) {
+        n = b < a.B ? tokens_of(a, b) : 0;
+        upto = scan_chunk((n + TOK - 1) / TOK * rows, total);
       }
-      __syncthreads();
-      if (lane == 31) sh.scan[warp] = upto;
-      __syncthreads();
-      long long total = 0;
-      for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) upto += sh.scan[w];
-        total += sh.scan[w];
+      if (n == 0 && b < a.B && b % gridDim.x == blockIdx.x) {  // no tokens, hence no tiles: this thread writes the result
+        for (int i = 0; i < a.H * D; i += 8) *reinterpret_cast<uint4*>(a.out + (long long)b * a.H * D + i) = make_uint4(0, 0, 0, 0);
+        if (a.lse != nullptr)
+          for (int i = 0; i < a.H; ++i) a.lse[(long long)b * a.H + i] = -INFINITY;
       }
-      const long long from = base + upto - tiles, to = base + upto;
-      for (int w = 0; w < WARPS; ++w) {
-        const long long at = block_from + w * per_warp;
-        if (at >= from && at < to) {
-          const int per_row = (n + TOK - 1) / TOK;
-          const long long in = at - from;
-          sh.start[w] = Cursor{b, (int)(in / per_row), (int)(in % per_row), per_row, n};
-        }
+      const int per_row = (n + TOK - 1) / TOK, from = base + upto - per_row * rows, to = base + upto;
+      if (from < block_to && to > block_from) {
+        // the warps that start inside this sequence
+        const int w0 = from <= block_from ? 0 : (from - block_from + per_warp - 1) / per_warp;
+        for (int w = w0; w < WARPS && block_from + w * per_warp < min(to, block_to); ++w) sh.start[w] = Cursor{b, 0, from, per_row, n};
       }
       base += total;
     }
   }
+  if (block_from >= block_to) return;
   __syncthreads();
 
-  const long long from = block_from + warp * per_warp;
-  const int count = (int)max(0ll, min(per_warp, block_to - from));
+  const int from = block_from + warp * per_warp;
+  const int count = max(0, min(per_warp, block_to - from));
   unsigned char* const ring = rings + warp * S::STAGES * S::STAGE;
   const uint32_t ring_addr = smem_addr(ring);
+  [[maybe_unused]] float4* const factors = reinterpret_cast<float4*>(pieces + WARPS * S::PIECE + warp * S::FACTORS);
 
   if (count > 0) {
-    Cursor load = sh.start[warp], use = load;
+    Cursor load = sh.start[warp];
+    load.tile = from - load.tile;  // was: the sequence's first tile on the line
+    load.row = load.tile / load.tiles;
+    load.tile -= load.row * load.tiles;
+    Cursor use = load;
     int to_load = count;
     uint32_t held = 0;  // per stage: which groups of 16 tokens are in the pool
-    int page = -1;      // lane i < GROUPS: page of the tile's group i
-    const auto look_up = [&] {
-      const int token = load.tile * TOK + lane * 16;
-      page = -1;
-      if (to_load > 0 && lane < GROUPS && token < load.n) page = a.table[load.b * a.table_row + (token >> a.pool.page_shift)];
+    // Pages are looked up 32 groups at a time, a window ahead of their use.
+    constexpr int WINDOW = 32 / GROUPS;  // tiles
+    const auto look_up = [&](const Cursor& c) {
+      const int token = c.tile * TOK + lane * 16;
+      return c.b < a.B && token < c.n ? a.table[c.b * a.table_row + (token >> a.pool.page_shift)] : -1;
     };
+    const auto next_window = [&](Cursor c) {
+      c.tile = min(c.tile + WINDOW, c.tiles) - 1;
+      advance<TOK>(a, c, rows);
+      return c;
+    };
+    int page = look_up(load), next_page = -1, window = load.tile;
+    bool turn = false;  // the next tile opens a window
     const auto issue = [&](int stage) {
       if (to_load > 0) {
+        const bool opens = turn;
+        if (opens) {
+          page = next_page;
+          window = load.tile;
+        }
         const uint32_t base = ring_addr + stage * S::STAGE;
         uint32_t bits = 0;
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
-          const int p = __shfl_sync(0xffffffffu, page, i);
+          const int p = __shfl_sync(0xffffffffu, page, (load.tile - window) * GROUPS + i);
           const int token = load.tile * TOK + i * 16;
           const bool in_pool = p >= 0 && p < a.pool.pages;
           bits |= (uint32_t)in_pool << i;
@@ -302,25 +331,28 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
           }
         }
         held = (held & ~(0xfu << (4 * stage))) | (bits << (4 * stage));
+        if (opens) next_page = look_up(next_window(load));
         advance<TOK>(a, load, rows);
         --to_load;
-        look_up();
+        turn = load.tile == 0 || load.tile == window + WINDOW;
       }
       copies_commit();
     };
 
-    look_up();
+    const Cursor ahead = next_window(load);
+    issue(0);
+    next_page = look_up(ahead);
 #pragma unroll
-    for (int s = 0; s < S::STAGES - 1; ++s) issue(s);
+    for (int s = 1; s < S::STAGES - 1; ++s) issue(s);
 
     // Per row: q as fragments of the first operand, the output's accumulators, and the softmax's state.
     constexpr int QR = D / 8;  // registers of q
     uint32_t q[QR];
-    float o[NT][4], m = -INFINITY, sum = 0.f, factor = 0.f;
+    float o[NT][4], m = -INFINITY, sum = 0.f, up = 1.f;  // up: the power of two that q was divided by
     int row_tile = 0;          // the row's first tile in this warp
     bool opened = false, first_row = true;
     int stage = 0;
-    long long row_start = from - use.tile;  // first tile of the row on the line
+    int row_start = from - use.tile;  // first tile of the row on the line
 
     for (int i = 0; i < count; ++i) {
       if (!opened) {
@@ -335,7 +367,6 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
         const __nv_bfloat16* src = a.q + use.b * a.q_seq + ((long long)(use.row / chunks) * group + in_group) * a.q_head;
         // lane (g, c4) holds, of head g, the 16-byte pieces of a key row that it will load: piece 4 j + c4
         if constexpr (F == kv::kBf16) {
-          factor = a.scale_log2;
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
             const uint4 x = real ? *reinterpret_cast<const uint4*>(src + (j * 4 + c4) * 8) : make_uint4(0, 0, 0, 0);
@@ -360,13 +391,13 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           // the power of two that brings the largest magnitude into [1, 2): exact both ways
           const int exponent = max(-126, min(126, (int)(__float_as_uint(top) >> 23) - 127));
-          const float down = __uint_as_float((uint32_t)(127 - exponent) << 23), up = __uint_as_float((uint32_t)(127 + exponent) << 23);
+          const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
+          up = __uint_as_float((uint32_t)(127 + exponent) << 23);
 #pragma unroll
           for (int r = 0; r < QR; ++r) {
             const float2 f = unpack<kv::kBf16>(q[r]);
             q[r] = pack<F>(f.x * down, f.y * down);
           }
-          factor = a.scale_log2 * up;
         }
       }
 
@@ -377,49 +408,67 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
         if (next >= S::STAGES) next -= S::STAGES;
         issue(next);
       }
-      const uint32_t kb = ring_addr + stage * S::STAGE, vb = kb + S::DATA, sb = kb + 2 * S::DATA;
+      const uint32_t kb = ring_addr + stage * S::STAGE, vb = kb + S::DATA;
       const uint32_t in_pool = held >> (4 * stage);
+      [[maybe_unused]] const float* const stage_scales = reinterpret_cast<const float*>(ring + stage * S::STAGE + 2 * S::DATA);
 
+      // 8 bits: one lane per token works out what its scales do.  A scale of zero (none that kv_cache_write leaves) counts as
+      // the smallest one, NaN stays NaN; masked tokens get a finite score factor and an exponent of -inf.
+      if constexpr (F != kv::kBf16) {
+#pragma unroll
+        for (int i = lane; i < TOK; i += 32) {
+          const bool real = ((in_pool >> (i / 16)) & 1u) && use.tile * TOK + i < use.n;
+          const float ks = stage_scales[i], raw = stage_scales[TOK + i];
+          const float vs = raw < kv::kMinScale ? kv::kMinScale : raw;
+          factors[i] = real ? make_float4(ks * a.scale_log2, fast_log2(vs), __fdividef(1.f, vs), 0.f) : make_float4(0.f, -INFINITY, 0.f, 0.f);
+        }
+        __syncwarp();
+      }
       // scores, in the accumulator's layout: head g, tokens 8 t + 2 c4 and + 1
+      float acc[TOK / 8][4];
+#pragma unroll
+      for (int t = 0; t < TOK / 8; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+      if constexpr (F == kv::kBf16) {
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+          for (int t = 0; t < TOK / 8; ++t) {
+            const uint4 k = lds128(kb + (t * 8 + g) * S::ROW + (((j * 4 + c4) ^ ((g & 1) << 2)) * 16));
+            mma<F>(acc[t], q[4 * j], 0u, q[4 * j + 1], 0u, k.x, k.y);
+            mma<F>(acc[t], q[4 * j + 2], 0u, q[4 * j + 3], 0u, k.z, k.w);
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+          uint32_t w[TOK / 8][4];
+#pragma unroll
+          for (int t = 0; t < TOK / 8; ++t) {
+            const uint4 k = lds128(kb + (t * 8 + g) * S::ROW + ((D == 128 ? (j * 4 + c4) ^ ((g & 1) << 2) : c4) * 16));
+            w[t][0] = unsign<F>(k.x), w[t][1] = unsign<F>(k.y), w[t][2] = unsign<F>(k.z), w[t][3] = unsign<F>(k.w);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int t = 0; t < TOK / 8; ++t)
+              mma<F>(acc[t], q[8 * j + 2 * r], 0u, q[8 * j + 2 * r + 1], 0u, half_pair<F, 0>(w[t][r]), half_pair<F, 1>(w[t][r]));
+        }
+      }
       float s[TOK / 8][2], inv[TOK / 8][2];
       float top = -INFINITY;
 #pragma unroll
       for (int t = 0; t < TOK / 8; ++t) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint32_t row = kb + (t * 8 + g) * S::ROW;
         if constexpr (F == kv::kBf16) {
-#pragma unroll
-          for (int j = 0; j < D / 32; ++j) {
-            const uint4 k = lds128(row + (((j * 4 + c4) ^ ((g & 1) << 2)) * 16));
-            mma<F>(acc, q[4 * j], 0u, q[4 * j + 1], 0u, k.x, k.y);
-            mma<F>(acc, q[4 * j + 2], 0u, q[4 * j + 3], 0u, k.z, k.w);
-          }
+          const int token = use.tile * TOK + t * 8 + 2 * c4;
+          const bool pool_ok = (in_pool >> (t / 2)) & 1u;
+          s[t][0] = pool_ok && token < use.n ? acc[t][0] * a.scale_log2 : -INFINITY;
+          s[t][1] = pool_ok && token + 1 < use.n ? acc[t][1] * a.scale_log2 : -INFINITY;
         } else {
-#pragma unroll
-          for (int j = 0; j < D / 64; ++j) {
-            const uint4 k = lds128(row + ((D == 128 ? (j * 4 + c4) ^ ((g & 1) << 2) : c4) * 16));
-            const uint32_t w[4] = {unsign<F>(k.x), unsign<F>(k.y), unsign<F>(k.z), unsign<F>(k.w)};
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              mma<F>(acc, q[8 * j + 2 * r], 0u, q[8 * j + 2 * r + 1], 0u, half_pair<F, 0>(w[r]), half_pair<F, 1>(w[r]));
-          }
+          const float4 f0 = factors[t * 8 + 2 * c4], f1 = factors[t * 8 + 2 * c4 + 1];
+          s[t][0] = fmaf(acc[t][0] * up, f0.x, f0.y);
+          s[t][1] = fmaf(acc[t][1] * up, f1.x, f1.y);
+          inv[t][0] = f0.z;
+          inv[t][1] = f1.z;
         }
-        float2 ks = make_float2(1.f, 1.f), shift = make_float2(0.f, 0.f);
-        inv[t][0] = inv[t][1] = 1.f;
-        if constexpr (F != kv::kBf16) {
-          const uint2 kw = lds64(sb + (t * 8 + 2 * c4) * 4), vw = lds64(sb + S::SCALES + (t * 8 + 2 * c4) * 4);
-          ks = make_float2(__uint_as_float(kw.x), __uint_as_float(kw.y));
-          // a scale of zero (none that kv_cache_write leaves) counts as the smallest one; NaN stays NaN
-          const float v0 = __uint_as_float(vw.x), v1 = __uint_as_float(vw.y);
-          const float s0 = v0 < kv::kMinScale ? kv::kMinScale : v0, s1 = v1 < kv::kMinScale ? kv::kMinScale : v1;
-          shift = make_float2(fast_log2(s0), fast_log2(s1));
-          inv[t][0] = __frcp_rn(s0);
-          inv[t][1] = __frcp_rn(s1);
-        }
-        const int token = use.tile * TOK + t * 8 + 2 * c4;
-        const bool pool_ok = (in_pool >> (t / 2)) & 1u;
-        s[t][0] = pool_ok && token < use.n ? acc[0] * factor * ks.x + shift.x : -INFINITY;
-        s[t][1] = pool_ok && token + 1 < use.n ? acc[1] * factor * ks.y + shift.y : -INFINITY;
         top = fmaxf(top, fmaxf(s[t][0], s[t][1]));
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -439,9 +488,9 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
       for (int t = 0; t < TOK / 8; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const bool masked = s[t][e] == -INFINITY;
-          const float p = masked ? 0.f : fast_exp2(s[t][e] - at);
-          sum += F == kv::kBf16 ? p : masked ? 0.f : p * inv[t][e];
+          const float p = fast_exp2(s[t][e] - at);
+          if constexpr (F == kv::kBf16) sum += p;
+          else sum = fmaf(p, inv[t][e], sum);
           s[t][e] = p;
         }
 
@@ -505,7 +554,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
           const int in_group = (use.row % chunks) * HEADS + g;
           if (in_group < group) {
             const long long head = (long long)use.b * a.H + (use.row / chunks) * group + in_group;
-            const float norm = sum == 0.f ? 0.f : 1.f / sum;
+            const float norm = sum == 0.f ? 0.f : __fdividef(1.f, sum);
             __nv_bfloat16* dst = a.out + head * D;
             if constexpr (F == kv::kBf16) {
 #pragma unroll
@@ -534,15 +583,16 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
             __syncwarp();
           }
           float* const piece = reinterpret_cast<float*>(which == 0 ? pieces + warp * S::PIECE : ring);
+          // in the order of the accumulators: value (t, e) of every lane next to one another
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) piece[g * D + dim(t, e)] = o[t][e] + o[t][e + 2];
+            for (int e = 0; e < 2; ++e) piece[(2 * t + e) * 32 + lane] = o[t][e] + o[t][e + 2];
           if (c4 == 0) {
             piece[HEADS * D + g] = m;
             piece[HEADS * D + HEADS + g] = sum;
           }
-          if (lane == 0) sh.meta[warp][which] = Meta{row_start, use.b, use.row, row_tile, use.tile + 1 - row_tile, use.tiles};
+          if (lane == 0) sh.meta[2 * warp + which] = Meta{row_start, use.b, use.row, row_tile, use.tile + 1 - row_tile, use.tiles};
           __syncwarp();
         }
         opened = first_row = false;
@@ -555,62 +605,108 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
   __syncthreads();
 
   // ---- pieces of the same row are neighbours: merge them
+  constexpr int STEP = HEADS * (D + 2);  // floats of a piece
+  const auto piece_of = [&](int i) {
+    return reinterpret_cast<float*>(i % 2 == 0 ? pieces + i / 2 * S::PIECE : rings + i / 2 * S::STAGES * S::STAGE);
+  };
   if (warp == 0) {
-    const bool some = lane < 2 * WARPS && sh.meta[lane / 2 % WARPS][lane % 2].count > 0;
-    const long long item = some ? sh.meta[lane / 2][lane % 2].item : -1;
+    const bool some = lane < 2 * WARPS && sh.meta[lane].count > 0;
+    const int item = some ? sh.meta[lane].item : -1;
     const uint32_t have = __ballot_sync(0xffffffffu, some), before = have & ((1u << lane) - 1);
-    const long long previous = __shfl_sync(0xffffffffu, item, before ? 31 - __clz(before) : 0);
+    const int previous = __shfl_sync(0xffffffffu, item, before ? 31 - __clz(before) : 0);
     const bool head = some && (before == 0 || previous != item);
     const uint32_t heads = __ballot_sync(0xffffffffu, head);
-    if (head) sh.head_of[__popc(heads & ((1u << lane) - 1))] = lane;
+    if (head) {
+      const uint32_t later = heads & ~((2u << lane) - 1);
+      const int to = later ? __ffs(later) - 1 : 2 * WARPS;
+      const int last = 31 - __clz(have & (to == 32 ? 0xffffffffu : (1u << to) - 1));
+      Group& group = sh.groups[__popc(heads & ((1u << lane) - 1))];
+      group.first = sh.meta[lane];
+      group.end_tile = sh.meta[last].tile + sh.meta[last].count;
+      group.from = lane;
+      group.to = last + 1;
+      group.whole = group.first.tile == 0 && group.end_tile == group.first.tiles;
+    }
     if (lane == 0) {
-      sh.groups = __popc(heads);
-      sh.head_of[__popc(heads)] = 2 * WARPS;
+      sh.count = __popc(heads);
+      sh.have = have;
       sh.join_count[0] = sh.join_count[1] = 0;
     }
   }
   __syncthreads();
-  const int real_heads = min(group, HEADS), columns = real_heads * D;
-  const auto piece_of = [&](int i) {
-    return reinterpret_cast<const float*>(i % 2 == 0 ? pieces + i / 2 * S::PIECE : rings + i / 2 * S::STAGES * S::STAGE);
+  const int real_heads = min(group, HEADS);
+  // The results of a row's head h, and whether the group has that head.
+  const auto head_of = [&](int b, int row, int h, long long& head) {
+    const int kv_head = chunks == 1 ? row : row / chunks, in_group = (row - kv_head * chunks) * HEADS + h;
+    head = (long long)b * a.H + (long long)kv_head * group + in_group;
+    return in_group < group;
   };
-  const auto ends_of = [&](int gi, Meta& first, Meta& last) {  // the group's first and last piece
-    first = sh.meta[sh.head_of[gi] / 2][sh.head_of[gi] % 2];
-    last = first;
-    for (int i = sh.head_of[gi] + 1; i < sh.head_of[gi + 1]; ++i)
-      if (sh.meta[i / 2][i % 2].count > 0) last = sh.meta[i / 2][i % 2];
+  // Dimension of accumulator place (v = 2 t + e, lane).
+  const auto dim_of = [&](int v, int lane_) {
+    return F == kv::kBf16 ? (v >> 1) * 8 + 2 * (lane_ & 3) + (v & 1) : (2 * (lane_ & 3) + (v & 1)) * NT + (v >> 1);
   };
-  const auto finish = [&](const Meta& row, int h, int d, float value, float top, float total) {
-    const int in_group = row.row % chunks * HEADS + h;
-    if (in_group >= group) return;
-    const long long head = (long long)row.b * a.H + (long long)(row.row / chunks) * group + in_group;
-    a.out[head * D + d] = __float2bfloat16_rn(total == 0.f ? 0.f : value / total);
-    if (d == 0 && a.lse != nullptr) a.lse[head] = total == 0.f ? -INFINITY : (top + fast_log2(total)) * LN2;
-  };
-  for (int x = tid; x < sh.groups * columns; x += S::THREADS) {
-    const int gi = x / columns, h = x % columns / D, d = x % D;
-    float top = -INFINITY, value = 0.f, total = 0.f;
-    for (int i = sh.head_of[gi]; i < sh.head_of[gi + 1]; ++i)
-      if (sh.meta[i / 2][i % 2].count > 0) top = fmaxf(top, piece_of(i)[HEADS * D + h]);
-    const float at = top == -INFINITY ? 0.f : top;
-    for (int i = sh.head_of[gi]; i < sh.head_of[gi + 1]; ++i)
-      if (sh.meta[i / 2][i % 2].count > 0) {
-        const float* p = piece_of(i);
-        const float w = fast_exp2(p[HEADS * D + h] - at);
-        value += w * p[h * D + d];
-        total += w * p[HEADS * D + HEADS + h];
+  float* const merged = a.partial + (long long)blockIdx.x * 2 * STEP;
+  // weights of the pieces: a warp per head, a lane per piece
+  static_assert(2 * WARPS <= 32 && WARPS >= HEADS, "one lane per piece, one warp per head");
+  if (warp < real_heads) {
+    const uint32_t have = sh.have;
+    const bool some = (have >> lane) & 1u;
+    const float* p = piece_of(some ? lane : 0);
+    const float mine = some ? p[HEADS * D + warp] : -INFINITY, part = some ? p[HEADS * D + HEADS + warp] : 0.f;
+    int gi = 0;
+    while (some && lane >= sh.groups[gi].to) ++gi;
+    const Group& grp = sh.groups[gi];
+    const uint32_t members = some ? have & (0xffffffffu << grp.from) & (0xffffffffu >> (32 - grp.to)) : 0u;
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2 * WARPS; ++i) {
+      const float other = __shfl_sync(0xffffffffu, mine, i);
+      if ((members >> i) & 1u) top = fmaxf(top, other);
+    }
+    const float at = top == -INFINITY ? 0.f : top, w = fast_exp2(mine - at);
+    const float weighted = w * part;
+#pragma unroll
+    for (int i = 0; i < 2 * WARPS; ++i) {
+      const float other = __shfl_sync(0xffffffffu, weighted, i);
+      if ((members >> i) & 1u) total += other;
+    }
+    if (some) {
+      sh.weight[lane][warp] = w * (!grp.whole ? 1.f : total == 0.f ? 0.f : __fdividef(1.f, total));
+      long long head;
+      if (lane == grp.from && head_of(grp.first.b, grp.first.row, warp, head)) {
+        if (!grp.whole) {
+          float* const out = merged + (grp.first.tile > 0 ? 0 : STEP);
+          out[HEADS * D + warp] = top;
+          out[HEADS * D + HEADS + warp] = total;
+        } else if (a.lse != nullptr) {
+          a.lse[head] = total == 0.f ? -INFINITY : (top + fast_log2(total)) * LN2;
+        }
       }
-    Meta first, last;
-    ends_of(gi, first, last);
-    if (first.tile == 0 && last.tile + last.count == last.tiles) {
-      finish(first, h, d, value, top, total);
+    }
+  }
+  __syncthreads();
+  // values: a warp takes VALUES per lane of one group at a time
+  constexpr int VALUES = 4, UNITS = 2 * NT / VALUES;
+  for (int unit = warp; unit < sh.count * UNITS; unit += WARPS) {
+    const Group& grp = sh.groups[unit / UNITS];
+    const int v0 = unit % UNITS * VALUES;
+    float x[VALUES] = {};
+    for (uint32_t m = sh.have & (0xffffffffu << grp.from) & (0xffffffffu >> (32 - grp.to)); m != 0; m &= m - 1) {
+      const int piece = __ffs(m) - 1;
+      const float w = sh.weight[piece][g];
+      const float* p = piece_of(piece) + v0 * 32 + lane;
+#pragma unroll
+      for (int y = 0; y < VALUES; ++y) x[y] = fmaf(w, p[y * 32], x[y]);
+    }
+    long long head;
+    if (!head_of(grp.first.b, grp.first.row, g, head)) continue;
+    if (grp.whole) {
+#pragma unroll
+      for (int y = 0; y < VALUES; ++y) a.out[head * D + dim_of(v0 + y, lane)] = __float2bfloat16_rn(x[y]);
     } else {
-      float* out = a.partial + ((long long)blockIdx.x * 2 + (first.tile > 0 ? 0 : 1)) * (HEADS * (D + 2));
-      out[h * D + d] = value;
-      if (d == 0) {
-        out[HEADS * D + h] = top;
-        out[HEADS * D + HEADS + h] = total;
-      }
+      float* const out = merged + (grp.first.tile > 0 ? 0 : STEP) + v0 * 32 + lane;
+#pragma unroll
+      for (int y = 0; y < VALUES; ++y) out[y * 32] = x[y];
     }
   }
 
@@ -620,17 +716,16 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
   __syncthreads();
   if (tid == 0) {
     int joins = 0;
-    for (int gi = 0; gi < sh.groups; gi += max(1, sh.groups - 1)) {
-      Meta first, last;
-      ends_of(gi, first, last);
-      if (first.tile == 0 && last.tile + last.count == last.tiles) continue;
-      const int b0 = (int)(first.item / per_block), b1 = (int)((first.item + first.tiles - 1) / per_block);
+    for (int gi = 0; gi < sh.count; gi += max(1, sh.count - 1)) {
+      const Group& grp = sh.groups[gi];
+      if (grp.whole) continue;
+      const int b0 = grp.first.item / per_block, b1 = (grp.first.item + grp.first.tiles - 1) / per_block;
       if (atomicAdd(a.arrived + b0, 1u) == (unsigned)(b1 - b0)) {
         a.arrived[b0] = 0;
         sh.join_first[joins] = b0;
         sh.join_count[joins] = b1 - b0 + 1;
-        sh.join_b[joins] = first.b;
-        sh.join_row[joins++] = first.row;
+        sh.join_b[joins] = grp.first.b;
+        sh.join_row[joins++] = grp.first.row;
       }
     }
   }
@@ -639,12 +734,11 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
     const int n = sh.join_count[join];
     if (n == 0) break;
     __threadfence();
-    const auto part = [&](int j) {
-      return a.partial + ((long long)(sh.join_first[join] + j) * 2 + (j == 0 ? 1 : 0)) * (HEADS * (D + 2));
-    };
-    float* const weights = reinterpret_cast<float*>(rings);  // [n][HEADS], then the heads' tops and totals, then the columns
-    float* const tops = weights + n * HEADS;
-    float* const sums = tops + 2 * HEADS;
+    // the first block's piece is its second, the others' their first
+    const auto part = [&](int j) { return a.partial + ((long long)(sh.join_first[join] + j) * 2 + (j == 0 ? 1 : 0)) * STEP; };
+    float* const weights = reinterpret_cast<float*>(rings);  // [n][HEADS], then the heads' norms, then the copies' sums
+    float* const norms = weights + n * HEADS;
+    float* const sums = norms + HEADS;
     if (warp < real_heads) {  // one warp per head
       float top = -INFINITY, total = 0.f;
       for (int j = lane; j < n; j += 32) top = fmaxf(top, __ldcg(part(j) + HEADS * D + warp));
@@ -657,30 +751,35 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
       }
       for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
       if (lane == 0) {
-        tops[warp] = top;
-        tops[HEADS + warp] = total;
+        norms[warp] = total == 0.f ? 0.f : __fdividef(1.f, total);
+        long long head;
+        if (head_of(sh.join_b[join], sh.join_row[join], warp, head) && a.lse != nullptr)
+          a.lse[head] = total == 0.f ? -INFINITY : (top + fast_log2(total)) * LN2;
       }
     }
     __syncthreads();
-    const int quads = columns / 4, copies = S::THREADS / quads;  // 8 heads of 128 make 256 quads: one per thread
+    // a thread takes 4 neighbouring places (of one head); the threads left over take further parts of the list
+    const int quads = 2 * NT * real_heads, copies = S::THREADS / quads;
     const int quad = tid % quads, copy = tid / quads;
+    const int place = quad / real_heads * 32 + quad % real_heads * 4;
     if (copy < copies) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      const int h = quad * 4 / D;
 #pragma unroll 4
       for (int j = copy; j < n; j += copies) {
-        const float w = weights[j * HEADS + h];
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(part(j)) + quad);
+        const float w = weights[j * HEADS + quad % real_heads];
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(part(j) + place));
         acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
       }
       reinterpret_cast<float4*>(sums)[copy * quads + quad] = acc;
     }
     __syncthreads();
-    const Meta row{0, sh.join_b[join], sh.join_row[join], 0, 0, 0};
-    for (int x = tid; x < columns; x += S::THREADS) {
+    for (int x = tid; x < quads * 4; x += S::THREADS) {
       float value = 0.f;
-      for (int y = 0; y < copies; ++y) value += sums[y * columns + x];
-      finish(row, x / D, x % D, value, tops[x / D], tops[HEADS + x / D]);
+      for (int y = 0; y < copies; ++y) value += sums[y * quads * 4 + x];
+      const int v = x / (4 * real_heads), lane_ = x - v * 4 * real_heads;
+      long long head;
+      if (head_of(sh.join_b[join], sh.join_row[join], lane_ / 4, head))
+        a.out[head * D + dim_of(v, lane_)] = __float2bfloat16_rn(value * norms[lane_ / 4]);
     }
     __syncthreads();
   }
