@@ -11,17 +11,22 @@
 // Logits of -inf or NaN cannot be drawn; a row without any other gives token -1 and -inf.
 //
 // Bound: memory (the logits once, and the random numbers of the tokens that may be drawn); at a handful of
-// rows, the latency of the steps.  A row belongs to a cluster of blocks.  Each block holds its stretch of
-// the row in shared memory, so the row is read from memory once, and the cluster exchanges a few numbers
-// per step through distributed shared memory.
+// rows, the latency of the steps.  A row belongs to a cluster of blocks, which exchange a few numbers per step
+// through distributed shared memory.  There are three ways through a row, each with fewer steps than the next:
 //
-// * A cut is found without sorting: one histogram of all tokens over 2048 bins of falling logit (a bin per
-//   1/256 of an octave of 1 + distance from the best: narrow where the mass is), whose bins hold
-//   counts for top_k and masses for top_p, then the one bin that holds the boundary is resolved: its tokens
-//   are gathered and ranked against one another, or, if there are many, divided further by their bits.
-// * Masses are integers, round(w 2^31), split into halves of 16 bits that 32-bit shared-memory atomics add
-//   without overflow.  Integer sums do not depend on their order, so neither does the result.
-// * The total for the log-probability is summed so that its order does not show either (Sum).
+// * Nothing to cut (no top_k, top_p or min_p, or T <= 0): one pass over logits and random numbers with a running
+//   reference for the exponentials, rescaled by powers of two, so that no step waits for the maximum.
+// * Short prefix: the row is held in shared memory.  The median of the warps' largest logits is a threshold that
+//   some 100 tokens reach, whatever the distribution; they are sent to the first block, which ranks them against
+//   one another, cuts and draws.  Taken when those tokens provably hold both cuts; otherwise
+// * a lower threshold of the same kind, that some 1500 tokens reach, is tried, and then all tokens: a cut is found
+//   without sorting from a histogram over 2048 bins of falling logit, of counts for top_k and of masses for
+//   top_p.  The one bin that holds the boundary is resolved: its tokens are ranked against one another, or, if
+//   there are many, divided further by their bits (those of the index below those of the logit, so that equal
+//   logits divide too).  The first block does that for the 1500, the cluster for all.
+//
+// Masses are integers, round(w 2^31), split into halves of 16 bits that 32-bit shared-memory atomics add without
+// overflow.  Integer sums do not depend on their order, so neither do the cuts.
 #include <cooperative_groups.h>
 
 #include "generation.cuh"
@@ -33,7 +38,9 @@ namespace sampling {
 
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int BINS = 2048;
-constexpr int LIST = 1024;      // tokens of one bin that are ranked directly
+constexpr int LIST = 256;       // tokens of one bin that are ranked directly
+constexpr int SHORT = 256;      // tokens of a short prefix
+constexpr int MEDIUM = 2048;    // tokens of a longer one
 constexpr int MOST_BLOCKS = 8;  // of a cluster
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -93,16 +100,28 @@ struct Found {  // where a running sum over the bins crosses its target
   unsigned long long before;  // sum of the bins in front of it
 };
 
+struct Warp {
+  float reference;
+  double sum;
+  unsigned long long pick;
+};
+
 struct Shared {
+  Warp warps[MOST_BLOCKS][WARPS];
+  uint32_t warp_top[2][WARPS];
+  bool fine;
   uint32_t count[BINS], low[BINS], high[BINS];  // masses: 2^16 high + low
-  unsigned long long list[LIST];
-  uint32_t list_mass[LIST];
-  uint32_t listed;
+  unsigned long long list[MEDIUM], bin_list[LIST];
+  uint32_t list_mass[SHORT], bin_mass[LIST];
+  uint32_t listed, bin_listed;
   unsigned long long scan[WARPS];
   uint32_t reduce32[WARPS];
   unsigned long long slice[MOST_BLOCKS];                      // per block of the cluster
-  uint32_t keys[2][MOST_BLOCKS], ties[MOST_BLOCKS];           // likewise
+  uint32_t keys[3][MOST_BLOCKS];                              // likewise
+  unsigned long long ends[2][MOST_BLOCKS];                    // likewise
   double totals[MOST_BLOCKS], reduce64[WARPS];                // likewise
+  unsigned long long masses[MOST_BLOCKS];                     // likewise
+  uint32_t counts[MOST_BLOCKS];                               // likewise
   Found found;
   unsigned long long cut;
 };
@@ -143,11 +162,10 @@ struct Piece {
   }
 };
 
-// A bin per 1/256 of an octave of 1 + x / 2: bins of 1/128 up to a distance of 2, of 1/64 up to 6, and so on; all tokens
-// beyond 510 share the last bin.  Monotone in l, as every step of its computation is.
+// Bins of 1/64 of the exponent (to base e) for the first 32; everything further away shares the last bin.  Monotone in l,
+// as every step of its computation is.
 __device__ __forceinline__ int first_bin(const Weights& weight, float l) {
-  const float away = fmaf(weight.exponent(l), -0.5f * LN2, 1.f);
-  return min((int)(min(__float_as_uint(away), 0x43800000u) >> 15) - (0x3f800000 >> 15), BINS - 1);
+  return (int)fminf(weight.exponent(l) * (-64.f * LN2), (float)(BINS - 1));
 }
 
 template <typename T>
@@ -161,6 +179,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
   const int row = blockIdx.x / blocks, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const auto peer = [&](auto* p, int r) { return cluster.map_shared_rank(p, r); };
 
+  const float temperature = a.temperature[row];
+  const bool greedy = !(temperature > 0.f);
+  const int top_k = a.top_k[row];
+  const float top_p = a.top_p[row], min_p = a.min_p[row];
+  const bool by_count = !greedy && top_k > 0 && top_k < a.V, by_mass = !greedy && !(top_p >= 1.f);
+  const float* const noise = a.noise + row * a.noise_stride;
+
   // ---- this block's stretch of the row, as aligned pieces of 16 bytes; places outside the row hold -inf
   const T* const logits = static_cast<const T*>(a.logits) + row * a.row_stride;
   const int skew = (int)((reinterpret_cast<uintptr_t>(logits) % 16) / sizeof(T));
@@ -168,6 +193,137 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
   const int pieces = (skew + a.V + E - 1) / E, each = (pieces + blocks - 1) / blocks;
   const int from = min(rank * each, pieces), count = min(each, pieces - from);
   const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+  // A token outside the row's ends may not be read: f(index in the piece, token) for those inside.
+  const auto inside = [&](int i) {  // whether all of the piece belongs to the row
+    const int first = (from + i) * E - skew;
+    return first >= 0 && first + E <= a.V;
+  };
+  const auto end_piece = [&](int i) {  // a piece at one of the row's ends
+    uint32_t u[4] = {none, none, none, none};
+    for (int e = 0; e < E; ++e) {
+      const int token = (from + i) * E - skew + e;
+      if (token < 0 || token >= a.V) continue;
+      if constexpr (sizeof(T) == 4) u[e] = __float_as_uint(logits[token]);
+      else u[e / 2] = (u[e / 2] & (e % 2 ? 0xffffu : 0xffff0000u)) | ((uint32_t)__bfloat16_as_ushort(logits[token]) << (16 * (e % 2)));
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  };
+  const auto better = [](unsigned long long x, unsigned long long y) { return x > y ? x : y; };
+
+  // ---- one pass, where nothing is cut and the temperature is an ordinary one
+  if (!by_count && !by_mass && (greedy || (!(min_p > 0.f) && temperature > 1e-3f && temperature < 1e3f))) {
+    const double rate = 1.4426950408889634 / (greedy ? 1.0 : (double)temperature);
+    const float hi = (float)rate, lo = (float)(rate - (double)hi);
+    const bool together = (reinterpret_cast<uintptr_t>(noise - skew) % 16) == 0;
+    constexpr int DEPTH = E == 4 ? 8 : 4;  // pieces of a thread in flight: 128 bytes of random numbers
+    // all logits are on their way to shared memory before the first is used
+    for (int i = tid; i < count; i += THREADS)
+      if (inside(i))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(held + i)), "l"(aligned + from + i) : "memory");
+    float reference = -1e30f, best = greedy ? -INFINITY : -1.f, sum = 0.f;  // exponents are taken from `reference`, an integer
+    int winner = a.V;
+    for (int i0 = tid; i0 < count; i0 += DEPTH * THREADS) {
+      float4 luck[DEPTH][E / 4];
+#pragma unroll
+      for (int j = 0; j < DEPTH; ++j) {
+        const int i = i0 + j * THREADS;
+        if (!greedy && together && i < count && inside(i)) {
+#pragma unroll
+          for (int x = 0; x < E / 4; ++x) luck[j][x] = __ldcs(reinterpret_cast<const float4*>(noise + (from + i) * E - skew) + x);
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");  // a thread reads what it copied itself
+#pragma unroll
+      for (int j = 0; j < DEPTH; ++j) {
+        const int i = i0 + j * THREADS, first = (from + i) * E - skew;
+        if (i >= count) continue;
+        Piece<T> p(inside(i) ? held[i] : end_piece(i));
+        if (!greedy && !(together && inside(i))) {
+          float* const e = reinterpret_cast<float*>(luck[j]);
+#pragma unroll
+          for (int x = 0; x < E; ++x) e[x] = first + x >= 0 && first + x < a.V ? noise[first + x] : 1.f;
+        }
+        float top = -1e30f;
+#pragma unroll
+        for (int x = 0; x < E; ++x) {
+          p.v[x] = fmaxf(p.v[x], -1e30f);  // -inf and NaN: no weight at any ordinary temperature
+          top = fmaxf(top, p.v[x]);
+        }
+        if (!(top > -1e30f)) continue;  // nothing to draw here
+        if (top * hi > reference) {
+          const float higher = ceilf(top * hi), scale = fast_exp2(reference - higher);
+          sum *= scale;
+          if (!greedy && best > 0.f) best *= scale;
+          reference = higher;
+        }
+#pragma unroll
+        for (int x = 0; x < E; ++x) {
+          const float w = fast_exp2(fmaf(p.v[x], lo, fmaf(p.v[x], hi, -reference)));
+          sum += w;
+          // a NaN (from a random number that is none) loses to every score, but still names a token
+          const float score =
+              greedy ? p.v[x] : p.v[x] > -1e30f ? fmaxf(__fdividef(w, reinterpret_cast<const float*>(luck[j])[x]), -0.5f) : -1.f;
+          if (score > best) {
+            best = score;
+            winner = first + x;
+          }
+        }
+      }
+    }
+    float highest = reference;
+    for (int o = 16; o > 0; o >>= 1) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, o));
+    const float scale = fast_exp2(reference - highest);
+    if (!greedy && best > 0.f) best *= scale;
+    double of_warp = (double)(sum * scale);
+    unsigned long long pick = ((unsigned long long)key_of(best) << 32) | (0xffffffffu - (uint32_t)winner);
+    for (int o = 16; o > 0; o >>= 1) {
+      of_warp += __shfl_xor_sync(0xffffffffu, of_warp, o);
+      pick = better(pick, __shfl_xor_sync(0xffffffffu, pick, o));
+    }
+    // every warp sends its three numbers to every block, which come to the same conclusion
+    if (lane < blocks) {
+      Warp& to = *peer(&sh.warps[rank][warp], lane);
+      to.reference = highest;
+      to.sum = of_warp;
+      to.pick = pick;
+    }
+    cluster.sync();
+    const int n = blocks * WARPS;
+    if (warp == 0) {
+      const Warp* const all = &sh.warps[0][0];
+      float most = -INFINITY;
+      for (int i = lane; i < n; i += 32) most = fmaxf(most, all[i].reference);
+      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      // beyond this the products with the rate lose the differences (or a logit is infinite): the row is held instead
+      const bool fine = fabsf(most) < 1e5f;
+      double whole = 0.0;
+      unsigned long long choice = 0;
+      for (int i = lane; i < n; i += 32) {
+        const float down = fast_exp2(all[i].reference - most);
+        whole += all[i].sum * (double)down;
+        const uint32_t key = (uint32_t)(all[i].pick >> 32);
+        const float score = value_of(key);
+        choice = better(choice, greedy || !(score > 0.f) ? all[i].pick
+                                                        : ((unsigned long long)key_of(score * down) << 32) | (uint32_t)all[i].pick);
+      }
+      for (int o = 16; o > 0; o >>= 1) {
+        whole += __shfl_xor_sync(0xffffffffu, whole, o);
+        choice = better(choice, __shfl_xor_sync(0xffffffffu, choice, o));
+      }
+      if (lane == 0) {
+        sh.fine = fine;
+        if (fine && rank == 0) {
+          const int token = (int)(0xffffffffu - (uint32_t)choice);
+          const float l = Piece<T>::one(logits[token]);
+          a.token[row] = token;
+          a.logprob[row] = (fmaf(l, lo, fmaf(l, hi, -most)) - __log2f((float)whole)) * LN2;
+        }
+      }
+    }
+    __syncthreads();
+    if (sh.fine) return;
+  }
+
   float top = -INFINITY;  // of the thread's own pieces
   const auto keep_piece = [&](int i, uint4 raw) {
     uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -191,10 +347,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
     }
     held[i] = make_uint4(u[0], u[1], u[2], u[3]);
   };
-  const auto inside = [&](int i) {  // whether all of the piece belongs to the row
-    const int first = (from + i) * E - skew;
-    return first >= 0 && first + E <= a.V;
-  };
   {
     constexpr int DEPTH = 4;
     for (int i0 = tid; i0 < count; i0 += DEPTH * THREADS) {
@@ -209,26 +361,55 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
       for (int j = 0; j < DEPTH; ++j) {
         const int i = i0 + j * THREADS;
         if (i >= count) continue;
-        if (!inside(i)) {  // the row's ends
-          uint32_t u[4] = {none, none, none, none};
-          for (int e = 0; e < E; ++e) {
-            const int token = (from + i) * E - skew + e;
-            if (token < 0 || token >= a.V) continue;
-            if constexpr (sizeof(T) == 4) u[e] = __float_as_uint(logits[token]);
-            else u[e / 2] = (u[e / 2] & (e % 2 ? 0xffffu : 0xffff0000u)) | ((uint32_t)__bfloat16_as_ushort(logits[token]) << (16 * (e % 2)));
-          }
-          raw[j] = make_uint4(u[0], u[1], u[2], u[3]);
-        }
+        if (!inside(i)) raw[j] = end_piece(i);
         keep_piece(i, raw[j]);
       }
     }
   }
-  const auto larger = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
   const uint32_t own_top = key_of(top);
-  uint32_t best_key = block_reduce(own_top, sh.reduce32, larger);
-  if (tid < blocks) *peer(&sh.keys[0][rank], tid) = best_key;
-  cluster.sync();
-  for (int r = 0; r < blocks; ++r) best_key = max(best_key, sh.keys[0][r]);
+  // The block's largest key, and two thresholds: the medians over its warps of the largest keys of their lanes' (in smaller
+  // clusters the second, fourth or eighth largest), and of the tenth largest (in smaller clusters lower ones, so that
+  // the number of tokens above it stays).  Some tokens of every block reach the lowest of the blocks' medians.
+  uint32_t best_key = 0, threshold = 0xffffffffu, lower = 0xffffffffu;
+  {
+    int above = 0;
+#pragma unroll 8
+    for (int x = 0; x < 32; ++x) {
+      const uint32_t other = __shfl_sync(0xffffffffu, own_top, x);
+      above += other > own_top || (other == own_top && x < lane);
+    }
+    if (above == 0) sh.reduce32[warp] = own_top;
+    if (above == MOST_BLOCKS / blocks - 1) sh.warp_top[0][warp] = own_top;
+    if (above == (blocks == 8 ? 9 : blocks == 4 ? 15 : blocks == 2 ? 23 : 29)) sh.warp_top[1][warp] = own_top;
+    if (tid == 0) sh.listed = sh.bin_listed = 0u;
+    __syncthreads();
+    if (warp == 0) {
+      uint32_t medians[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const uint32_t mine = lane < WARPS ? sh.warp_top[y][lane] : 0u;
+        int higher = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const uint32_t other = __shfl_sync(0xffffffffu, mine, w);
+          higher += other > mine || (other == mine && w < lane);
+        }
+        medians[y] = __reduce_max_sync(0xffffffffu, lane < WARPS && higher == WARPS / 2 - 1 ? mine : 0u);
+      }
+      const uint32_t most = __reduce_max_sync(0xffffffffu, lane < WARPS ? sh.reduce32[lane] : 0u);
+      if (lane < blocks) {
+        *peer(&sh.keys[0][rank], lane) = most;
+        *peer(&sh.keys[1][rank], lane) = medians[0];
+        *peer(&sh.keys[2][rank], lane) = medians[1];
+      }
+    }
+    cluster.sync();
+    for (int r = 0; r < blocks; ++r) {
+      best_key = max(best_key, sh.keys[0][r]);
+      threshold = min(threshold, sh.keys[1][r]);
+      lower = min(lower, sh.keys[2][r]);
+    }
+  }
   if (best_key == 0u) {  // the same for every block of the cluster
     if (rank == 0 && tid == 0) {
       a.token[row] = -1;
@@ -237,12 +418,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
     return;
   }
 
-  const float temperature = a.temperature[row];
-  const bool greedy = !(temperature > 0.f);
   const Weights weight(value_of(best_key), greedy ? 1.f : temperature);
-  const int top_k = a.top_k[row];
-  const float top_p = a.top_p[row];
-  const bool by_count = !greedy && top_k > 0 && top_k < a.V, by_mass = !greedy && !(top_p >= 1.f);
 
   // Visits the thread's tokens that lie at or above a key: f(logit, index).  A thread whose largest logit is below has none.
   const auto visit = [&](uint32_t least, auto f) {
@@ -253,14 +429,24 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
       for (int e = 0; e < E; ++e) f(p.v[e], (from + i) * E - skew + e);
     }
   };
-  // A token as one number, in falling order of which the prefixes are cut.
+  // A token as one number, in falling order of which the prefixes are cut; all of them are different.
   const auto rank_of = [](float l, int token) { return ((unsigned long long)key_of(l) << 32) | (0xffffffffu - (uint32_t)token); };
+  const auto logit_of = [](unsigned long long number) { return value_of((uint32_t)(number >> 32)); };
 
-  unsigned long long cut = 1ull << 32;  // tokens at or above it stay: at first all but -inf
+  // Who looks for a cut: the cluster, among all tokens, or the first block, among those of its list.
+  const auto all_tokens = [&](unsigned long long least, auto f) {
+    visit((uint32_t)(least >> 32), [&](float l, int token) {
+      const unsigned long long number = rank_of(l, token);
+      if (number >= least) f(number);
+    });
+  };
+  const auto listed_tokens = [&](unsigned long long least, auto f) {
+    for (int i = tid; i < (int)sh.listed; i += THREADS)
+      if (sh.list[i] >= least) f(sh.list[i]);
+  };
 
   const auto clear_bins = [&] {
     for (int i = tid; i < BINS; i += THREADS) sh.count[i] = sh.low[i] = sh.high[i] = 0u;
-    if (tid == 0) sh.listed = 0u;
     __syncthreads();
   };
   const auto put = [&](int bin, float l, bool masses) {
@@ -271,24 +457,33 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
       if (w >> 16 != 0u) atomicAdd(&sh.high[bin], w >> 16);
     }
   };
-  // The sum over all bins of all blocks, and where the sum from the first bin on reaches `target` (of a share of the sum).
-  const auto cross = [&](bool masses, double share, unsigned long long target, unsigned long long& sum) {
-    cluster.sync();  // every block's bins are complete
-    const int slice = BINS / blocks;
+  // Where the sum over the bins of `n` blocks, from the first bin on, reaches `target`: the n-th token, or that mass.  Returns
+  // the sum of all bins; `target` of 0 stands for a share of it.
+  const auto cross = [&](auto wide, bool masses, double share, unsigned long long& target) {
+    constexpr bool WIDE = decltype(wide)::value;
+    const int n = WIDE ? blocks : 1, me = WIDE ? rank : 0;
+    const auto sync = [&] {
+      if (WIDE) cluster.sync();
+      else __syncthreads();
+    };
+    sync();  // every block's bins are complete
+    const int slice = BINS / n;
     constexpr int PER = BINS / THREADS;
-    const int own = min(PER, slice * PER / BINS + (slice * PER % BINS ? 1 : 0));  // bins of one thread
+    const int own = max(1, PER / n);  // bins of one thread
     unsigned long long mine[PER], upto = 0;
     uint32_t counts[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       mine[j] = 0;
       counts[j] = 0;
-      const int bin = rank * slice + tid * own + j;
+      const int bin = me * slice + tid * own + j;
       if (j < own && tid * own + j < slice) {
-        for (int r = 0; r < blocks; ++r) {
-          const uint32_t c = *peer(&sh.count[bin], r);
+        for (int r = 0; r < n; ++r) {
+          const uint32_t c = WIDE ? *peer(&sh.count[bin], r) : sh.count[bin];
           counts[j] += c;
-          mine[j] += masses ? *peer(&sh.low[bin], r) + ((unsigned long long)*peer(&sh.high[bin], r) << 16) : c;
+          if (masses) mine[j] += WIDE ? *peer(&sh.low[bin], r) + ((unsigned long long)*peer(&sh.high[bin], r) << 16)
+                                      : sh.low[bin] + ((unsigned long long)sh.high[bin] << 16);
+          else mine[j] += c;
         }
       }
       upto += mine[j];
@@ -300,248 +495,290 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
     }
     if (lane == 31) sh.scan[warp] = upto;
     __syncthreads();
-    unsigned long long total = 0;
+    unsigned long long sum = 0, base = 0;
     for (int w = 0; w < WARPS; ++w) {
       if (w < warp) upto += sh.scan[w];
-      total += sh.scan[w];
+      sum += sh.scan[w];
     }
-    if (tid < blocks) *peer(&sh.slice[rank], tid) = total;
-    cluster.sync();
-    sum = 0;
-    unsigned long long base = 0;
-    for (int r = 0; r < blocks; ++r) {
-      if (r < rank) base += sh.slice[r];
-      sum += sh.slice[r];
+    if (WIDE) {
+      if (tid < n) *peer(&sh.slice[me], tid) = sum;
+      cluster.sync();
+      sum = 0;
+      for (int r = 0; r < n; ++r) {
+        if (r < me) base += sh.slice[r];
+        sum += sh.slice[r];
+      }
     }
-    if (masses && target == 0) target = max(1ull, (unsigned long long)ceil(share * (double)sum));
+    if (target == 0) target = max(1ull, (unsigned long long)ceil(share * (double)sum));
     unsigned long long before = base + upto - of_thread;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       if (j < own && before < target && target <= before + mine[j]) {
-        const Found found{rank * slice + tid * own + j, counts[j], before};
-        for (int r = 0; r < blocks; ++r) *peer(&sh.found, r) = found;
+        const Found found{me * slice + tid * own + j, counts[j], before};
+        for (int r = 0; r < n; ++r) *(WIDE ? peer(&sh.found, r) : &sh.found) = found;
       }
       before += mine[j];
     }
-    cluster.sync();
-    return target;
+    sync();
+    return sum;
   };
 
-  // Cuts to the shortest prefix that holds `target` tokens, or `share` of the mass of what is left.
-  const auto shorten = [&](bool masses, double share, unsigned long long target) {
-    unsigned long long sum = 0;
-    target = cross(masses, share, target, sum);
-    if (sum < target) return;  // fewer tokens than top_k
-    Found found = sh.found;
-    uint32_t low_key = 0, high_key = 0;  // of the bin's tokens, once it has been divided
-    bool divided = false;
-    int bin = found.bin;
-    unsigned long long before = found.before;
-    const auto member = [&](float l, int token) {
-      if (rank_of(l, token) < cut) return false;
-      return divided ? key_of(l) >= low_key && key_of(l) <= high_key : first_bin(weight, l) == bin;
+  // The lowest token of the shortest prefix of those at or above `cut` that holds `target` tokens, or (target 0) `share` of
+  // their mass.
+  const auto shorten = [&](auto wide, const auto& tokens, unsigned long long cut, bool masses, double share, unsigned long long target) {
+    constexpr bool WIDE = decltype(wide)::value;
+    const int n = WIDE ? blocks : 1;
+    const auto sync = [&] {
+      if (WIDE) cluster.sync();
+      else __syncthreads();
     };
-    while (found.count > LIST && !(divided && low_key == high_key)) {
-      if (!divided) {
-        uint32_t least = 0xffffffffu, most = 0u;
-        visit((uint32_t)(cut >> 32), [&](float l, int token) {
-          if (member(l, token)) {
-            least = min(least, key_of(l));
-            most = max(most, key_of(l));
-          }
-        });
-        least = block_reduce(least, sh.reduce32, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
-        most = block_reduce(most, sh.reduce32, larger);
-        if (tid < blocks) {
-          *peer(&sh.keys[0][rank], tid) = least;
-          *peer(&sh.keys[1][rank], tid) = most;
-        }
-        cluster.sync();
-        low_key = 0xffffffffu;
-        for (int r = 0; r < blocks; ++r) {
-          low_key = min(low_key, sh.keys[0][r]);
-          high_key = max(high_key, sh.keys[1][r]);
-        }
-        divided = true;
-        continue;
-      }
-      int shift = 0;
-      while ((high_key - low_key) >> shift >= BINS) ++shift;
-      clear_bins();
-      visit(low_key, [&](float l, int token) {
-        if (member(l, token)) put((high_key - key_of(l)) >> shift, l, masses);
+    clear_bins();
+    tokens(cut, [&](unsigned long long number) { put(first_bin(weight, logit_of(number)), logit_of(number), masses); });
+    if (cross(wide, masses, share, target) < target) return cut;  // fewer tokens than top_k
+    Found found = sh.found;
+    const int bin = found.bin;
+    unsigned long long before = found.before, low = cut, high = ~0ull;  // bounds of the bin's tokens, once it has been divided
+    bool divided = false;
+    const auto members = [&](auto f) {
+      tokens(low, [&](unsigned long long number) {
+        if (divided ? number <= high : first_bin(weight, logit_of(number)) == bin) f(number);
       });
-      cross(masses, share, target - before, sum);
+    };
+    while (found.count > LIST) {
+      if (!divided) {
+        unsigned long long least = ~0ull, most = 0ull;
+        members([&](unsigned long long number) {
+          least = min(least, number);
+          most = max(most, number);
+        });
+        least = block_reduce(least, sh.scan, [](unsigned long long x, unsigned long long y) { return x < y ? x : y; });
+        most = block_reduce(most, sh.scan, better);
+        if (WIDE) {
+          if (tid < n) {
+            *peer(&sh.ends[0][rank], tid) = least;
+            *peer(&sh.ends[1][rank], tid) = most;
+          }
+          cluster.sync();
+          for (int r = 0; r < n; ++r) {
+            least = min(least, sh.ends[0][r]);
+            most = max(most, sh.ends[1][r]);
+          }
+        }
+        low = least;
+        high = most;
+        divided = true;
+      }
+      const int shift = max(0, 64 - __clzll((long long)(high - low)) - 11);  // 2^11 bins
+      clear_bins();
+      members([&](unsigned long long number) { put((int)((high - number) >> shift), logit_of(number), masses); });
+      unsigned long long left = target - before;
+      cross(wide, masses, share, left);
       found = sh.found;
       before += found.before;
-      high_key -= (uint32_t)found.bin << shift;
-      low_key = max(low_key, high_key - (uint32_t)((1ull << shift) - 1));
+      high -= (unsigned long long)found.bin << shift;
+      low = max(low, high - ((1ull << shift) - 1));
     }
-    if (found.count <= LIST) {
-      // The first block ranks the bin's tokens against one another.
-      visit(divided ? low_key : (uint32_t)(cut >> 32), [&](float l, int token) {
-        if (!member(l, token)) return;
-        const uint32_t at = atomicAdd(peer(&sh.listed, 0), 1u);
-        *peer(&sh.list[at], 0) = rank_of(l, token);
-        *peer(&sh.list_mass[at], 0) = masses ? weight.fixed(l) : 1u;
-      });
-      cluster.sync();
-      if (rank == 0) {
-        unsigned long long last = ~0ull;
-        for (int i = tid; i < (int)found.count; i += THREADS) {
-          const unsigned long long mine = sh.list[i];
-          unsigned long long ahead = before;
-          for (int j = 0; j < (int)found.count; ++j)
-            if (sh.list[j] > mine) ahead += sh.list_mass[j];
-          if (ahead < target) last = min(last, mine);
-        }
-        last = block_reduce(last, sh.scan, [](unsigned long long x, unsigned long long y) { return x < y ? x : y; });
-        if (tid < blocks) *peer(&sh.cut, tid) = last;
-      }
-      cluster.sync();
-      cut = sh.cut;
-      return;
+    // The first block ranks the bin's tokens against one another.
+    members([&](unsigned long long number) {
+      const uint32_t at = atomicAdd(WIDE ? peer(&sh.bin_listed, 0) : &sh.bin_listed, 1u);
+      *(WIDE ? peer(&sh.bin_list[at], 0) : &sh.bin_list[at]) = number;
+      *(WIDE ? peer(&sh.bin_mass[at], 0) : &sh.bin_mass[at]) = masses ? weight.fixed(logit_of(number)) : 1u;
+    });
+    sync();
+    if (!WIDE || rank == 0) {
+      constexpr int PARTS = THREADS / LIST;
+      const int mine = tid / PARTS;
+      const unsigned long long me = mine < (int)found.count ? sh.bin_list[mine] : ~0ull;
+      unsigned long long ahead = 0;
+      for (int j = tid % PARTS; j < (int)found.count; j += PARTS)
+        if (sh.bin_list[j] > me) ahead += sh.bin_mass[j];
+      for (int o = PARTS / 2; o > 0; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+      const unsigned long long last =
+          block_reduce(before + ahead < target ? me : ~0ull, sh.scan, [](unsigned long long x, unsigned long long y) { return x < y ? x : y; });
+      if (tid < n) *(WIDE ? peer(&sh.cut, tid) : &sh.cut) = last;
+      if (tid == 0) sh.bin_listed = 0u;
     }
-    // Many equal logits: the first n of them, in the order of their index, stay.
-    const unsigned long long w = masses ? weight.fixed(value_of(high_key)) : 1ull;
-    unsigned long long n = (target - before + w - 1) / w;
-    uint32_t equal = 0;
-    visit(high_key, [&](float l, int token) { equal += key_of(l) == high_key && rank_of(l, token) >= cut; });
-    const uint32_t of_block = block_reduce(equal, sh.reduce32, [](uint32_t x, uint32_t y) { return x + y; });
-    if (tid < blocks) *peer(&sh.ties[rank], tid) = of_block;
-    cluster.sync();
-    for (int r = 0; r < rank; ++r) n -= min(n, (unsigned long long)sh.ties[r]);
-    if (n >= 1 && n <= of_block) {  // the last one is in this block: count on in the order of the index
-      uint32_t seen = 0;
-      for (int i0 = 0; i0 < count; i0 += THREADS) {
-        uint32_t here = 0;
-        const int i = i0 + tid;
-        if (i < count) {
-          const Piece<T> p(held[i]);
-#pragma unroll
-          for (int e = 0; e < E; ++e) here += key_of(p.v[e]) == high_key && rank_of(p.v[e], (from + i) * E - skew + e) >= cut;
-        }
-        uint32_t upto = here;
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t other = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += other;
-        }
-        __syncthreads();
-        if (lane == 31) sh.reduce32[warp] = upto;
-        __syncthreads();
-        uint32_t all = 0;
-        for (int x = 0; x < WARPS; ++x) {
-          if (x < warp) upto += sh.reduce32[x];
-          all += sh.reduce32[x];
-        }
-        uint32_t ahead = seen + upto - here;
-        if (ahead < n && n <= ahead + here) {
-          const Piece<T> p(held[i]);
-          for (int e = 0; e < E; ++e) {
-            const int token = (from + i) * E - skew + e;
-            if (key_of(p.v[e]) == high_key && rank_of(p.v[e], token) >= cut && ++ahead == n)
-              for (int r = 0; r < blocks; ++r) *peer(&sh.cut, r) = rank_of(p.v[e], token);
-          }
-        }
-        seen += all;
-      }
-    }
-    cluster.sync();
-    cut = sh.cut;
+    sync();
+    return sh.cut;
   };
+  using Cluster = std::integral_constant<bool, true>;
+  using Block = std::integral_constant<bool, false>;
 
   Sum total;
-  if (by_count || by_mass) {
-    clear_bins();
-    const bool masses = !by_count;
-    visit(0u, [&](float l, int) {
-      total.add(weight(l));
-      if (l > -INFINITY) put(first_bin(weight, l), l, masses);
-    });
-    shorten(masses, top_p, by_count ? top_k : 0);
-    if (by_count && by_mass) {
-      clear_bins();
-      visit((uint32_t)(cut >> 32), [&](float l, int token) {
-        if (rank_of(l, token) >= cut) put(first_bin(weight, l), l, true);
-      });
-      shorten(true, top_p, 0);
-    }
-  }
-
-  // ---- the race
-  const float min_p = a.min_p[row];
-  const float* const noise = a.noise + row * a.noise_stride;
-  float best_score = -1.f;
-  int winner = a.V;
-  const auto run = [&](float l, float e, int token) {
-    const float w = weight(l);
-    // a NaN (from a random number that is none) loses to every score, but still names a token
-    const float score = fmaxf(__fdividef(w, e), -0.5f);
-    if (score > best_score && (w >= min_p || l == weight.best)) {
-      best_score = score;
-      winner = token;
-    }
-    return w;
-  };
-  if (greedy) {
+  // ---- a short prefix: the tokens that reach the threshold, ranked by the first block
+  threshold = max(threshold, 1u);
+  {
+    const float least = value_of(threshold);
+    uint32_t sent = 0;
+    unsigned long long sent_mass = 0;
     visit(0u, [&](float l, int token) {
       total.add(weight(l));
-      if (l == weight.best && token < winner) winner = token, best_score = 1.f;
-    });
-  } else if (by_count || by_mass) {
-    visit((uint32_t)(cut >> 32), [&](float l, int token) {
-      if (rank_of(l, token) >= cut) run(l, noise[token], token);
-    });
-  } else if (min_p > 0.f) {
-    visit(0u, [&](float l, int token) {
-      const float w = weight(l);
-      total.add(w);
-      if (w >= min_p || l == weight.best) run(l, noise[token], token);
-    });
-  } else {
-    // every token: whole pieces of the random numbers where the two rows are aligned to one another
-    const bool together = (reinterpret_cast<uintptr_t>(noise - skew) % 16) == 0;
-    for (int i = tid; i < count; i += THREADS) {
-      const Piece<T> p(held[i]);
-      const int first = (from + i) * E - skew;
-      float e[E];
-      if (together && inside(i)) {
-#pragma unroll
-        for (int j = 0; j < E / 4; ++j) {
-          const float4 x = __ldcs(reinterpret_cast<const float4*>(noise + first) + j);
-          e[4 * j] = x.x, e[4 * j + 1] = x.y, e[4 * j + 2] = x.z, e[4 * j + 3] = x.w;
+      if (l >= least) {
+        const uint32_t at = atomicAdd(peer(&sh.listed, 0), 1u), mass = weight.fixed(l);
+        if (at < SHORT) {
+          *peer(&sh.list[at], 0) = rank_of(l, token);
+          *peer(&sh.list_mass[at], 0) = mass;
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < E; ++j) e[j] = first + j >= 0 && first + j < a.V ? noise[first + j] : 1.f;
+        ++sent;
+        sent_mass += mass;
       }
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (p.v[j] > -INFINITY) total.add(run(p.v[j], e[j], first + j));
+    });
+    double of_warp = total.value();
+    sent = __reduce_add_sync(0xffffffffu, sent);
+    for (int o = 16; o > 0; o >>= 1) {
+      of_warp += __shfl_xor_sync(0xffffffffu, of_warp, o);
+      sent_mass += __shfl_xor_sync(0xffffffffu, sent_mass, o);
+    }
+    if (lane == 0) {
+      sh.reduce64[warp] = of_warp;
+      sh.scan[warp] = sent_mass;
+      sh.reduce32[warp] = sent;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      of_warp = lane < WARPS ? sh.reduce64[lane] : 0.0;
+      sent_mass = lane < WARPS ? sh.scan[lane] : 0ull;
+      sent = __reduce_add_sync(0xffffffffu, lane < WARPS ? sh.reduce32[lane] : 0u);
+      for (int o = WARPS / 2; o > 0; o >>= 1) {
+        of_warp += __shfl_xor_sync(0xffffffffu, of_warp, o);
+        sent_mass += __shfl_xor_sync(0xffffffffu, sent_mass, o);
+      }
+      of_warp = __shfl_sync(0xffffffffu, of_warp, 0);
+      sent_mass = __shfl_sync(0xffffffffu, sent_mass, 0);
+      if (lane < blocks) {
+        *peer(&sh.totals[rank], lane) = of_warp;
+        *peer(&sh.masses[rank], lane) = sent_mass;
+        *peer(&sh.counts[rank], lane) = sent;
+      }
+    }
+    cluster.sync();
+    double whole = 0.0;
+    unsigned long long held_mass = 0;
+    uint32_t n = 0;
+    for (int r = 0; r < blocks; ++r) {
+      whole += sh.totals[r];
+      held_mass += sh.masses[r];
+      n += sh.counts[r];
+    }
+    unsigned long long limit = max(1ull, (unsigned long long)ceil((double)top_p * whole * 2147483648.0));
+    const bool holds = greedy || (by_count ? n >= (uint32_t)top_k : by_mass ? held_mass >= limit : min_p > 0.f && weight(least) < min_p);
+    if (n <= SHORT && holds) {
+      if (rank != 0) return;
+      // `parts` neighbouring threads share a token
+      int parts = 1;
+      while (parts < 32 && (int)n * parts * 2 <= THREADS) parts *= 2;
+      const int mine = tid / parts;
+      const bool on = mine < (int)n;
+      const unsigned long long me = on ? sh.list[mine] : 0ull;
+      const uint32_t my_mass = on ? sh.list_mass[mine] : 0u;
+      const int token = (int)(0xffffffffu - (uint32_t)me);
+      const float luck = on && !greedy ? noise[token] : 1.f;
+      uint32_t ahead = 0;
+      unsigned long long mass_ahead = 0;
+      if (on) {
+        for (int j = tid % parts; j < (int)n; j += parts) {
+          if (sh.list[j] > me) {
+            ++ahead;
+            mass_ahead += sh.list_mass[j];
+          }
+        }
+      }
+      for (int o = parts / 2; o > 0; o >>= 1) {
+        ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+        mass_ahead += __shfl_xor_sync(0xffffffffu, mass_ahead, o);
+      }
+      bool stays = on && (!by_count || ahead < (uint32_t)top_k);
+      if (by_mass) {
+        if (by_count) {
+          const unsigned long long left =
+              block_reduce(stays && tid % parts == 0 ? (unsigned long long)my_mass : 0ull, sh.scan, [](unsigned long long x, unsigned long long y) { return x + y; });
+          limit = max(1ull, (unsigned long long)ceil((double)top_p * (double)left));
+        }
+        stays = stays && mass_ahead < limit;
+      }
+      const float l = value_of((uint32_t)(me >> 32)), w = weight(l);
+      stays = stays && (greedy ? ahead == 0 : w >= min_p || l == weight.best);
+      const float score = stays ? fmaxf(__fdividef(w, luck), -0.5f) : -1.f;
+      const unsigned long long first =
+          block_reduce(((unsigned long long)key_of(score) << 32) | (0xffffffffu - (uint32_t)token), sh.scan, better);
+      if (tid == 0) {
+        const int drawn = (int)(0xffffffffu - (uint32_t)first);
+        a.token[row] = drawn;
+        a.logprob[row] = (weight.exponent(Piece<T>::one(logits[drawn])) - __log2f((float)whole)) * LN2;
+      }
+      return;
     }
   }
 
-  // ---- over the block and the cluster
-  const double of_block = block_reduce(total.value(), sh.reduce64, [](double x, double y) { return x + y; });
-  const auto better = [](unsigned long long x, unsigned long long y) { return x > y ? x : y; };
-  const unsigned long long first_of =
-      block_reduce(((unsigned long long)key_of(best_score) << 32) | (0xffffffffu - (uint32_t)winner), sh.scan, better);
-  if (tid == 0) {
-    *peer(&sh.totals[rank], 0) = of_block;
-    *peer(&sh.slice[rank], 0) = first_of;
-  }
-  cluster.sync();
-  if (rank == 0 && tid == 0) {
-    unsigned long long most = 0;
-    double sum = 0.0;
-    for (int r = 0; r < blocks; ++r) {
-      most = better(most, sh.slice[r]);
-      sum += sh.totals[r];
-    }
-    const int token = (int)(0xffffffffu - (uint32_t)most);
-    const float l = Piece<T>::one(logits[token]);
+  // ---- a longer one, or all tokens
+  const auto cut_both = [&](auto wide, const auto& tokens, unsigned long long limit) {
+    unsigned long long cut = 1ull << 32;  // all but -inf
+    if (by_count) cut = shorten(wide, tokens, cut, false, 0.0, top_k);
+    if (by_mass) cut = shorten(wide, tokens, cut, true, top_p, by_count ? 0 : limit);
+    return cut;
+  };
+  // The race among the tokens at or above `cut`: (score, lowest index) of the block's best as one ordered number.
+  const auto race = [&](const auto& tokens, unsigned long long cut) {
+    float best_score = -1.f;
+    uint32_t winner = 0xffffffffu;
+    tokens(cut, [&](unsigned long long number) {
+      const float l = logit_of(number), w = weight(l);
+      const uint32_t token = 0xffffffffu - (uint32_t)number;
+      if (l != weight.best && (greedy || !(w >= min_p))) return;
+      const float score = greedy ? 1.f : fmaxf(__fdividef(w, noise[token]), -0.5f);
+      if (score > best_score || (score == best_score && token < winner)) {
+        best_score = score;
+        winner = token;
+      }
+    });
+    return block_reduce(((unsigned long long)key_of(best_score) << 32) | (0xffffffffu - winner), sh.scan, better);
+  };
+  double whole = 0.0;
+  for (int r = 0; r < blocks; ++r) whole += sh.totals[r];
+  const unsigned long long limit = max(1ull, (unsigned long long)ceil((double)top_p * whole * 2147483648.0));
+  const auto finish = [&](unsigned long long first) {
+    if (tid != 0) return;
+    const int token = (int)(0xffffffffu - (uint32_t)first);
     a.token[row] = token;
-    a.logprob[row] = (weight.exponent(l) - __log2f((float)sum)) * LN2;
+    a.logprob[row] = (weight.exponent(Piece<T>::one(logits[token])) - __log2f((float)whole)) * LN2;
+  };
+  if (by_count || by_mass) {
+    if (tid == 0) sh.listed = 0u;
+    cluster.sync();
+    const unsigned long long least = (unsigned long long)max(lower, 1u) << 32;
+    uint32_t sent = 0;
+    unsigned long long sent_mass = 0;
+    all_tokens(least, [&](unsigned long long number) {
+      const uint32_t at = atomicAdd(peer(&sh.listed, 0), 1u);
+      if (at < MEDIUM) *peer(&sh.list[at], 0) = number;
+      ++sent;
+      sent_mass += weight.fixed(logit_of(number));
+    });
+    const auto add = [](unsigned long long x, unsigned long long y) { return x + y; };
+    sent_mass = block_reduce(sent_mass, sh.scan, add);
+    const unsigned long long sent_all = block_reduce((unsigned long long)sent, sh.scan, add);
+    if (tid < blocks) {
+      *peer(&sh.masses[rank], tid) = sent_mass;
+      *peer(&sh.slice[rank], tid) = sent_all;
+    }
+    cluster.sync();
+    unsigned long long held_mass = 0, n = 0;
+    for (int r = 0; r < blocks; ++r) {
+      held_mass += sh.masses[r];
+      n += sh.slice[r];
+    }
+    if (n <= MEDIUM && (by_count ? n >= (unsigned long long)top_k : held_mass >= limit)) {
+      if (rank == 0) finish(race(listed_tokens, cut_both(Block(), listed_tokens, limit)));
+      return;
+    }
+  }
+  const unsigned long long first = race(all_tokens, cut_both(Cluster(), all_tokens, limit));
+  if (tid == 0) *peer(&sh.slice[rank], 0) = first;
+  cluster.sync();
+  if (rank == 0) {
+    unsigned long long most = 0;
+    for (int r = 0; r < blocks; ++r) most = better(most, sh.slice[r]);
+    finish(most);
   }
 }
 
@@ -577,9 +814,12 @@ static cudaError_t launch_as(const Args& a, int blocks, cudaStream_t stream) {
 }
 
 cudaError_t launch(const Args& a, int sms, cudaStream_t stream) {
-  // blocks per row: a block of 512 threads with at least a piece of 16 bytes for each, at most 8
+  // Blocks per row: as many as let two of them share an SM (72 KB of the row each), and more while all of them run at
+  // once and have some tokens for each thread.
+  const int size = a.wide ? 4 : 2;
   int blocks = 1;
-  while (blocks < MOST_BLOCKS && a.V > blocks * 4096) blocks *= 2;
+  while (blocks < MOST_BLOCKS && (long long)a.V * size > blocks * 73728ll) blocks *= 2;
+  while (blocks < MOST_BLOCKS && (long long)a.B * blocks <= sms && a.V > blocks * 4096) blocks *= 2;
   return a.wide ? launch_as<float>(a, blocks, stream) : launch_as<__nv_bfloat16>(a, blocks, stream);
 }
 
