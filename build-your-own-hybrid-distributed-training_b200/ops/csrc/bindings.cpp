@@ -47,14 +47,17 @@ void attention_backward(at::Tensor qkv, at::Tensor out, at::Tensor dout, at::Ten
                         int64_t H, int64_t HKV, int64_t D, bool causal, double scale, int64_t q_begin, int64_t q_len);
 void kv_cache_write(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale, c10::optional<at::Tensor> v_scale,
                     at::Tensor k, at::Tensor v, at::Tensor slots);
-void kv_cache_read(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale, c10::optional<at::Tensor> v_scale,
-                   at::Tensor slots, at::Tensor k, at::Tensor v);
-void paged_attention(at::Tensor q, at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale,
-                     c10::optional<at::Tensor> v_scale, at::Tensor block_table, at::Tensor lengths, at::Tensor out,
-                     c10::optional<at::Tensor> lse, double scale);
-void sample_tokens(at::Tensor logits, at::Tensor noise, c10::optional<at::Tensor> temperature_rows, double temperature,
-                   c10::optional<at::Tensor> top_k_rows, int64_t top_k, c10::optional<at::Tensor> top_p_rows, double top_p,
-                   c10::optional<at::Tensor> min_p_rows, double min_p, at::Tensor token, at::Tensor logprob);
+std::tuple<at::Tensor, at::Tensor> kv_cache_read(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale,
+                                                 c10::optional<at::Tensor> v_scale, at::Tensor slots, c10::optional<at::Tensor> k_out,
+                                                 c10::optional<at::Tensor> v_out);
+std::tuple<at::Tensor, c10::optional<at::Tensor>> paged_attention(at::Tensor q, at::Tensor k_pool, at::Tensor v_pool,
+                                                                  c10::optional<at::Tensor> k_scale, c10::optional<at::Tensor> v_scale,
+                                                                  at::Tensor block_table, at::Tensor lengths, c10::optional<double> scale,
+                                                                  bool with_lse);
+std::tuple<at::Tensor, at::Tensor> sample_tokens(at::Tensor logits, at::Tensor noise, c10::optional<at::Tensor> temperature_rows,
+                                                 double temperature, c10::optional<at::Tensor> top_k_rows, int64_t top_k,
+                                                 c10::optional<at::Tensor> top_p_rows, double top_p,
+                                                 c10::optional<at::Tensor> min_p_rows, double min_p);
 void bucket_all_reduce(at::Tensor flat, std::vector<int64_t> buffer_ptrs, std::vector<int64_t> pad_ptrs, int64_t multicast_ptr,
                        int64_t start, int64_t numel, double scale, int64_t rank, int64_t slot_base, int64_t max_blocks,
                        at::Tensor status, double timeout_s, bool wide, int64_t min_peer_slots);

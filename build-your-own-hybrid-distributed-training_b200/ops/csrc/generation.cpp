@@ -3,6 +3,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <utility>
@@ -55,6 +56,11 @@ void check_rows(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slot
   HT_CHECK(slots.device() == pool.device() && (slots.scalar_type() == at::kLong || slots.scalar_type() == at::kInt) && slots.dim() == 1 &&
                slots.size(0) == k.size(0),
            "slots must be int32 or int64, one per token, on the pool's device");
+  HT_CHECK(k.size(0) <= (1ll << 30) / pool.size(1), "too many rows (tokens x heads) for one call: split it");
+}
+
+void check_no_gradient(const at::Tensor& x, const char* what) {
+  HT_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()), what, " has no gradient: call it under torch.no_grad()");
 }
 
 // Rows that 16-byte accesses can take.
@@ -105,6 +111,8 @@ void kv_cache_write(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tens
                     at::Tensor k, at::Tensor v, at::Tensor slots) {
   const kv::Pool p = checked_pool(k_pool, v_pool, k_scale, v_scale);
   check_rows(k, v, slots, k_pool);
+  check_no_gradient(k, "kv_cache_write");
+  check_no_gradient(v, "kv_cache_write");
   if (k.size(0) == 0) return;
   const c10::cuda::CUDAGuard guard(k_pool.device());
   // rows of another order or alignment are copied first
@@ -121,12 +129,16 @@ void kv_cache_write(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tens
   check_launch(kv::launch_write(a, sms(), at::cuda::getCurrentCUDAStream()), "kv_cache_write");
 }
 
-void kv_cache_read(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale, c10::optional<at::Tensor> v_scale,
-                   at::Tensor slots, at::Tensor k, at::Tensor v) {
+std::tuple<at::Tensor, at::Tensor> kv_cache_read(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale,
+                                                 c10::optional<at::Tensor> v_scale, at::Tensor slots, c10::optional<at::Tensor> k_out,
+                                                 c10::optional<at::Tensor> v_out) {
   const kv::Pool p = checked_pool(k_pool, v_pool, k_scale, v_scale);
-  check_rows(k, v, slots, k_pool);
-  if (k.size(0) == 0) return;
   const c10::cuda::CUDAGuard guard(k_pool.device());
+  HT_CHECK(slots.dim() == 1 && k_out.has_value() == v_out.has_value(), "slots must be a vector, and out a pair");
+  const auto fresh = [&] { return at::empty({slots.size(0), p.Hkv, p.D}, k_pool.options().dtype(at::kBFloat16)); };
+  at::Tensor k = k_out.has_value() ? *k_out : fresh(), v = v_out.has_value() ? *v_out : fresh();
+  check_rows(k, v, slots, k_pool);
+  if (k.size(0) == 0) return {k, v};
   HT_CHECK(vector_rows(k) && vector_rows(v), "k and v must have unit inner stride and rows on 16-byte boundaries");
   if (slots.size(0) > 1) slots = slots.contiguous();
   const kv::ReadArgs a{p,
@@ -137,12 +149,15 @@ void kv_cache_read(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tenso
                        k.size(0),
                        slots.scalar_type() == at::kLong};
   check_launch(kv::launch_read(a, sms(), at::cuda::getCurrentCUDAStream()), "kv_cache_read");
+  return {k, v};
 }
 
-void paged_attention(at::Tensor q, at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_scale,
-                     c10::optional<at::Tensor> v_scale, at::Tensor block_table, at::Tensor lengths, at::Tensor out,
-                     c10::optional<at::Tensor> lse, double scale) {
+std::tuple<at::Tensor, c10::optional<at::Tensor>> paged_attention(at::Tensor q, at::Tensor k_pool, at::Tensor v_pool,
+                                                                  c10::optional<at::Tensor> k_scale, c10::optional<at::Tensor> v_scale,
+                                                                  at::Tensor block_table, at::Tensor lengths, c10::optional<double> scale,
+                                                                  bool with_lse) {
   const kv::Pool p = checked_pool(k_pool, v_pool, k_scale, v_scale);
+  check_no_gradient(q, "paged_attention");
   HT_CHECK(q.device() == k_pool.device() && q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.size(2) == p.D &&
                q.size(1) % p.Hkv == 0 && q.size(1) > 0 && q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX,
            "q must be bf16 [B, H, ", p.D, "] on the pool's device with H a multiple of the pool's ", p.Hkv, " heads");
@@ -155,29 +170,27 @@ void paged_attention(at::Tensor q, at::Tensor k_pool, at::Tensor v_pool, c10::op
   HT_CHECK(lengths.device() == q.device() && lengths.scalar_type() == at::kInt && lengths.is_contiguous() && lengths.dim() == 1 &&
                lengths.size(0) == B,
            "lengths must be a contiguous int32 tensor [B] on the pool's device");
-  HT_CHECK(out.device() == q.device() && out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.sizes() == q.sizes(),
-           "out must be contiguous bf16 [B, H, D]");
-  if (B == 0) return;
   const c10::cuda::CUDAGuard guard(k_pool.device());
+  at::Tensor out = at::empty({B, H, p.D}, q.options().requires_grad(false));
+  c10::optional<at::Tensor> lse;
+  if (with_lse) lse = at::empty({B, H}, q.options().dtype(at::kFloat).requires_grad(false));
+  if (B == 0) return {out, lse};
   if (!vector_rows(q)) q = q.clone(at::MemoryFormat::Contiguous);
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   paged::Args a{reinterpret_cast<const __nv_bfloat16*>(q.data_ptr()), q.stride(0), q.stride(1), p, block_table.data_ptr<int>(),
                 block_table.stride(0), (int)block_table.size(1), lengths.data_ptr<int>(),
-                reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), nullptr, (int)B, (int)H, (float)(scale * 1.4426950408889634),
-                nullptr, nullptr};
-  if (lse.has_value() && lse->defined()) {
-    HT_CHECK(lse->device() == q.device() && lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->numel() == B * H,
-             "lse must be contiguous fp32 [B, H]");
-    a.lse = lse->data_ptr<float>();
-  }
+                reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), with_lse ? lse->data_ptr<float>() : nullptr, (int)B, (int)H,
+                (float)((scale.has_value() ? *scale : 1.0 / std::sqrt((double)p.D)) * 1.4426950408889634), nullptr, nullptr};
   at::Tensor keep;
   std::tie(a.partial, a.arrived) = attention_scratch(q, stream, keep);
   check_launch(paged::launch(a, sms(), stream), "paged_attention");
+  return {out, lse};
 }
 
-void sample_tokens(at::Tensor logits, at::Tensor noise, c10::optional<at::Tensor> temperature_rows, double temperature,
-                   c10::optional<at::Tensor> top_k_rows, int64_t top_k, c10::optional<at::Tensor> top_p_rows, double top_p,
-                   c10::optional<at::Tensor> min_p_rows, double min_p, at::Tensor token, at::Tensor logprob) {
+std::tuple<at::Tensor, at::Tensor> sample_tokens(at::Tensor logits, at::Tensor noise, c10::optional<at::Tensor> temperature_rows,
+                                                 double temperature, c10::optional<at::Tensor> top_k_rows, int64_t top_k,
+                                                 c10::optional<at::Tensor> top_p_rows, double top_p,
+                                                 c10::optional<at::Tensor> min_p_rows, double min_p) {
   HT_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat),
            "logits must be a CUDA bf16 or fp32 tensor [B, V]");
   const int64_t B = logits.size(0), V = logits.size(1);
@@ -185,11 +198,13 @@ void sample_tokens(at::Tensor logits, at::Tensor noise, c10::optional<at::Tensor
            " tokens and up to 2^24 rows, got ", V, " and ", B);
   HT_CHECK(noise.device() == logits.device() && noise.scalar_type() == at::kFloat && noise.sizes() == logits.sizes(),
            "noise must be an fp32 tensor of the logits' shape and device");
-  HT_CHECK(token.device() == logits.device() && token.scalar_type() == at::kLong && token.is_contiguous() && token.numel() == B &&
-               logprob.device() == logits.device() && logprob.scalar_type() == at::kFloat && logprob.is_contiguous() && logprob.numel() == B,
-           "results must be contiguous int64 and fp32 [B]");
-  if (B == 0) return;
+  const auto in_range = [](double x, double most) { return x >= 0.0 && x <= most; };  // false for NaN
+  HT_CHECK(in_range(temperature, INFINITY) && top_k >= 0 && in_range(top_p, 1.0) && in_range(min_p, 1.0),
+           "temperature and top_k must be 0 or more, top_p and min_p between 0 and 1");
   const c10::cuda::CUDAGuard guard(logits.device());
+  at::Tensor token = at::empty({B}, logits.options().dtype(at::kLong).requires_grad(false));
+  at::Tensor logprob = at::empty({B}, logits.options().dtype(at::kFloat).requires_grad(false));
+  if (B == 0) return {token, logprob};
   if (V > 1 && logits.stride(1) != 1) logits = logits.contiguous();
   if (V > 1 && noise.stride(1) != 1) noise = noise.contiguous();
   const sampling::Args a{logits.data_ptr(),
@@ -199,13 +214,14 @@ void sample_tokens(at::Tensor logits, at::Tensor noise, c10::optional<at::Tensor
                          per_row<float>(temperature_rows, temperature, logits, at::kFloat, "temperature"),
                          per_row<float>(top_p_rows, top_p, logits, at::kFloat, "top_p"),
                          per_row<float>(min_p_rows, min_p, logits, at::kFloat, "min_p"),
-                         per_row<int>(top_k_rows, (double)std::min<int64_t>(std::max<int64_t>(top_k, 0), V), logits, at::kInt, "top_k"),
+                         per_row<int>(top_k_rows, (double)std::min<int64_t>(top_k, V), logits, at::kInt, "top_k"),
                          reinterpret_cast<long long*>(token.data_ptr<int64_t>()),
                          logprob.data_ptr<float>(),
                          (int)B,
                          (int)V,
                          logits.scalar_type() == at::kFloat};
   check_launch(sampling::launch(a, sms(), at::cuda::getCurrentCUDAStream()), "sample_tokens");
+  return {token, logprob};
 }
 
 }  // namespace ht

@@ -10,151 +10,187 @@
 // computes them.  The floor on the scale keeps fl(1/scale) finite for rows of zeros; a row with an
 // infinity or a NaN gets a NaN scale, so that it reads back as NaN instead of as a plausible value.
 //
-// Bound: memory.  Both kernels touch every byte once, 16 bytes of bf16 per lane and D / 8 lanes per
-// row.
+// Bound: memory; every byte is touched once.  A row takes D / 8 lanes with 16 bytes of bf16 each.  A thread
+// works on ROWS places at once, keys and values of each, and issues all their loads before it uses the
+// first.  Integers are converted with additions of a power of two and byte permutes: the conversion
+// instructions run at an eighth of their rate and would bind before the memory does.
 #include "generation.cuh"
 
 namespace ht {
 namespace kv {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, ROWS = 2;
 
+__device__ __forceinline__ long long slot_of(const void* slots, int wide, int t) {
+  return wide ? static_cast<const long long*>(slots)[t] : (long long)static_cast<const int*>(slots)[t];
+}
+
+// Row of the pool that holds head h of `slot`, or -1 for a slot outside it.
+__device__ __forceinline__ long long pool_row(const Pool& p, long long slot, int h) {
+  if (slot < 0 || slot >= p.pages << p.page_shift) return -1;
+  return (((slot >> p.page_shift) * p.Hkv + h) << p.page_shift) + (slot & ((1ll << p.page_shift) - 1));
+}
+
+// rn(x * inv) of 8 values as bytes.  |x * inv| is at most Q (1 + 2^-22), which rounds to Q: nothing has to be cut off.
 template <int F>
 __device__ __forceinline__ uint2 quantise8(const float* x, float inv) {
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint32_t b[4];
+    if constexpr (F == kInt8) {
+      // 1.5 * 2^23 + y has a last place of 1: the sum is rounded to the nearest integer, whose low byte is the value
+      uint32_t b[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float y = __fmul_rn(x[4 * h + j], inv);
-      if constexpr (F == kInt8) {
-        b[j] = (uint32_t)max(-127, min(127, __float2int_rn(y))) & 0xffu;
-      } else {
-        b[j] = __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
-      }
+      for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn(x[4 * h + j], inv), 12582912.f));
+      w[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    } else {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(x[4 * h], inv), __fmul_rn(x[4 * h + 1], inv)), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi =
+          __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(x[4 * h + 2], inv), __fmul_rn(x[4 * h + 3], inv)), __NV_SATFINITE, __NV_E4M3);
+      w[h] = lo | (hi << 16);
     }
-    w[h] = b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24);
   }
   return make_uint2(w[0], w[1]);
 }
 
+// The four values of a word.
 template <int F>
-__device__ __forceinline__ float value_of(uint32_t byte) {
-  if constexpr (F == kInt8) return (float)(int8_t)byte;
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
-}
-
-__device__ __forceinline__ long long slot_of(const void* slots, int wide, long long t) {
-  return wide ? static_cast<const long long*>(slots)[t] : (long long)static_cast<const int*>(slots)[t];
-}
-
-// Row index (in rows of D) of `slot` for head h in a [pages, Hkv, page_size, D] pool.
-__device__ __forceinline__ long long pool_row(long long slot, int h, int Hkv, int page_shift) {
-  const long long page = slot >> page_shift;
-  return ((page * Hkv + h) << page_shift) + (slot & ((1ll << page_shift) - 1));
+__device__ __forceinline__ float4 values_of(uint32_t w) {
+  if constexpr (F == kInt8) {
+    const uint32_t u = w ^ 0x80808080u;  // value + 128 as an unsigned byte; 2^23 + byte is a float with that byte at its end
+    const auto one = [&](uint32_t pick) { return __fadd_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, pick)), -8388736.f); };
+    return make_float4(one(0x7440), one(0x7441), one(0x7442), one(0x7443));
+  } else {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    const float2 x = __half22float2(__half2(a)), y = __half22float2(__half2(b));
+    return make_float4(x.x, x.y, y.x, y.y);
+  }
 }
 
 template <int F, int D>
-__global__ void __launch_bounds__(THREADS) write_kernel(WriteArgs a) {
-  constexpr int LANES = D / 8;
-  const long long rows = a.T * a.pool.Hkv;
-  const int lane = threadIdx.x % LANES;
-  const int which = blockIdx.y;  // 0: keys, 1: values
-  const __nv_bfloat16* const src = which ? a.src[1] : a.src[0];
-  const long long tok = which ? a.tok[1] : a.tok[0], head = which ? a.head[1] : a.head[0];
-  void* const pool = which ? a.pool.v : a.pool.k;
-  float* const scales = which ? a.pool.v_scale : a.pool.k_scale;
-  const long long step = (long long)gridDim.x * (THREADS / LANES);
-  const long long first = (long long)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
+__global__ void __launch_bounds__(THREADS) write_kernel(const WriteArgs a) {
+  constexpr int LANES = D / 8, PER_BLOCK = THREADS / LANES;
+  const int rows = (int)a.T * a.pool.Hkv, lane = threadIdx.x % LANES;
   // every lane of a warp makes the same number of turns, so the shuffles below always see a full warp
-  for (long long base = first; base - threadIdx.x / LANES < rows; base += step) {
-    const bool on = base < rows;
-    const long long t = on ? base / a.pool.Hkv : 0;
-    const int h = on ? (int)(base - t * a.pool.Hkv) : 0;
-    const long long slot = on ? slot_of(a.slots, a.wide, t) : -1;
-    const bool stored = slot >= 0 && slot < a.pool.pages << a.pool.page_shift;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (stored) raw = *reinterpret_cast<const uint4*>(src + t * tok + h * head + lane * 8);
-    const long long row = stored ? pool_row(slot, h, a.pool.Hkv, a.pool.page_shift) : 0;
-    if constexpr (F == kBf16) {
-      if (stored) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(pool) + row * D + lane * 8) = raw;
-    } else {
-      const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-      float x[8];
-      uint32_t top = 0;  // the largest magnitude as bits: NaN > infinity > every finite value
+  for (int base = blockIdx.x * PER_BLOCK * ROWS; base < rows; base += gridDim.x * PER_BLOCK * ROWS) {
+    uint4 raw[ROWS][2];
+    long long at[ROWS];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[2 * j] = __uint_as_float(u[j] << 16);
-        x[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-        top = max(top, max((u[j] << 16) & 0x7fffffffu, u[j] & 0x7fff0000u));
-      }
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = base + i * PER_BLOCK + threadIdx.x / LANES;
+      at[i] = -1;
+      raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
+      if (r >= rows) continue;
+      const int t = r / a.pool.Hkv, h = r - t * a.pool.Hkv;
+      raw[i][0] = __ldcs(reinterpret_cast<const uint4*>(a.src[0] + t * a.tok[0] + h * a.head[0] + lane * 8));
+      raw[i][1] = __ldcs(reinterpret_cast<const uint4*>(a.src[1] + t * a.tok[1] + h * a.head[1] + lane * 8));
+      at[i] = pool_row(a.pool, slot_of(a.slots, a.wide, t), h);
+    }
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const bool finite = top < 0x7f800000u;
-      const float scale = finite ? fmaxf(__fmul_rn(__uint_as_float(top), F == kInt8 ? 1.0f / 127.0f : 1.0f / 448.0f), kMinScale)
-                                 : __int_as_float(0x7fc00000);
-      const uint2 q = finite ? quantise8<F>(x, __frcp_rn(scale)) : make_uint2(0, 0);
-      if (stored) {
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + row * D + lane * 8) = q;
-        if (lane == 0) scales[row] = scale;
+    for (int i = 0; i < ROWS; ++i) {
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        void* const pool = which ? a.pool.v : a.pool.k;
+        if constexpr (F == kBf16) {
+          if (at[i] >= 0) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(pool) + at[i] * D + lane * 8) = raw[i][which];
+        } else {
+          const uint32_t u[4] = {raw[i][which].x, raw[i][which].y, raw[i][which].z, raw[i][which].w};
+          float x[8];
+          uint32_t top = 0;  // the largest magnitude as bits: NaN > infinity > every finite value
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[2 * j] = __uint_as_float(u[j] << 16);
+            x[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+            top = max(top, max((u[j] << 16) & 0x7fffffffu, u[j] & 0x7fff0000u));
+          }
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const bool finite = top < 0x7f800000u;
+          const float scale = finite ? fmaxf(__fmul_rn(__uint_as_float(top), F == kInt8 ? 1.0f / 127.0f : 1.0f / 448.0f), kMinScale)
+                                     : __int_as_float(0x7fc00000);
+          const uint2 q = finite ? quantise8<F>(x, __frcp_rn(scale)) : make_uint2(0, 0);
+          if (at[i] >= 0) {
+            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + at[i] * D + lane * 8) = q;
+            if (lane == 0) (which ? a.pool.v_scale : a.pool.k_scale)[at[i]] = scale;
+          }
+        }
       }
     }
   }
 }
 
 template <int F, int D>
-__global__ void __launch_bounds__(THREADS) read_kernel(ReadArgs a) {
-  constexpr int LANES = D / 8;
-  const long long rows = a.T * a.pool.Hkv;
-  const int lane = threadIdx.x % LANES;
-  const int which = blockIdx.y;  // 0: keys, 1: values
-  __nv_bfloat16* const dst = which ? a.dst[1] : a.dst[0];
-  const long long tok = which ? a.tok[1] : a.tok[0], head = which ? a.head[1] : a.head[0];
-  void* const pool = which ? a.pool.v : a.pool.k;
-  float* const scales = which ? a.pool.v_scale : a.pool.k_scale;
-  const long long step = (long long)gridDim.x * (THREADS / LANES);
-  for (long long r = (long long)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES; r < rows; r += step) {
-    const long long t = r / a.pool.Hkv;
-    const int h = (int)(r - t * a.pool.Hkv);
-    const long long slot = slot_of(a.slots, a.wide, t);
-    uint4 out = make_uint4(0, 0, 0, 0);
-    if (slot >= 0 && slot < a.pool.pages << a.pool.page_shift) {
-      const long long row = pool_row(slot, h, a.pool.Hkv, a.pool.page_shift);
-      if constexpr (F == kBf16) {
-        out = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(pool) + row * D + lane * 8);
-      } else {
-        const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pool) + row * D + lane * 8);
-        const float scale = scales[row];
-        uint32_t w[4];
+__global__ void __launch_bounds__(THREADS) read_kernel(const ReadArgs a) {
+  constexpr int LANES = D / 8, PER_BLOCK = THREADS / LANES;
+  const int rows = (int)a.T * a.pool.Hkv, lane = threadIdx.x % LANES;
+  for (int base = blockIdx.x * PER_BLOCK * ROWS; base < rows; base += gridDim.x * PER_BLOCK * ROWS) {
+    uint4 raw[ROWS][2];
+    float scale[ROWS][2];
+    int token[ROWS], head[ROWS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t two = (j < 2 ? q.x : q.y) >> (16 * (j & 1));
-          const __nv_bfloat162 p = __floats2bfloat162_rn(__fmul_rn(value_of<F>(two & 0xff), scale),
-                                                         __fmul_rn(value_of<F>((two >> 8) & 0xff), scale));
-          w[j] = *reinterpret_cast<const uint32_t*>(&p);
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = min(base + i * PER_BLOCK + (int)threadIdx.x / LANES, rows - 1);
+      token[i] = r / a.pool.Hkv;
+      head[i] = r - token[i] * a.pool.Hkv;
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const long long at = pool_row(a.pool, slot_of(a.slots, a.wide, token[i]), head[i]);
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        raw[i][which] = make_uint4(0, 0, 0, 0);
+        scale[i][which] = 0.f;
+        if (at < 0) continue;
+        const void* const pool = which ? a.pool.v : a.pool.k;
+        if constexpr (F == kBf16) {
+          raw[i][which] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(pool) + at * D + lane * 8);
+        } else {
+          const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pool) + at * D + lane * 8);
+          raw[i][which].x = q.x;
+          raw[i][which].y = q.y;
+          scale[i][which] = (which ? a.pool.v_scale : a.pool.k_scale)[at];
         }
-        out = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    *reinterpret_cast<uint4*>(dst + t * tok + h * head + lane * 8) = out;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      if (base + i * PER_BLOCK + (int)threadIdx.x / LANES >= rows) continue;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        uint4 out = raw[i][which];
+        if constexpr (F != kBf16) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float4 x = values_of<F>(j ? raw[i][which].y : raw[i][which].x);
+            const __nv_bfloat162 p = __floats2bfloat162_rn(__fmul_rn(x.x, scale[i][which]), __fmul_rn(x.y, scale[i][which]));
+            const __nv_bfloat162 q = __floats2bfloat162_rn(__fmul_rn(x.z, scale[i][which]), __fmul_rn(x.w, scale[i][which]));
+            w[2 * j] = *reinterpret_cast<const uint32_t*>(&p);
+            w[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&q);
+          }
+          out = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        __stcs(reinterpret_cast<uint4*>(a.dst[which] + token[i] * a.tok[which] + head[i] * a.head[which] + lane * 8), out);
+      }
+    }
   }
 }
 
-static dim3 row_grid(long long rows, int D, int sms) {
-  const long long per_block = THREADS / (D / 8), blocks = (rows + per_block - 1) / per_block;
-  return dim3((unsigned)(blocks < sms * 8ll ? blocks : sms * 8ll), 2);
+static unsigned row_blocks(long long rows, int D, int sms) {
+  const long long per_block = THREADS / (D / 8) * ROWS, blocks = (rows + per_block - 1) / per_block;
+  return (unsigned)(blocks < sms * 8ll ? blocks : sms * 8ll);
 }
 
 cudaError_t launch_write(const WriteArgs& a, int sms, cudaStream_t stream) {
-  const dim3 grid = row_grid(a.T * a.pool.Hkv, a.pool.D, sms);
-  by_format(a.pool, [&](auto f, auto d) { write_kernel<decltype(f)::value, decltype(d)::value><<<grid, THREADS, 0, stream>>>(a); });
+  const unsigned blocks = row_blocks(a.T * a.pool.Hkv, a.pool.D, sms);
+  by_format(a.pool, [&](auto f, auto d) { write_kernel<decltype(f)::value, decltype(d)::value><<<blocks, THREADS, 0, stream>>>(a); });
   return cudaGetLastError();
 }
 
 cudaError_t launch_read(const ReadArgs& a, int sms, cudaStream_t stream) {
-  const dim3 grid = row_grid(a.T * a.pool.Hkv, a.pool.D, sms);
-  by_format(a.pool, [&](auto f, auto d) { read_kernel<decltype(f)::value, decltype(d)::value><<<grid, THREADS, 0, stream>>>(a); });
+  const unsigned blocks = row_blocks(a.T * a.pool.Hkv, a.pool.D, sms);
+  by_format(a.pool, [&](auto f, auto d) { read_kernel<decltype(f)::value, decltype(d)::value><<<blocks, THREADS, 0, stream>>>(a); });
   return cudaGetLastError();
 }
 

@@ -185,18 +185,43 @@ def reference_paged_attention(q: torch.Tensor, pages: KVPages, block_table: torc
     return out.reshape(b, h, d).to(q.dtype if compute_dtype == torch.float32 else compute_dtype), lse.reshape(b, h)
 
 
+def _check_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor) -> None:
+    kvh = pages.num_kv_heads
+    if q.dim() != 3 or q.shape[2] != pages.head_dim or q.shape[1] % kvh or q.shape[1] == 0:
+        raise _refuse("paged_attention", "the queries do not fit the pool", f"[B, a multiple of {kvh}, {pages.head_dim}]", tuple(q.shape),
+                      "pass one token per sequence with the pool's head layout")
+    b = q.shape[0]
+    if block_table.dim() != 2 or block_table.shape[0] != b or lengths.shape != (b,):
+        raise _refuse("paged_attention", "every query needs a row of the block table and a length", f"[{b}, W] and [{b}]",
+                      f"{tuple(block_table.shape)} and {tuple(lengths.shape)}", "pass one row and one length per sequence")
+    if block_table.dtype != torch.int32 or lengths.dtype != torch.int32 or not (q.device == block_table.device == lengths.device == pages.k.device):
+        raise _refuse("paged_attention", "the block table and the lengths must be int32, and everything on one device", f"int32 on {pages.k.device}",
+                      f"{block_table.dtype} and {lengths.dtype} on {block_table.device} and {lengths.device}, q on {q.device}", "convert or move them")
+    if q.is_cuda and q.dtype != torch.bfloat16:
+        raise _refuse("paged_attention", "unsupported query type", "bfloat16", q.dtype, "cast q to bfloat16")
+    _no_gradient("paged_attention", q)
+
+
+# On CUDA the native entry points check every argument themselves, in the time that a check or two takes here.  Where
+# one of them refuses, the checks of this module say why in the framework's words.
+
+
 def kv_cache_write(pages: KVPages, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Store the rows ``k``, ``v`` ``[T, Hkv, D]`` (any strides) at ``slots`` ``[T]``, quantised as the pool holds them.
 
     The slots of one call are distinct.  A slot outside the pool stores nothing: ``-1`` marks a row of padding.
     A row with an infinity or a NaN in an 8-bit pool reads back as NaN.
     """
+    if pages.k.is_cuda:
+        try:
+            return extension().kv_cache_write(pages.k, pages.v, pages.k_scale, pages.v_scale, k, v, slots)
+        except RuntimeError:
+            _check_rows("kv_cache_write", pages, k, v, slots)
+            _no_gradient("kv_cache_write", k, v)
+            raise
     _check_rows("kv_cache_write", pages, k, v, slots)
     _no_gradient("kv_cache_write", k, v)
-    if not k.is_cuda:
-        reference_kv_cache_write(pages, k, v, slots)
-        return
-    extension().kv_cache_write(pages.k, pages.v, pages.k_scale, pages.v_scale, k, v, slots)
+    reference_kv_cache_write(pages, k, v, slots)
 
 
 def kv_cache_read(pages: KVPages, slots: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -205,18 +230,24 @@ def kv_cache_read(pages: KVPages, slots: torch.Tensor, out: tuple[torch.Tensor, 
     ``out`` takes a pair of tensors to write into, whose rows may be strided (the key and value columns of a
     packed QKV tensor, for one).
     """
-    if out is None:
-        if slots.dim() != 1:
-            raise _refuse("kv_cache_read", "slots must be a vector", "[T]", tuple(slots.shape), "flatten them")
-        shape = (slots.shape[0], pages.num_kv_heads, pages.head_dim)
-        out = (torch.empty(shape, dtype=torch.bfloat16, device=pages.k.device), torch.empty(shape, dtype=torch.bfloat16, device=pages.k.device))
-    _check_rows("kv_cache_read", pages, out[0], out[1], slots)
-    if not pages.k.is_cuda:
-        for o, x in zip(out, reference_kv_cache_read(pages, slots, out[0].dtype)):
-            o.copy_(x)
-        return out
-    extension().kv_cache_read(pages.k, pages.v, pages.k_scale, pages.v_scale, slots, out[0], out[1])
-    return out
+    k, v = (None, None) if out is None else out
+    if pages.k.is_cuda:
+        try:
+            return extension().kv_cache_read(pages.k, pages.v, pages.k_scale, pages.v_scale, slots, k, v)
+        except RuntimeError:
+            if slots.dim() != 1:
+                raise _refuse("kv_cache_read", "slots must be a vector", "[T]", tuple(slots.shape), "flatten them") from None
+            if k is not None and v is not None:
+                _check_rows("kv_cache_read", pages, k, v, slots)
+            raise
+    if slots.dim() != 1:
+        raise _refuse("kv_cache_read", "slots must be a vector", "[T]", tuple(slots.shape), "flatten them")
+    if k is None or v is None:
+        return reference_kv_cache_read(pages, slots)
+    _check_rows("kv_cache_read", pages, k, v, slots)
+    for o, x in zip((k, v), reference_kv_cache_read(pages, slots, k.dtype)):
+        o.copy_(x)
+    return k, v
 
 
 def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor, *, scale: float | None = None,
@@ -230,24 +261,13 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     gives zeros and ``-inf``; lengths beyond the table are cut to it, and tokens of pages outside the pool count as
     masked, as do whatever values lie behind a sequence's length.
     """
-    b, kvh = q.shape[0], pages.num_kv_heads
-    if q.dim() != 3 or q.shape[2] != pages.head_dim or q.shape[1] % kvh or q.shape[1] == 0:
-        raise _refuse("paged_attention", "the queries do not fit the pool", f"[B, a multiple of {kvh}, {pages.head_dim}]", tuple(q.shape),
-                      "pass one token per sequence with the pool's head layout")
-    if block_table.shape[0] != b or block_table.dim() != 2 or lengths.shape != (b,):
-        raise _refuse("paged_attention", "every query needs a row of the block table and a length", f"[{b}, W] and [{b}]",
-                      f"{tuple(block_table.shape)} and {tuple(lengths.shape)}", "pass one row and one length per sequence")
-    if block_table.dtype != torch.int32 or lengths.dtype != torch.int32 or not (q.device == block_table.device == lengths.device == pages.k.device):
-        raise _refuse("paged_attention", "the block table and the lengths must be int32, and everything on one device", f"int32 on {pages.k.device}",
-                      f"{block_table.dtype} and {lengths.dtype} on {block_table.device} and {lengths.device}, q on {q.device}", "convert or move them")
-    if q.is_cuda and q.dtype != torch.bfloat16:
-        raise _refuse("paged_attention", "unsupported query type", "bfloat16", q.dtype, "cast q to bfloat16")
-    _no_gradient("paged_attention", q)
-    if not q.is_cuda:
+    if q.is_cuda:
+        try:
+            out, lse = extension().paged_attention(q, pages.k, pages.v, pages.k_scale, pages.v_scale, block_table, lengths, scale, return_lse)
+        except RuntimeError:
+            _check_attention(q, pages, block_table, lengths)
+            raise
+    else:
+        _check_attention(q, pages, block_table, lengths)
         out, lse = reference_paged_attention(q, pages, block_table, lengths, scale=scale)
-        return (out, lse) if return_lse else out
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    extension().paged_attention(q, pages.k, pages.v, pages.k_scale, pages.v_scale, block_table, lengths, out, lse,
-                                q.shape[2] ** -0.5 if scale is None else scale)
     return (out, lse) if return_lse else out

@@ -19,21 +19,29 @@ from ._ext import extension
 __all__ = ["reference_sample_tokens", "sample_tokens"]
 
 Number = float | int | torch.Tensor
+_MOST_TOKENS = 1 << 18  # vocabulary of the kernel
 
 
 def _refuse(problem: str, expected: object, observed: object, resolution: str) -> ConfigurationError:
     return ConfigurationError(format_error("ops.sample_tokens", problem, expected=expected, observed=observed, resolution=resolution))
 
 
-def _checked(name: str, value: Number, logits: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor | None, float | int]:
-    if isinstance(value, torch.Tensor):
-        if value.shape != logits.shape[:1] or value.dtype != dtype or value.device != logits.device:
-            raise _refuse(f"{name} does not fit the logits", f"a number or a {dtype} tensor [{logits.shape[0]}] on {logits.device}",
-                          f"{value.dtype} {tuple(value.shape)} on {value.device}", "pass one value per row, or one number")
-        return value.contiguous(), 0
-    if math.isnan(value) or value < 0 or (name == "top_p" and value > 1) or (name == "min_p" and value > 1):
-        raise _refuse(f"{name} is out of range", "0 to 1" if name in ("top_p", "min_p") else "0 or more", value, "choose a value in range")
-    return None, value
+def _check(logits: torch.Tensor, noise: torch.Tensor, filters: dict[str, Number]) -> None:
+    if logits.dim() != 2 or logits.shape[1] == 0 or noise.shape != logits.shape or noise.dtype != torch.float32 or noise.device != logits.device:
+        raise _refuse("logits and noise must be alike", "[B, V] logits and fp32 noise of the same shape and device",
+                      f"{tuple(logits.shape)} and {noise.dtype} {tuple(noise.shape)} on {noise.device}", "draw one Exp(1) number per logit")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise _refuse("unsupported logit type", "bfloat16 or float32", logits.dtype, "cast the logits")
+    if logits.is_cuda and logits.shape[1] > _MOST_TOKENS:
+        raise _refuse("the vocabulary is too large", f"at most {_MOST_TOKENS} tokens", logits.shape[1], "sample from slices of it")
+    for name, value in filters.items():
+        if isinstance(value, torch.Tensor):
+            dtype = torch.int32 if name == "top_k" else torch.float32
+            if value.shape != logits.shape[:1] or value.dtype != dtype or value.device != logits.device or not value.is_contiguous():
+                raise _refuse(f"{name} does not fit the logits", f"a number or a contiguous {dtype} tensor [{logits.shape[0]}] on {logits.device}",
+                              f"{value.dtype} {tuple(value.shape)} on {value.device}", "pass one value per row, or one number")
+        elif not value >= 0 or (name in ("top_p", "min_p") and value > 1):
+            raise _refuse(f"{name} is out of range", "0 to 1" if name in ("top_p", "min_p") else "0 or more", value, "choose a value in range")
 
 
 def reference_sample_tokens(logits: torch.Tensor, noise: torch.Tensor, temperature: Number = 1.0, top_k: Number = 0, top_p: Number = 1.0,
@@ -76,19 +84,16 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, *, temperature: Num
     row at this temperature (at 1 where the temperature is 0), before any filter.  Logits of ``-inf`` or NaN cannot
     be drawn; a row without any other gives ``-1`` and ``-inf``.
     """
-    if logits.dim() != 2 or logits.shape[1] == 0 or noise.shape != logits.shape or noise.dtype != torch.float32 or noise.device != logits.device:
-        raise _refuse("logits and noise must be alike", "[B, V] logits and fp32 noise of the same shape and device",
-                      f"{tuple(logits.shape)} and {noise.dtype} {tuple(noise.shape)} on {noise.device}", "draw one Exp(1) number per logit")
-    if logits.dtype not in (torch.bfloat16, torch.float32):
-        raise _refuse("unsupported logit type", "bfloat16 or float32", logits.dtype, "cast the logits")
-    t_rows, t = _checked("temperature", temperature, logits, torch.float32)
-    k_rows, k = _checked("top_k", top_k, logits, torch.int32)
-    p_rows, p = _checked("top_p", top_p, logits, torch.float32)
-    m_rows, m = _checked("min_p", min_p, logits, torch.float32)
-    logits = logits.detach()
-    if not logits.is_cuda:
-        return reference_sample_tokens(logits, noise, temperature, top_k, top_p, min_p)
-    token = torch.empty(logits.shape[0], dtype=torch.int64, device=logits.device)
-    logprob = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-    extension().sample_tokens(logits, noise, t_rows, t, k_rows, k, p_rows, p, m_rows, m, token, logprob)
-    return token, logprob
+    if logits.is_cuda:
+        try:
+            # a filter is a tensor with a value per row, or a number
+            t = (temperature, 1.0) if isinstance(temperature, torch.Tensor) else (None, temperature)
+            k = (top_k, 0) if isinstance(top_k, torch.Tensor) else (None, top_k)
+            p = (top_p, 1.0) if isinstance(top_p, torch.Tensor) else (None, top_p)
+            m = (min_p, 0.0) if isinstance(min_p, torch.Tensor) else (None, min_p)
+            return extension().sample_tokens(logits, noise, *t, *k, *p, *m)
+        except RuntimeError:
+            _check(logits, noise, {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p})
+            raise
+    _check(logits, noise, {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p})
+    return reference_sample_tokens(logits.detach(), noise, temperature, top_k, top_p, min_p)
