@@ -10,16 +10,17 @@
 // computes them.  The floor on the scale keeps fl(1/scale) finite for rows of zeros; a row with an
 // infinity or a NaN gets a NaN scale, so that it reads back as NaN instead of as a plausible value.
 //
-// Bound: memory; every byte is touched once.  A row takes D / 8 lanes with 16 bytes of bf16 each.  A thread
-// works on ROWS places at once, keys and values of each, and issues all their loads before it uses the
-// first.  Integers are converted with additions of a power of two and byte permutes: the conversion
+// Bound: memory; every byte is touched once.  A row takes D / 8 lanes with 16 bytes of bf16 each; a thread has
+// its place of the keys and of the values in flight together.  (Two or four rows a thread measured the same on
+// 16384 tokens of 8 x 128 -- 40 and 41 us for writing and reading back against 37 -- and up to twice the time on 32
+// tokens, where there are then fewer warps than schedulers.)  Integers are converted with additions of a power of two and byte permutes: the conversion
 // instructions run at an eighth of their rate and would bind before the memory does.
 #include "generation.cuh"
 
 namespace ht {
 namespace kv {
 
-constexpr int THREADS = 256, ROWS = 2;
+constexpr int THREADS = 256;
 
 __device__ __forceinline__ long long slot_of(const void* slots, int wide, int t) {
   return wide ? static_cast<const long long*>(slots)[t] : (long long)static_cast<const int*>(slots)[t];
@@ -73,47 +74,40 @@ __global__ void __launch_bounds__(THREADS) write_kernel(const WriteArgs a) {
   constexpr int LANES = D / 8, PER_BLOCK = THREADS / LANES;
   const int rows = (int)a.T * a.pool.Hkv, lane = threadIdx.x % LANES;
   // every lane of a warp makes the same number of turns, so the shuffles below always see a full warp
-  for (int base = blockIdx.x * PER_BLOCK * ROWS; base < rows; base += gridDim.x * PER_BLOCK * ROWS) {
-    uint4 raw[ROWS][2];
-    long long at[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const int r = base + i * PER_BLOCK + threadIdx.x / LANES;
-      at[i] = -1;
-      raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
-      if (r >= rows) continue;
+  for (int base = blockIdx.x * PER_BLOCK; base < rows; base += gridDim.x * PER_BLOCK) {
+    const int r = base + threadIdx.x / LANES;
+    uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    long long at = -1;
+    if (r < rows) {
       const int t = r / a.pool.Hkv, h = r - t * a.pool.Hkv;
-      raw[i][0] = __ldcs(reinterpret_cast<const uint4*>(a.src[0] + t * a.tok[0] + h * a.head[0] + lane * 8));
-      raw[i][1] = __ldcs(reinterpret_cast<const uint4*>(a.src[1] + t * a.tok[1] + h * a.head[1] + lane * 8));
-      at[i] = pool_row(a.pool, slot_of(a.slots, a.wide, t), h);
+      raw[0] = __ldcs(reinterpret_cast<const uint4*>(a.src[0] + t * a.tok[0] + h * a.head[0] + lane * 8));
+      raw[1] = __ldcs(reinterpret_cast<const uint4*>(a.src[1] + t * a.tok[1] + h * a.head[1] + lane * 8));
+      at = pool_row(a.pool, slot_of(a.slots, a.wide, t), h);
     }
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
+    for (int which = 0; which < 2; ++which) {
+      void* const pool = which ? a.pool.v : a.pool.k;
+      if constexpr (F == kBf16) {
+        if (at >= 0) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(pool) + at * D + lane * 8) = raw[which];
+      } else {
+        const uint32_t u[4] = {raw[which].x, raw[which].y, raw[which].z, raw[which].w};
+        float x[8];
+        uint32_t top = 0;  // the largest magnitude as bits: NaN > infinity > every finite value
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        void* const pool = which ? a.pool.v : a.pool.k;
-        if constexpr (F == kBf16) {
-          if (at[i] >= 0) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(pool) + at[i] * D + lane * 8) = raw[i][which];
-        } else {
-          const uint32_t u[4] = {raw[i][which].x, raw[i][which].y, raw[i][which].z, raw[i][which].w};
-          float x[8];
-          uint32_t top = 0;  // the largest magnitude as bits: NaN > infinity > every finite value
+        for (int j = 0; j < 4; ++j) {
+          x[2 * j] = __uint_as_float(u[j] << 16);
+          x[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+          top = max(top, max((u[j] << 16) & 0x7fffffffu, u[j] & 0x7fff0000u));
+        }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[2 * j] = __uint_as_float(u[j] << 16);
-            x[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-            top = max(top, max((u[j] << 16) & 0x7fffffffu, u[j] & 0x7fff0000u));
-          }
-#pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const bool finite = top < 0x7f800000u;
-          const float scale = finite ? fmaxf(__fmul_rn(__uint_as_float(top), F == kInt8 ? 1.0f / 127.0f : 1.0f / 448.0f), kMinScale)
-                                     : __int_as_float(0x7fc00000);
-          const uint2 q = finite ? quantise8<F>(x, __frcp_rn(scale)) : make_uint2(0, 0);
-          if (at[i] >= 0) {
-            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + at[i] * D + lane * 8) = q;
-            if (lane == 0) (which ? a.pool.v_scale : a.pool.k_scale)[at[i]] = scale;
-          }
+        for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const bool finite = top < 0x7f800000u;
+        const float scale = finite ? fmaxf(__fmul_rn(__uint_as_float(top), F == kInt8 ? 1.0f / 127.0f : 1.0f / 448.0f), kMinScale)
+                                   : __int_as_float(0x7fc00000);
+        const uint2 q = finite ? quantise8<F>(x, __frcp_rn(scale)) : make_uint2(0, 0);
+        if (at >= 0) {
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + at * D + lane * 8) = q;
+          if (lane == 0) (which ? a.pool.v_scale : a.pool.k_scale)[at] = scale;
         }
       }
     }
@@ -124,62 +118,48 @@ template <int F, int D>
 __global__ void __launch_bounds__(THREADS) read_kernel(const ReadArgs a) {
   constexpr int LANES = D / 8, PER_BLOCK = THREADS / LANES;
   const int rows = (int)a.T * a.pool.Hkv, lane = threadIdx.x % LANES;
-  for (int base = blockIdx.x * PER_BLOCK * ROWS; base < rows; base += gridDim.x * PER_BLOCK * ROWS) {
-    uint4 raw[ROWS][2];
-    float scale[ROWS][2];
-    int token[ROWS], head[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const int r = min(base + i * PER_BLOCK + (int)threadIdx.x / LANES, rows - 1);
-      token[i] = r / a.pool.Hkv;
-      head[i] = r - token[i] * a.pool.Hkv;
-    }
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const long long at = pool_row(a.pool, slot_of(a.slots, a.wide, token[i]), head[i]);
+  for (int r = blockIdx.x * PER_BLOCK + threadIdx.x / LANES; r < rows; r += gridDim.x * PER_BLOCK) {
+    const int t = r / a.pool.Hkv, h = r - t * a.pool.Hkv;
+    const long long at = pool_row(a.pool, slot_of(a.slots, a.wide, t), h);
+    uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    float scale[2] = {0.f, 0.f};
+    if (at >= 0) {
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
-        raw[i][which] = make_uint4(0, 0, 0, 0);
-        scale[i][which] = 0.f;
-        if (at < 0) continue;
         const void* const pool = which ? a.pool.v : a.pool.k;
         if constexpr (F == kBf16) {
-          raw[i][which] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(pool) + at * D + lane * 8);
+          raw[which] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(pool) + at * D + lane * 8);
         } else {
           const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pool) + at * D + lane * 8);
-          raw[i][which].x = q.x;
-          raw[i][which].y = q.y;
-          scale[i][which] = (which ? a.pool.v_scale : a.pool.k_scale)[at];
+          raw[which].x = q.x;
+          raw[which].y = q.y;
+          scale[which] = (which ? a.pool.v_scale : a.pool.k_scale)[at];
         }
       }
     }
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      if (base + i * PER_BLOCK + (int)threadIdx.x / LANES >= rows) continue;
+    for (int which = 0; which < 2; ++which) {
+      uint4 out = raw[which];
+      if constexpr (F != kBf16) {
+        uint32_t w[4];
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        uint4 out = raw[i][which];
-        if constexpr (F != kBf16) {
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float4 x = values_of<F>(j ? raw[i][which].y : raw[i][which].x);
-            const __nv_bfloat162 p = __floats2bfloat162_rn(__fmul_rn(x.x, scale[i][which]), __fmul_rn(x.y, scale[i][which]));
-            const __nv_bfloat162 q = __floats2bfloat162_rn(__fmul_rn(x.z, scale[i][which]), __fmul_rn(x.w, scale[i][which]));
-            w[2 * j] = *reinterpret_cast<const uint32_t*>(&p);
-            w[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&q);
-          }
-          out = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int j = 0; j < 2; ++j) {
+          const float4 x = values_of<F>(j ? raw[which].y : raw[which].x);
+          const __nv_bfloat162 p = __floats2bfloat162_rn(__fmul_rn(x.x, scale[which]), __fmul_rn(x.y, scale[which]));
+          const __nv_bfloat162 q = __floats2bfloat162_rn(__fmul_rn(x.z, scale[which]), __fmul_rn(x.w, scale[which]));
+          w[2 * j] = *reinterpret_cast<const uint32_t*>(&p);
+          w[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&q);
         }
-        __stcs(reinterpret_cast<uint4*>(a.dst[which] + token[i] * a.tok[which] + head[i] * a.head[which] + lane * 8), out);
+        out = make_uint4(w[0], w[1], w[2], w[3]);
       }
+      __stcs(reinterpret_cast<uint4*>(a.dst[which] + t * a.tok[which] + h * a.head[which] + lane * 8), out);
     }
   }
 }
 
 static unsigned row_blocks(long long rows, int D, int sms) {
-  const long long per_block = THREADS / (D / 8) * ROWS, blocks = (rows + per_block - 1) / per_block;
-  return (unsigned)(blocks < sms * 8ll ? blocks : sms * 8ll);
+  const long long per_block = THREADS / (D / 8), blocks = (rows + per_block - 1) / per_block;
+  return (unsigned)(blocks < sms * 16ll ? blocks : sms * 16ll);
 }
 
 cudaError_t launch_write(const WriteArgs& a, int sms, cudaStream_t stream) {

@@ -58,8 +58,14 @@ struct Shape {
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 // 16 bytes, or zeros without reading `src`.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0), "l"(policy) : "memory");
+}
+// Keys and values are read once per call: they should leave the L2 before what is needed again (code, tables, pieces).
+__device__ __forceinline__ uint64_t stream_policy() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -171,8 +177,16 @@ __device__ __forceinline__ void advance(const Args& a, Cursor& c, int rows) {
   } while (c.tiles == 0);
 }
 
+// Counts one more and returns the count before.  Releases what the block wrote before its last barrier, and acquires what the
+// blocks that arrived earlier had written.
+__device__ __forceinline__ unsigned arrive(unsigned* counter) {
+  unsigned before;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before;
+}
+
 template <int F, int D>
-__global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const Args a) {
+__global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const __grid_constant__ Args a) {
   using S = Shape<F, D>;
   constexpr int TOK = S::TOK, GROUPS = TOK / 16, NT = D / 8, WARPS = S::WARPS;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -191,8 +205,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
     int count;
     uint32_t have;
     float weight[2 * WARPS][HEADS];
-    int scan[WARPS];
-    Cursor start[WARPS];
+    bool shared_rows;  // whether a row of this block goes on in another one
     int join_first[2], join_count[2], join_b[2], join_row[2];
   };
   static_assert(sizeof(Shared) <= WARPS * S::BOOK, "shared bookkeeping");
@@ -206,80 +219,74 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
   const int chunks = (group + HEADS - 1) / HEADS;  // rows per key/value head
   const int rows = a.pool.Hkv * chunks;
 
-  // ---- this block's and its warps' ranges of the line, from one scan of the lengths (in chunks of a block's threads)
-  int per_block = 0, block_from = 0, block_to = 0, per_warp = 0;
-  if (tid < 2 * WARPS) sh.meta[tid].count = 0;
-  const auto scan_chunk = [&](int tiles, int& total) {  // inclusive
-    int upto = tiles;
+  // ---- this warp's range of the line.  Every warp works it out for itself: sums of the tiles of 32 sequences at a time, a
+  // lane for each sum, then the 32 sequences among which the range starts.  Nobody waits for another warp.
+  const auto tiles_of = [&](int n) { return (n + TOK - 1) / TOK * rows; };
+  const auto scan = [&](int v) {  // inclusive, over the lanes
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int other = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += other;
+      const int other = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += other;
     }
-    __syncthreads();
-    if (lane == 31) sh.scan[warp] = upto;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const int of_warp = sh.scan[w];
-      if (w < warp) upto += of_warp;
-      total += of_warp;
-    }
-    return upto;
+    return v;
   };
-  {
-    const int my_n = tid < a.B ? tokens_of(a, tid) : 0;
-    const int my_tiles = (my_n + TOK - 1) / TOK * rows;
-    int total = 0;
-    const int my_upto = scan_chunk(my_tiles, total);
-    int line = total;
-    for (int b0 = S::THREADS; b0 < a.B; b0 += S::THREADS) {
-      int more = 0;
-      scan_chunk(b0 + tid < a.B ? (tokens_of(a, b0 + tid) + TOK - 1) / TOK * rows : 0, more);
-      line += more;
-    }
-    // at least one tile for each warp of a block: fewer, fuller blocks have fewer pieces to join
-    per_block = max((int)((line + gridDim.x - 1) / gridDim.x), WARPS);
-    block_from = min((long long)line, (long long)per_block * blockIdx.x);
-    block_to = min(line - block_from, per_block) + block_from;
-    per_warp = (block_to - block_from + WARPS - 1) / WARPS;
-    int base = 0;  // tiles of the sequences before this chunk of them
-    for (int b0 = 0; b0 < a.B; b0 += S::THREADS) {
-      const int b = b0 + tid;
-      int n = my_n, upto = my_upto;
-      if (b0 > 0) {
-        n = b < a.B ? tokens_of(a, b) : 0;
-        upto = scan_chunk((n + TOK - 1) / TOK * rows, total);
-      }
-      if (n == 0 && b < a.B && b % gridDim.x == blockIdx.x) {  // no tokens, hence no tiles: this thread writes the result
+  const auto sums = [&](int b0, bool first) {  // of the 1024 sequences from b0 on
+    int mine = 0;
+#pragma unroll 4
+    for (int k = 0; k < 32; ++k) {
+      const int b = b0 + 32 * k + lane;
+      if (b0 + 32 * k >= a.B) break;
+      const int n = b < a.B ? tokens_of(a, b) : 0;
+      if (first && warp == 0 && n == 0 && b < a.B && b % gridDim.x == blockIdx.x) {  // no tokens, hence no tiles: write the result here
         for (int i = 0; i < a.H * D; i += 8) *reinterpret_cast<uint4*>(a.out + (long long)b * a.H * D + i) = make_uint4(0, 0, 0, 0);
         if (a.lse != nullptr)
           for (int i = 0; i < a.H; ++i) a.lse[(long long)b * a.H + i] = -INFINITY;
       }
-      const int per_row = (n + TOK - 1) / TOK, from = base + upto - per_row * rows, to = base + upto;
-      if (from < block_to && to > block_from) {
-        // the warps that start inside this sequence
-        const int w0 = from <= block_from ? 0 : (from - block_from + per_warp - 1) / per_warp;
-        for (int w = w0; w < WARPS && block_from + w * per_warp < min(to, block_to); ++w) sh.start[w] = Cursor{b, 0, from, per_row, n};
-      }
-      base += total;
+      const int sum = (int)__reduce_add_sync(0xffffffffu, (uint32_t)tiles_of(n));
+      if (lane == k) mine = sum;
     }
-  }
+    return mine;
+  };
+  int mine = sums(0, true), upto = scan(mine);
+  int line = __shfl_sync(0xffffffffu, upto, 31);
+  for (int b0 = 1024; b0 < a.B; b0 += 1024) line += (int)__reduce_add_sync(0xffffffffu, (uint32_t)sums(b0, true));
+  // at least one tile for each warp of a block: fewer, fuller blocks have fewer pieces to join
+  const int per_block = max((int)((line + gridDim.x - 1) / gridDim.x), WARPS);
+  const int block_from = (int)min((long long)line, (long long)per_block * blockIdx.x);
+  const int block_to = min(line - block_from, per_block) + block_from;
   if (block_from >= block_to) return;
-  __syncthreads();
-
+  const int per_warp = (block_to - block_from + WARPS - 1) / WARPS;
   const int from = block_from + warp * per_warp;
   const int count = max(0, min(per_warp, block_to - from));
+  if (lane < 2) sh.meta[2 * warp + lane].count = 0;
+  Cursor start{0, 0, 0, 1, 0};
+  if (count > 0) {
+    int base = 0, b0 = 0;
+    while (from >= base + __shfl_sync(0xffffffffu, upto, 31)) {  // beyond these 1024 sequences
+      base += __shfl_sync(0xffffffffu, upto, 31);
+      b0 += 1024;
+      mine = sums(b0, false);
+      upto = scan(mine);
+    }
+    const int chunk = __popc(__ballot_sync(0xffffffffu, base + upto <= from));
+    base += __shfl_sync(0xffffffffu, upto - mine, chunk);
+    b0 += 32 * chunk;
+    const int n = b0 + lane < a.B ? tokens_of(a, b0 + lane) : 0;
+    const int reach = scan(tiles_of(n)), at = __popc(__ballot_sync(0xffffffffu, base + reach <= from));
+    start.b = b0 + at;
+    start.n = __shfl_sync(0xffffffffu, n, at);
+    start.tiles = (start.n + TOK - 1) / TOK;
+    const int in = from - (base + __shfl_sync(0xffffffffu, reach - tiles_of(n), at));
+    start.row = in / start.tiles;
+    start.tile = in - start.row * start.tiles;
+  }
   unsigned char* const ring = rings + warp * S::STAGES * S::STAGE;
   const uint32_t ring_addr = smem_addr(ring);
   [[maybe_unused]] float4* const factors = reinterpret_cast<float4*>(pieces + WARPS * S::PIECE + warp * S::FACTORS);
 
   if (count > 0) {
-    Cursor load = sh.start[warp];
-    load.tile = from - load.tile;  // was: the sequence's first tile on the line
-    load.row = load.tile / load.tiles;
-    load.tile -= load.row * load.tiles;
+    const uint64_t policy = stream_policy();
+    Cursor load = start;
     Cursor use = load;
     int to_load = count;
     uint32_t held = 0;  // per stage: which groups of 16 tokens are in the pool
@@ -322,12 +329,12 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
             const int q = j * 32 + lane, r = q / PER, ch = q % PER;
             const int kch = PER >= 8 ? ch ^ ((r & 1) << 2) : ch;
             const int vch = F == kv::kBf16 ? ch ^ (r & 7) : PER >= 8 ? ch ^ (((r >> 1) & 3) << 1) : ch;
-            copy16(base + (i * 16 + r) * S::ROW + kch * 16, ks + q * 16, r < real);
-            copy16(base + S::DATA + (i * 16 + r) * S::ROW + vch * 16, vs + q * 16, r < real);
+            copy16(base + (i * 16 + r) * S::ROW + kch * 16, ks + q * 16, r < real, policy);
+            copy16(base + S::DATA + (i * 16 + r) * S::ROW + vch * 16, vs + q * 16, r < real, policy);
           }
           if (F != kv::kBf16 && lane < 8) {
             const float* scales = (lane < 4 ? a.pool.k_scale : a.pool.v_scale) + first;
-            copy16(base + 2 * S::DATA + (lane < 4 ? 0 : S::SCALES) + i * 64 + (lane & 3) * 16, scales + (lane & 3) * 4, in_pool);
+            copy16(base + 2 * S::DATA + (lane < 4 ? 0 : S::SCALES) + i * 64 + (lane & 3) * 16, scales + (lane & 3) * 4, in_pool, policy);
           }
         }
         held = (held & ~(0xfu << (4 * stage))) | (bits << (4 * stage));
@@ -632,6 +639,10 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
       sh.have = have;
       sh.join_count[0] = sh.join_count[1] = 0;
     }
+    const bool whole = !head || sh.groups[__popc(heads & ((1u << lane) - 1))].whole;
+    if (lane == 0) sh.shared_rows = false;
+    __syncwarp();
+    if (!whole) sh.shared_rows = true;
   }
   __syncthreads();
   const int real_heads = min(group, HEADS);
@@ -712,7 +723,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
 
   // ---- rows that cross blocks: the last block to arrive joins them.  A row that goes on behind its first block is that
   // block's last one, so the block's number names the counter.
-  __threadfence();
+  if (!sh.shared_rows) return;
   __syncthreads();
   if (tid == 0) {
     int joins = 0;
@@ -720,7 +731,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
       const Group& grp = sh.groups[gi];
       if (grp.whole) continue;
       const int b0 = grp.first.item / per_block, b1 = (grp.first.item + grp.first.tiles - 1) / per_block;
-      if (atomicAdd(a.arrived + b0, 1u) == (unsigned)(b1 - b0)) {
+      if (arrive(a.arrived + b0) == (unsigned)(b1 - b0)) {
         a.arrived[b0] = 0;
         sh.join_first[joins] = b0;
         sh.join_count[joins] = b1 - b0 + 1;
@@ -733,23 +744,32 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
   for (int join = 0; join < 2; ++join) {
     const int n = sh.join_count[join];
     if (n == 0) break;
-    __threadfence();
     // the first block's piece is its second, the others' their first
     const auto part = [&](int j) { return a.partial + ((long long)(sh.join_first[join] + j) * 2 + (j == 0 ? 1 : 0)) * STEP; };
     float* const weights = reinterpret_cast<float*>(rings);  // [n][HEADS], then the heads' norms, then the copies' sums
     float* const norms = weights + n * HEADS;
     float* const sums = norms + HEADS;
+    // a thread takes 4 neighbouring places (of one head); the threads left over take further parts of the list
+    const int quads = 2 * NT * real_heads, copies = S::THREADS / quads;
+    const int quad = tid % quads, copy = tid / quads;
+    const int place = quad / real_heads * 32 + quad % real_heads * 4;
+    float4 ahead = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (copy < copies && copy < n) ahead = __ldcg(reinterpret_cast<const float4*>(part(copy) + place));
     if (warp < real_heads) {  // one warp per head
       float top = -INFINITY, total = 0.f;
-      for (int j = lane; j < n; j += 32) top = fmaxf(top, __ldcg(part(j) + HEADS * D + warp));
+      for (int j = lane; j < n; j += 32) {
+        const float m = __ldcg(part(j) + HEADS * D + warp), l = __ldcg(part(j) + HEADS * D + HEADS + warp);
+        const float higher = fmaxf(top, m), at = higher == -INFINITY ? 0.f : higher;
+        weights[j * HEADS + warp] = m;
+        total = total * fast_exp2(top - at) + l * fast_exp2(m - at);
+        top = higher;
+      }
+      const float mine = top;
       for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
       const float at = top == -INFINITY ? 0.f : top;
-      for (int j = lane; j < n; j += 32) {
-        const float w = fast_exp2(__ldcg(part(j) + HEADS * D + warp) - at);
-        weights[j * HEADS + warp] = w;
-        total += w * __ldcg(part(j) + HEADS * D + HEADS + warp);
-      }
+      total *= fast_exp2(mine - at);
       for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+      for (int j = lane; j < n; j += 32) weights[j * HEADS + warp] = fast_exp2(weights[j * HEADS + warp] - at);
       if (lane == 0) {
         norms[warp] = total == 0.f ? 0.f : __fdividef(1.f, total);
         long long head;
@@ -758,16 +778,12 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const A
       }
     }
     __syncthreads();
-    // a thread takes 4 neighbouring places (of one head); the threads left over take further parts of the list
-    const int quads = 2 * NT * real_heads, copies = S::THREADS / quads;
-    const int quad = tid % quads, copy = tid / quads;
-    const int place = quad / real_heads * 32 + quad % real_heads * 4;
     if (copy < copies) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
       for (int j = copy; j < n; j += copies) {
         const float w = weights[j * HEADS + quad % real_heads];
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(part(j) + place));
+        const float4 v = j == copy ? ahead : __ldcg(reinterpret_cast<const float4*>(part(j) + place));
         acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
       }
       reinterpret_cast<float4*>(sums)[copy * quads + quad] = acc;

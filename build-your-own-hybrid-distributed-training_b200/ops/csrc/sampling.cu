@@ -169,7 +169,7 @@ __device__ __forceinline__ int first_bin(const Weights& weight, float l) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constant__ Args a) {
   constexpr int E = Piece<T>::E;
   extern __shared__ __align__(16) unsigned char smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
@@ -478,7 +478,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
       counts[j] = 0;
       const int bin = me * slice + tid * own + j;
       if (j < own && tid * own + j < slice) {
-        for (int r = 0; r < n; ++r) {
+#pragma unroll 2
+        for (int r = 0; r < n; ++r) {  // several blocks' loads under way together
           const uint32_t c = WIDE ? *peer(&sh.count[bin], r) : sh.count[bin];
           counts[j] += c;
           if (masses) mine[j] += WIDE ? *peer(&sh.low[bin], r) + ((unsigned long long)*peer(&sh.high[bin], r) << 16)
