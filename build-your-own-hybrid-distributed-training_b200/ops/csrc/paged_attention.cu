@@ -15,16 +15,20 @@
 //   one persistent block per SM, no idle SM for ragged batches, long rows split without a plan on the
 //   host.  Every warp streams its range through a ring of its own in shared memory with 16-byte
 //   cp.async; warps never wait for one another before their range is done.
-// * Matrix instructions.  S = Q K^T and O += P V are m16n8k16 with the 8 heads as rows 0-7: at these
-//   intensities the tensor pipe is far from its limit, and a tile of 16 rows is the smallest there is.
-//   Rows 8-15 are not wasted: in the second product they carry what rounding P to 16 bits left over, so
-//   P enters with 16 (bf16) or 22 (fp16) significant bits at no extra instruction.  The dimensions of q and
-//   k are summed in the order in which 16-byte loads deliver them (the order of a dot product is free),
-//   so 8-bit keys go from shared memory to the instruction's fragments with byte permutes alone.
-// * 8 bits.  int8 and e4m3 values are exact in fp16, and q is scaled by a power of two per head so that
-//   its bf16 values are exact there too (down to 2^-24 of the head's largest).  A token's key scale
-//   multiplies its score.  Its value scale sv joins the exponent: with s'_t = s_t + log2(sv_t), the running
-//   maximum m of s' and p_t = 2^(s'_t - m) <= 1, the output is sum p_t v_t / sum (p_t / sv_t): p fits fp16
+// * Matrix instructions.  S = Q K^T and O += P V have the 8 heads as rows 0-7 of a tile of 16 rows, the smallest
+//   there is: at these intensities the tensor pipe is far from its limit.  Rows 8-15 are not wasted; they carry
+//   what rounding left over of the same heads' operand.  In bf16 (m16n8k16) P enters as two bf16 terms.  The
+//   dimensions of q and k are summed in the order in which 16-byte loads deliver them, and the tokens of a tile in
+//   the order in which score accumulators and the second product's operand agree: no data is moved for either.
+// * 8 bits (m16n8k32).  Keys and values enter the instructions as they are held, so the other operand has to be in
+//   8 bits too, as digits.  int8: q of a head, scaled by a power of two and rounded to 22 bits, is three signed
+//   digits, p is rint(65535 p) in two unsigned ones, and the sums are exact integers (below 2^22, read as floats by
+//   starting the accumulators at the bits of 1.5 2^23).  e4m3: q is two terms of 4 bits each, which hold all 8 bits
+//   of a bf16, and p three.  p is taken relative to the tile's own maximum, so that its digits always start
+//   at the tile's largest weight, and the tile's product is added to the output in fp32.  (With values converted to
+//   fp16 instead, the conversions alone were half of the instructions: 64 against NN us on 32 rows of 4096 int8.)
+//   A token's key scale multiplies its score.  Its value scale sv joins the exponent: with s'_t = s_t + log2(sv_t) and
+//   m the maximum of s', p_t = 2^(s'_t - m) <= 1, the output is sum p_t v_t / sum (p_t / sv_t): p stays in range
 //   whatever the scales are.
 // * Joining.  A row inside one warp's range is finished by that warp.  Otherwise warps leave (o, m, sum)
 //   in shared memory, the block merges neighbours, and rows that cross blocks go through a workspace:
@@ -90,51 +94,58 @@ __device__ __forceinline__ void ldmatrix4t(uint32_t* r, uint32_t a) {
                : "memory");
 }
 
-template <int F>
-__device__ __forceinline__ void mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  if constexpr (F == kv::kBf16)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_e4m3(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <bool SIGNED>
+__device__ __forceinline__ void mma_int8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (SIGNED)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Two 8-bit values (the bytes `SEL` of x) as a pair of fp16.  int8: x holds value + 128 as a byte u, and the fp16 with
-// bits 0x6400 | u is 1024 + u, so one subtraction gives the value exactly.
-template <int F, int PAIR>
-__device__ __forceinline__ uint32_t half_pair(uint32_t x) {
-  if constexpr (F == kv::kInt8) {
-    const uint32_t biased = __byte_perm(x, 0x64646464u, PAIR == 0 ? 0x4140 : 0x4342);
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2_raw v = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(PAIR == 0 ? x & 0xffffu : x >> 16), __NV_E4M3);
-    return (uint32_t)v.x | ((uint32_t)v.y << 16);
-  }
-}
-template <int F>
-__device__ __forceinline__ uint32_t unsign(uint32_t x) {
-  return F == kv::kInt8 ? x ^ 0x80808080u : x;
+// An integer accumulator that starts at these bits is, read as a float, 1.5 2^23 plus the sum (below 2^22 in magnitude).
+constexpr int ZERO_BITS = 0x4b400000;
+__device__ __forceinline__ float sum_of(int bits) { return __fadd_rn(__int_as_float(bits), -12582912.f); }
+
+// Byte `BYTE` of four words as one word.
+template <int BYTE>
+__device__ __forceinline__ uint32_t gather_bytes(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
+  constexpr uint32_t pick = BYTE | ((BYTE + 4) << 4);
+  return __byte_perm(__byte_perm(x0, x1, pick), __byte_perm(x2, x3, pick), 0x5410);
 }
 
-template <int F>
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
-  if constexpr (F == kv::kBf16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
+// Four floats rounded to e4m3, and 16 times what the rounding left of each.
+__device__ __forceinline__ uint32_t take_digit(float* x) {
+  uint32_t word = 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * h], x[2 * h + 1]), __NV_SATFINITE, __NV_E4M3);
+    const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+    x[2 * h] = 16.f * (x[2 * h] - back.x);
+    x[2 * h + 1] = 16.f * (x[2 * h + 1] - back.y);
+    word |= (uint32_t)two << (16 * h);
   }
+  return word;
 }
-template <int F>
-__device__ __forceinline__ float2 unpack(uint32_t x) {
-  if constexpr (F == kv::kBf16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-  else return __half22float2(*reinterpret_cast<const __half2*>(&x));
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
+__device__ __forceinline__ float2 unpack_bf16(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
 
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
@@ -328,7 +339,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
             constexpr int PER = S::ROW / 16;  // 16-byte pieces of a row
             const int q = j * 32 + lane, r = q / PER, ch = q % PER;
             const int kch = PER >= 8 ? ch ^ ((r & 1) << 2) : ch;
-            const int vch = F == kv::kBf16 ? ch ^ (r & 7) : PER >= 8 ? ch ^ (((r >> 1) & 3) << 1) : ch;
+            const int vch = F == kv::kBf16 ? ch ^ (r & 7) : PER >= 8 ? ch ^ (((r >> 2) & 3) << 1) : ch ^ ((r >> 2) & 3);
             copy16(base + (i * 16 + r) * S::ROW + kch * 16, ks + q * 16, r < real, policy);
             copy16(base + S::DATA + (i * 16 + r) * S::ROW + vch * 16, vs + q * 16, r < real, policy);
           }
@@ -353,9 +364,10 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
     for (int s = 1; s < S::STAGES - 1; ++s) issue(s);
 
     // Per row: q as fragments of the first operand, the output's accumulators, and the softmax's state.
-    constexpr int QR = D / 8;  // registers of q
+    constexpr int DIGITS = F == kv::kInt8 ? 3 : 2;  // 8 bits: of q
+    constexpr int QR = F == kv::kBf16 ? D / 8 : DIGITS * (D / 16);
     uint32_t q[QR];
-    float o[NT][4], m = -INFINITY, sum = 0.f, up = 1.f;  // up: the power of two that q was divided by
+    float o[NT][F == kv::kBf16 ? 4 : 2], m = -INFINITY, sum = 0.f, up = 1.f;  // up: what scores are multiplied by for the digits of q
     int row_tile = 0;          // the row's first tile in this warp
     bool opened = false, first_row = true;
     int stage = 0;
@@ -368,7 +380,10 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
         m = -INFINITY;
         sum = 0.f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+        for (int t = 0; t < NT; ++t) {
+          o[t][0] = o[t][1] = 0.f;
+          if constexpr (F == kv::kBf16) o[t][2] = o[t][3] = 0.f;
+        }
         const int in_group = (use.row % chunks) * HEADS + g;
         const bool real = in_group < group;
         const __nv_bfloat16* src = a.q + use.b * a.q_seq + ((long long)(use.row / chunks) * group + in_group) * a.q_head;
@@ -380,30 +395,44 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
             q[4 * j] = x.x, q[4 * j + 1] = x.y, q[4 * j + 2] = x.z, q[4 * j + 3] = x.w;
           }
         } else {
-          float top = 0.f;
+          float x[D / 4];
+          uint32_t largest = 0;  // magnitude as bits: infinities and NaN above all numbers
 #pragma unroll
           for (int j = 0; j < D / 64; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint4 x = real ? *reinterpret_cast<const uint4*>(src + (j * 4 + c4) * 16 + h * 8) : make_uint4(0, 0, 0, 0);
-              uint32_t* to = q + 8 * j + 4 * h;
-              to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+              const uint4 raw = real ? *reinterpret_cast<const uint4*>(src + (j * 4 + c4) * 16 + h * 8) : make_uint4(0, 0, 0, 0);
+              const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const float2 f = unpack<kv::kBf16>(to[r]);
-                top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                const float2 f = unpack_bf16(w[r]);
+                x[16 * j + 8 * h + 2 * r] = f.x;
+                x[16 * j + 8 * h + 2 * r + 1] = f.y;
+                largest = max(largest, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
               }
             }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+          largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
           // the power of two that brings the largest magnitude into [1, 2): exact both ways
-          const int exponent = max(-126, min(126, (int)(__float_as_uint(top) >> 23) - 127));
-          const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
-          up = __uint_as_float((uint32_t)(127 + exponent) << 23);
+          const int exponent = max(-100, min(100, (int)(largest >> 23) - 127));
+          constexpr int BITS = F == kv::kInt8 ? 21 : 7;
+          const float down = __uint_as_float((uint32_t)(127 - exponent + BITS) << 23);
+          up = largest < 0x7f800000u ? __uint_as_float((uint32_t)(127 + exponent - BITS) << 23) : __int_as_float(0x7fc00000);
 #pragma unroll
-          for (int r = 0; r < QR; ++r) {
-            const float2 f = unpack<kv::kBf16>(q[r]);
-            q[r] = pack<F>(f.x * down, f.y * down);
+          for (int r = 0; r < D / 16; ++r) {
+            if constexpr (F == kv::kInt8) {
+              // bytes of y + 0x808080, less 128 each, are its signed digits
+              uint32_t y[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[e] = (uint32_t)(__float2int_rn(x[4 * r + e] * down) + 0x808080);
+              q[3 * r] = gather_bytes<2>(y[0], y[1], y[2], y[3]) ^ 0x80808080u;
+              q[3 * r + 1] = gather_bytes<1>(y[0], y[1], y[2], y[3]) ^ 0x80808080u;
+              q[3 * r + 2] = gather_bytes<0>(y[0], y[1], y[2], y[3]) ^ 0x80808080u;
+            } else {
+              float y[4] = {x[4 * r] * down, x[4 * r + 1] * down, x[4 * r + 2] * down, x[4 * r + 3] * down};
+              q[2 * r] = take_digit(y);
+              q[2 * r + 1] = take_digit(y);
+            }
           }
         }
       }
@@ -431,120 +460,207 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
         }
         __syncwarp();
       }
-      // scores, in the accumulator's layout: head g, tokens 8 t + 2 c4 and + 1
-      float acc[TOK / 8][4];
-#pragma unroll
-      for (int t = 0; t < TOK / 8; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
       if constexpr (F == kv::kBf16) {
+        // scores, in the accumulator's layout: head g, tokens 8 t + 2 c4 and + 1
+        float acc[TOK / 8][4], s[TOK / 8][2];
+#pragma unroll
+        for (int t = 0; t < TOK / 8; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
 #pragma unroll
           for (int t = 0; t < TOK / 8; ++t) {
             const uint4 k = lds128(kb + (t * 8 + g) * S::ROW + (((j * 4 + c4) ^ ((g & 1) << 2)) * 16));
-            mma<F>(acc[t], q[4 * j], 0u, q[4 * j + 1], 0u, k.x, k.y);
-            mma<F>(acc[t], q[4 * j + 2], 0u, q[4 * j + 3], 0u, k.z, k.w);
+            mma_bf16(acc[t], q[4 * j], 0u, q[4 * j + 1], 0u, k.x, k.y);
+            mma_bf16(acc[t], q[4 * j + 2], 0u, q[4 * j + 3], 0u, k.z, k.w);
           }
-      } else {
+        float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-          uint32_t w[TOK / 8][4];
-#pragma unroll
-          for (int t = 0; t < TOK / 8; ++t) {
-            const uint4 k = lds128(kb + (t * 8 + g) * S::ROW + ((D == 128 ? (j * 4 + c4) ^ ((g & 1) << 2) : c4) * 16));
-            w[t][0] = unsign<F>(k.x), w[t][1] = unsign<F>(k.y), w[t][2] = unsign<F>(k.z), w[t][3] = unsign<F>(k.w);
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int t = 0; t < TOK / 8; ++t)
-              mma<F>(acc[t], q[8 * j + 2 * r], 0u, q[8 * j + 2 * r + 1], 0u, half_pair<F, 0>(w[t][r]), half_pair<F, 1>(w[t][r]));
-        }
-      }
-      float s[TOK / 8][2], inv[TOK / 8][2];
-      float top = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < TOK / 8; ++t) {
-        if constexpr (F == kv::kBf16) {
+        for (int t = 0; t < TOK / 8; ++t) {
           const int token = use.tile * TOK + t * 8 + 2 * c4;
           const bool pool_ok = (in_pool >> (t / 2)) & 1u;
           s[t][0] = pool_ok && token < use.n ? acc[t][0] * a.scale_log2 : -INFINITY;
           s[t][1] = pool_ok && token + 1 < use.n ? acc[t][1] * a.scale_log2 : -INFINITY;
-        } else {
-          const float4 f0 = factors[t * 8 + 2 * c4], f1 = factors[t * 8 + 2 * c4 + 1];
-          s[t][0] = fmaf(acc[t][0] * up, f0.x, f0.y);
-          s[t][1] = fmaf(acc[t][1] * up, f1.x, f1.y);
-          inv[t][0] = f0.z;
-          inv[t][1] = f1.z;
+          top = fmaxf(top, fmaxf(s[t][0], s[t][1]));
         }
-        top = fmaxf(top, fmaxf(s[t][0], s[t][1]));
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float higher = fmaxf(m, top);
-      const float at = higher == -INFINITY ? 0.f : higher;  // nothing but masked tokens so far
-      if (__any_sync(0xffffffffu, higher > m)) {
-        const float keep = fast_exp2(m - at);
-        sum *= keep;
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float higher = fmaxf(m, top);
+        const float at = higher == -INFINITY ? 0.f : higher;  // nothing but masked tokens so far
+        if (__any_sync(0xffffffffu, higher > m)) {
+          const float keep = fast_exp2(m - at);
+          sum *= keep;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          o[t][0] *= keep, o[t][1] *= keep, o[t][2] *= keep, o[t][3] *= keep;
+          for (int t = 0; t < NT; ++t) o[t][0] *= keep, o[t][1] *= keep, o[t][2] *= keep, o[t][3] *= keep;
+          m = higher;
         }
-        m = higher;
-      }
 #pragma unroll
-      for (int t = 0; t < TOK / 8; ++t)
+        for (int t = 0; t < TOK / 8; ++t)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float p = fast_exp2(s[t][e] - at);
-          if constexpr (F == kv::kBf16) sum += p;
-          else sum = fmaf(p, inv[t][e], sum);
-          s[t][e] = p;
-        }
-
-      // o += p v, the rounding's remainder of p in rows 8 to 15
+          for (int e = 0; e < 2; ++e) {
+            s[t][e] = fast_exp2(s[t][e] - at);
+            sum += s[t][e];
+          }
+        // o += p v, the rounding's remainder of p in rows 8 to 15
 #pragma unroll
-      for (int kk = 0; kk < GROUPS; ++kk) {
-        uint32_t hi[2], lo[2];
+        for (int kk = 0; kk < GROUPS; ++kk) {
+          uint32_t hi[2], lo[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float x = s[2 * kk + h][0], y = s[2 * kk + h][1];
-          hi[h] = pack<F>(x, y);
-          const float2 back = unpack<F>(hi[h]);
-          lo[h] = pack<F>(x - back.x, y - back.y);
-        }
-        if constexpr (F == kv::kBf16) {
+          for (int h = 0; h < 2; ++h) {
+            const float x = s[2 * kk + h][0], y = s[2 * kk + h][1];
+            hi[h] = pack_bf16(x, y);
+            const float2 back = unpack_bf16(hi[h]);
+            lo[h] = pack_bf16(x - back.x, y - back.y);
+          }
           const int mat = lane / 8, r = kk * 16 + (mat & 1) * 8 + (lane & 7);
           const uint32_t row = vb + r * S::ROW;
 #pragma unroll
           for (int np = 0; np < NT / 2; ++np) {
             uint32_t v[4];
             ldmatrix4t(v, row + (((2 * np + (mat >> 1)) ^ (r & 7)) * 16));
-            mma<F>(o[2 * np], hi[0], lo[0], hi[1], lo[1], v[0], v[1]);
-            mma<F>(o[2 * np + 1], hi[0], lo[0], hi[1], lo[1], v[2], v[3]);
+            mma_bf16(o[2 * np], hi[0], lo[0], hi[1], lo[1], v[0], v[1]);
+            mma_bf16(o[2 * np + 1], hi[0], lo[0], hi[1], lo[1], v[2], v[3]);
           }
-        } else {
-          // lane (g, c4) takes dimensions g * NT ... + NT - 1 of the tokens 2 c4, 2 c4 + 1, 2 c4 + 8, 2 c4 + 9
-          constexpr int WORDS = NT / 4;
-          uint32_t w[4][WORDS];
+        }
+      } else {
+        // Column n of score tile i is the token place(i) + 4 (n / 2) + n % 2: the lane's scores of four tiles are then tokens
+        // 4 c4 ... + 3 and 16 + 4 c4 ... + 3 of a block of 32, in the order of the second product's operand.
+        constexpr int BLOCKS = TOK / 32;
+        const auto place = [](int i) { return i / 4 * 32 + i % 4 / 2 * 16 + i % 2 * 2; };
+        float s[TOK / 8][2];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int r = kk * 16 + 2 * c4 + (x & 1) + (x >> 1) * 8;
-            if constexpr (D == 128) {
-              const uint4 v = lds128(vb + r * S::ROW + ((g ^ (((r >> 1) & 3) << 1)) * 16));
-              w[x][0] = unsign<F>(v.x), w[x][1] = unsign<F>(v.y), w[x][2] = unsign<F>(v.z), w[x][3] = unsign<F>(v.w);
+        for (int i = 0; i < TOK / 8; ++i) {
+          const uint32_t row = kb + (place(i) + 4 * (g >> 1) + (g & 1)) * S::ROW;
+          if constexpr (F == kv::kInt8) {
+            int x[4] = {ZERO_BITS, ZERO_BITS, ZERO_BITS, ZERO_BITS}, y[4] = {ZERO_BITS, ZERO_BITS, ZERO_BITS, ZERO_BITS};
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) {
+              const uint4 k = lds128(row + ((D == 128 ? (j * 4 + c4) ^ ((g & 1) << 2) : c4) * 16));
+              const uint32_t* d = q + 12 * j;
+              mma_int8<true>(x, d[0], d[1], d[3], d[4], k.x, k.y);
+              mma_int8<true>(y, d[2], 0u, d[5], 0u, k.x, k.y);
+              mma_int8<true>(x, d[6], d[7], d[9], d[10], k.z, k.w);
+              mma_int8<true>(y, d[8], 0u, d[11], 0u, k.z, k.w);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[i][e] = fmaf(sum_of(x[e]), 65536.f, fmaf(sum_of(x[e + 2]), 256.f, sum_of(y[e])));
+          } else {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) {
+              const uint4 k = lds128(row + ((D == 128 ? (j * 4 + c4) ^ ((g & 1) << 2) : c4) * 16));
+              const uint32_t* d = q + 8 * j;
+              mma_e4m3(x, d[0], d[1], d[2], d[3], k.x, k.y);
+              mma_e4m3(x, d[4], d[5], d[6], d[7], k.z, k.w);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[i][e] = fmaf(x[e + 2], 0.0625f, x[e]);
+          }
+        }
+        float inv[TOK / 8][2], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < TOK / 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float4 f = factors[place(i) + 4 * c4 + e];
+            s[i][e] = fmaf(s[i][e] * up, f.x, f.y);
+            inv[i][e] = f.z;
+            top = fmaxf(top, s[i][e]);
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float at = top == -INFINITY ? 0.f : top;  // of this tile
+        const float higher = fmaxf(m, top), now = higher == -INFINITY ? 0.f : higher;
+        if (__any_sync(0xffffffffu, higher > m)) {
+          const float keep = fast_exp2(m - now);
+          sum *= keep;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) o[t][0] *= keep, o[t][1] *= keep;
+          m = higher;
+        }
+        const float share = fast_exp2(top - now);  // of the tile's weights
+        float tile_sum = 0.f;
+        constexpr int TERMS = F == kv::kInt8 ? 2 : 3;
+        uint32_t p[BLOCKS][2][TERMS];  // digits of the weights of tokens 4 c4 ... and 16 + 4 c4 ...
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = 4 * b + 2 * h + e / 2;
+              x[e] = fast_exp2(s[i][e % 2] - at);
+              tile_sum = fmaf(x[e], inv[i][e % 2], tile_sum);
+            }
+            if constexpr (F == kv::kInt8) {
+              // 2^23 + rint(65535 x): the low bytes are the digits
+              uint32_t y[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(fmaf(x[e], 65535.f, 8388608.f));
+              p[b][h][0] = gather_bytes<1>(y[0], y[1], y[2], y[3]);
+              p[b][h][1] = gather_bytes<0>(y[0], y[1], y[2], y[3]);
             } else {
-              const uint2 v = lds64(vb + r * S::ROW + g * 8);
-              w[x][0] = unsign<F>(v.x), w[x][1] = unsign<F>(v.y);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] *= 256.f;
+              p[b][h][0] = take_digit(x);
+              p[b][h][1] = take_digit(x);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] *= 0.0625f;  // the third digit counts as much as the second
+              p[b][h][2] = take_digit(x);
             }
           }
+        sum = fmaf(share, tile_sum, sum);
+
+        // o += share p v; lane (g, c4) takes dimensions g NT ... + NT - 1 of the tokens whose weights it has
+        constexpr int WORDS = NT / 4;
+        uint32_t w[BLOCKS][8][WORDS];
 #pragma unroll
-          for (int y = 0; y < WORDS; ++y) {
-            const uint32_t a01 = __byte_perm(w[0][y], w[1][y], 0x5140), a23 = __byte_perm(w[0][y], w[1][y], 0x7362);
-            const uint32_t b01 = __byte_perm(w[2][y], w[3][y], 0x5140), b23 = __byte_perm(w[2][y], w[3][y], 0x7362);
-            mma<F>(o[4 * y], hi[0], lo[0], hi[1], lo[1], half_pair<F, 0>(a01), half_pair<F, 0>(b01));
-            mma<F>(o[4 * y + 1], hi[0], lo[0], hi[1], lo[1], half_pair<F, 1>(a01), half_pair<F, 1>(b01));
-            mma<F>(o[4 * y + 2], hi[0], lo[0], hi[1], lo[1], half_pair<F, 0>(a23), half_pair<F, 0>(b23));
-            mma<F>(o[4 * y + 3], hi[0], lo[0], hi[1], lo[1], half_pair<F, 1>(a23), half_pair<F, 1>(b23));
+        for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int r = b * 32 + x / 4 * 16 + 4 * c4 + x % 4;
+            if constexpr (D == 128) {
+              const uint4 v = lds128(vb + r * S::ROW + ((g ^ (c4 << 1)) * 16));
+              w[b][x][0] = v.x, w[b][x][1] = v.y, w[b][x][2] = v.z, w[b][x][3] = v.w;
+            } else {
+              const uint2 v = lds64(vb + r * S::ROW + ((g / 2 ^ c4) * 16) + (g & 1) * 8);
+              w[b][x][0] = v.x, w[b][x][1] = v.y;
+            }
+          }
+        const float first = share * (F == kv::kInt8 ? 256.f / 65535.f : 1.f / 256.f), second = share * (F == kv::kInt8 ? 1.f / 65535.f : 1.f / 4096.f);
+#pragma unroll
+        for (int y = 0; y < WORDS; ++y) {
+          uint32_t v[BLOCKS][2][4];  // four tokens' bytes of each of four dimensions
+#pragma unroll
+          for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t a01 = __byte_perm(w[b][4 * h][y], w[b][4 * h + 1][y], 0x5140), a23 = __byte_perm(w[b][4 * h][y], w[b][4 * h + 1][y], 0x7362);
+              const uint32_t b01 = __byte_perm(w[b][4 * h + 2][y], w[b][4 * h + 3][y], 0x5140), b23 = __byte_perm(w[b][4 * h + 2][y], w[b][4 * h + 3][y], 0x7362);
+              v[b][h][0] = __byte_perm(a01, b01, 0x5410);
+              v[b][h][1] = __byte_perm(a01, b01, 0x7632);
+              v[b][h][2] = __byte_perm(a23, b23, 0x5410);
+              v[b][h][3] = __byte_perm(a23, b23, 0x7632);
+            }
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            float* const out = o[4 * y + z];
+            if constexpr (F == kv::kInt8) {
+              int x[4] = {ZERO_BITS, ZERO_BITS, ZERO_BITS, ZERO_BITS};
+#pragma unroll
+              for (int b = 0; b < BLOCKS; ++b) mma_int8<false>(x, p[b][0][0], p[b][0][1], p[b][1][0], p[b][1][1], v[b][0][z], v[b][1][z]);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) out[e] = fmaf(sum_of(x[e]), first, fmaf(sum_of(x[e + 2]), second, out[e]));
+            } else {
+              float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int b = 0; b < BLOCKS; ++b) {
+                mma_e4m3(x, p[b][0][0], p[b][0][1], p[b][1][0], p[b][1][1], v[b][0][z], v[b][1][z]);
+                mma_e4m3(x, 0u, p[b][0][2], 0u, p[b][1][2], v[b][0][z], v[b][1][z]);
+              }
+#pragma unroll
+              for (int e = 0; e < 2; ++e) out[e] = fmaf(x[e], first, fmaf(x[e + 2], second, out[e]));
+            }
           }
         }
       }
@@ -555,6 +671,10 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
       if (row_ends || last) {
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const auto value = [&](int t, int e) {
+          if constexpr (F == kv::kBf16) return o[t][e] + o[t][e + 2];
+          else return o[t][e];
+        };
         // where accumulator column n of tile t lies in the head's dimensions
         const auto dim = [&](int t, int e) { return F == kv::kBf16 ? t * 8 + 2 * c4 + e : (2 * c4 + e) * NT + t; };
         if (row_ends && row_tile == 0) {
@@ -566,7 +686,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
             if constexpr (F == kv::kBf16) {
 #pragma unroll
               for (int t = 0; t < NT; ++t)
-                *reinterpret_cast<uint32_t*>(dst + dim(t, 0)) = pack<kv::kBf16>((o[t][0] + o[t][2]) * norm, (o[t][1] + o[t][3]) * norm);
+                *reinterpret_cast<uint32_t*>(dst + dim(t, 0)) = pack_bf16(value(t, 0) * norm, value(t, 1) * norm);
             } else {
 #pragma unroll
               for (int e = 0; e < 2; ++e)
@@ -575,7 +695,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
                   uint32_t x[4];
 #pragma unroll
                   for (int y = 0; y < 4; ++y)
-                    x[y] = pack<kv::kBf16>((o[t + 2 * y][e] + o[t + 2 * y][e + 2]) * norm, (o[t + 2 * y + 1][e] + o[t + 2 * y + 1][e + 2]) * norm);
+                    x[y] = pack_bf16(value(t + 2 * y, e) * norm, value(t + 2 * y + 1, e) * norm);
                   *reinterpret_cast<uint4*>(dst + dim(t, e)) = make_uint4(x[0], x[1], x[2], x[3]);
                 }
             }
@@ -594,7 +714,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) piece[(2 * t + e) * 32 + lane] = o[t][e] + o[t][e + 2];
+            for (int e = 0; e < 2; ++e) piece[(2 * t + e) * 32 + lane] = value(t, e);
           if (c4 == 0) {
             piece[HEADS * D + g] = m;
             piece[HEADS * D + HEADS + g] = sum;
