@@ -20,13 +20,14 @@
 //   what rounding left over of the same heads' operand.  In bf16 (m16n8k16) P enters as two bf16 terms.  The
 //   dimensions of q and k are summed in the order in which 16-byte loads deliver them, and the tokens of a tile in
 //   the order in which score accumulators and the second product's operand agree: no data is moved for either.
-// * 8 bits (m16n8k32).  Keys and values enter the instructions as they are held, so the other operand has to be in
-//   8 bits too, as digits.  int8: q of a head, scaled by a power of two and rounded to 22 bits, is three signed
-//   digits, p is rint(65535 p) in two unsigned ones, and the sums are exact integers (below 2^22, read as floats by
-//   starting the accumulators at the bits of 1.5 2^23).  e4m3: q is two terms of 4 bits each, which hold all 8 bits
-//   of a bf16, and p three.  p is taken relative to the tile's own maximum, so that its digits always start
-//   at the tile's largest weight, and the tile's product is added to the output in fp32.  (With values converted to
-//   fp16 instead, the conversions alone were half of the instructions: 64 against NN us on 32 rows of 4096 int8.)
+// * 8 bits.  Keys enter the instructions (m16n8k32) as they are held, so q has to be in 8 bits too, as digits, worked
+//   out once per row.  int8: q of a head, scaled by a power of two and rounded to 22 bits, is three signed digits, and
+//   the sums are exact integers (below 2^22, read as floats by starting the accumulators at the bits of 1.5 2^23).
+//   e4m3: q is two terms of 4 bits each, which hold all 8 bits of a bf16.  int8 values are used as they are as well,
+//   with rint(65535 p) as two unsigned digits: p is taken relative to the tile's own maximum, so that its digits always
+//   start at the tile's largest weight, and the tile's product is added to the output in fp32.  e4m3 values are
+//   converted to fp16 pairs (one conversion costs what a byte permute does; three e4m3 terms of p per token
+//   cost more: 82 us against 71 on 32 rows of 4096).
 //   A token's key scale multiplies its score.  Its value scale sv joins the exponent: with s'_t = s_t + log2(sv_t) and
 //   m the maximum of s', p_t = 2^(s'_t - m) <= 1, the output is sum p_t v_t / sum (p_t / sv_t): p stays in range
 //   whatever the scales are.
@@ -48,10 +49,12 @@ template <int F, int D>
 struct Shape {
   static constexpr int ROW = D * (F == kv::kBf16 ? 2 : 1);  // bytes of one key
   static constexpr int TOK = ROW == 256 ? 16 : ROW == 64 ? 64 : 32;  // tokens of one tile: 8 KB of keys and values
-  static constexpr int WARPS = 8;
+  // Warps of a block, as many as registers and shared memory take and measured best (10 and 12 instead of 8: 91 against 94 us
+  // on 32 rows of 4096 at D = 128 in bf16, 69 against 73 at D = 64; int8 at D = 128 spills registers with 10: 67 against 59).
+  static constexpr int WARPS = F == kv::kBf16 ? (D == 64 ? 12 : 10) : (D == 64 ? 10 : 8);
   static constexpr int DATA = TOK * ROW, SCALES = F == kv::kBf16 ? 0 : TOK * 4;
   static constexpr int STAGE = 2 * (DATA + SCALES);
-  static constexpr int STAGES = F == kv::kBf16 ? 3 : 2;
+  static constexpr int STAGES = 2;  // one tile under way while the other is used
   static constexpr int PIECE = HEADS * (D + 2) * 4;  // o, m and sum of one row's piece
   static constexpr int THREADS = WARPS * 32;
   static constexpr int FACTORS = F == kv::kBf16 ? 0 : TOK * 16;  // per token: what its scales do to score and weight
@@ -96,6 +99,11 @@ __device__ __forceinline__ void ldmatrix4t(uint32_t* r, uint32_t a) {
 
 __device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -144,6 +152,17 @@ __device__ __forceinline__ uint32_t take_digit(float* x) {
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float2 unpack_half(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+// Two e4m3 values (the first or the second two bytes) as fp16.
+template <int PAIR>
+__device__ __forceinline__ uint32_t half_pair(uint32_t x) {
+  const __half2_raw v = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(PAIR == 0 ? x & 0xffffu : x >> 16), __NV_E4M3);
+  return (uint32_t)v.x | ((uint32_t)v.y << 16);
 }
 __device__ __forceinline__ float2 unpack_bf16(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
 
@@ -261,8 +280,9 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
   int mine = sums(0, true), upto = scan(mine);
   int line = __shfl_sync(0xffffffffu, upto, 31);
   for (int b0 = 1024; b0 < a.B; b0 += 1024) line += (int)__reduce_add_sync(0xffffffffu, (uint32_t)sums(b0, true));
-  // at least one tile for each warp of a block: fewer, fuller blocks have fewer pieces to join
-  const int per_block = max((int)((line + gridDim.x - 1) / gridDim.x), WARPS);
+  // at least 8 tiles, a tile a warp: fewer, fuller blocks have fewer pieces to join, and rows of a power of two of tiles end with
+  // a block
+  const int per_block = max((int)((line + gridDim.x - 1) / gridDim.x), 8);
   const int block_from = (int)min((long long)line, (long long)per_block * blockIdx.x);
   const int block_to = min(line - block_from, per_block) + block_from;
   if (block_from >= block_to) return;
@@ -367,7 +387,8 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
     constexpr int DIGITS = F == kv::kInt8 ? 3 : 2;  // 8 bits: of q
     constexpr int QR = F == kv::kBf16 ? D / 8 : DIGITS * (D / 16);
     uint32_t q[QR];
-    float o[NT][F == kv::kBf16 ? 4 : 2], m = -INFINITY, sum = 0.f, up = 1.f;  // up: what scores are multiplied by for the digits of q
+    constexpr int PLACES = F == kv::kInt8 ? 2 : 4;  // of an accumulator; int8 adds up tiles in fp32 itself
+    float o[NT][PLACES], m = -INFINITY, sum = 0.f, up = 1.f;  // up: what scores are multiplied by for the digits of q
     int row_tile = 0;          // the row's first tile in this warp
     bool opened = false, first_row = true;
     int stage = 0;
@@ -382,7 +403,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           o[t][0] = o[t][1] = 0.f;
-          if constexpr (F == kv::kBf16) o[t][2] = o[t][3] = 0.f;
+          if constexpr (PLACES == 4) o[t][2] = o[t][3] = 0.f;
         }
         const int in_group = (use.row % chunks) * HEADS + g;
         const bool real = in_group < group;
@@ -568,50 +589,17 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
           }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float at = top == -INFINITY ? 0.f : top;  // of this tile
-        const float higher = fmaxf(m, top), now = higher == -INFINITY ? 0.f : higher;
+        const float higher = fmaxf(m, top), now = higher == -INFINITY ? 0.f : higher;  // nothing but masked tokens so far
         if (__any_sync(0xffffffffu, higher > m)) {
           const float keep = fast_exp2(m - now);
           sum *= keep;
 #pragma unroll
-          for (int t = 0; t < NT; ++t) o[t][0] *= keep, o[t][1] *= keep;
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < PLACES; ++e) o[t][e] *= keep;
           m = higher;
         }
-        const float share = fast_exp2(top - now);  // of the tile's weights
-        float tile_sum = 0.f;
-        constexpr int TERMS = F == kv::kInt8 ? 2 : 3;
-        uint32_t p[BLOCKS][2][TERMS];  // digits of the weights of tokens 4 c4 ... and 16 + 4 c4 ...
-#pragma unroll
-        for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int i = 4 * b + 2 * h + e / 2;
-              x[e] = fast_exp2(s[i][e % 2] - at);
-              tile_sum = fmaf(x[e], inv[i][e % 2], tile_sum);
-            }
-            if constexpr (F == kv::kInt8) {
-              // 2^23 + rint(65535 x): the low bytes are the digits
-              uint32_t y[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(fmaf(x[e], 65535.f, 8388608.f));
-              p[b][h][0] = gather_bytes<1>(y[0], y[1], y[2], y[3]);
-              p[b][h][1] = gather_bytes<0>(y[0], y[1], y[2], y[3]);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] *= 256.f;
-              p[b][h][0] = take_digit(x);
-              p[b][h][1] = take_digit(x);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] *= 0.0625f;  // the third digit counts as much as the second
-              p[b][h][2] = take_digit(x);
-            }
-          }
-        sum = fmaf(share, tile_sum, sum);
-
-        // o += share p v; lane (g, c4) takes dimensions g NT ... + NT - 1 of the tokens whose weights it has
+        // lane (g, c4) takes dimensions g NT ... + NT - 1 of the tokens whose weights it has
         constexpr int WORDS = NT / 4;
         uint32_t w[BLOCKS][8][WORDS];
 #pragma unroll
@@ -627,41 +615,79 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
               w[b][x][0] = v.x, w[b][x][1] = v.y;
             }
           }
-        const float first = share * (F == kv::kInt8 ? 256.f / 65535.f : 1.f / 256.f), second = share * (F == kv::kInt8 ? 1.f / 65535.f : 1.f / 4096.f);
-#pragma unroll
-        for (int y = 0; y < WORDS; ++y) {
-          uint32_t v[BLOCKS][2][4];  // four tokens' bytes of each of four dimensions
+        if constexpr (F == kv::kInt8) {
+          const float at = top == -INFINITY ? 0.f : top;  // of this tile
+          const float share = fast_exp2(top - now);       // of the tile's weights
+          float tile_sum = 0.f;
+          uint32_t p[BLOCKS][2][2];  // digits of the weights of tokens 4 c4 ... and 16 + 4 c4 ...
 #pragma unroll
           for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t a01 = __byte_perm(w[b][4 * h][y], w[b][4 * h + 1][y], 0x5140), a23 = __byte_perm(w[b][4 * h][y], w[b][4 * h + 1][y], 0x7362);
-              const uint32_t b01 = __byte_perm(w[b][4 * h + 2][y], w[b][4 * h + 3][y], 0x5140), b23 = __byte_perm(w[b][4 * h + 2][y], w[b][4 * h + 3][y], 0x7362);
-              v[b][h][0] = __byte_perm(a01, b01, 0x5410);
-              v[b][h][1] = __byte_perm(a01, b01, 0x7632);
-              v[b][h][2] = __byte_perm(a23, b23, 0x5410);
-              v[b][h][3] = __byte_perm(a23, b23, 0x7632);
-            }
+              uint32_t y[4];  // 2^23 + rint(65535 p): the low bytes are the digits
 #pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            float* const out = o[4 * y + z];
-            if constexpr (F == kv::kInt8) {
+              for (int e = 0; e < 4; ++e) {
+                const int i = 4 * b + 2 * h + e / 2;
+                const float x = fast_exp2(s[i][e % 2] - at);
+                tile_sum = fmaf(x, inv[i][e % 2], tile_sum);
+                y[e] = __float_as_uint(fmaf(x, 65535.f, 8388608.f));
+              }
+              p[b][h][0] = gather_bytes<1>(y[0], y[1], y[2], y[3]);
+              p[b][h][1] = gather_bytes<0>(y[0], y[1], y[2], y[3]);
+            }
+          sum = fmaf(share, tile_sum, sum);
+          const float first = share * (256.f / 65535.f), second = share * (1.f / 65535.f);
+#pragma unroll
+          for (int y = 0; y < WORDS; ++y) {
+            uint32_t v[BLOCKS][2][4];  // four tokens' bytes of each of four dimensions
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t t0 = w[b][4 * h][y], t1 = w[b][4 * h + 1][y], t2 = w[b][4 * h + 2][y], t3 = w[b][4 * h + 3][y];
+                const uint32_t a01 = __byte_perm(t0, t1, 0x5140), a23 = __byte_perm(t0, t1, 0x7362);
+                const uint32_t b01 = __byte_perm(t2, t3, 0x5140), b23 = __byte_perm(t2, t3, 0x7362);
+                v[b][h][0] = __byte_perm(a01, b01, 0x5410);
+                v[b][h][1] = __byte_perm(a01, b01, 0x7632);
+                v[b][h][2] = __byte_perm(a23, b23, 0x5410);
+                v[b][h][3] = __byte_perm(a23, b23, 0x7632);
+              }
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
               int x[4] = {ZERO_BITS, ZERO_BITS, ZERO_BITS, ZERO_BITS};
 #pragma unroll
               for (int b = 0; b < BLOCKS; ++b) mma_int8<false>(x, p[b][0][0], p[b][0][1], p[b][1][0], p[b][1][1], v[b][0][z], v[b][1][z]);
 #pragma unroll
-              for (int e = 0; e < 2; ++e) out[e] = fmaf(sum_of(x[e]), first, fmaf(sum_of(x[e + 2]), second, out[e]));
-            } else {
-              float x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int b = 0; b < BLOCKS; ++b) {
-                mma_e4m3(x, p[b][0][0], p[b][0][1], p[b][1][0], p[b][1][1], v[b][0][z], v[b][1][z]);
-                mma_e4m3(x, 0u, p[b][0][2], 0u, p[b][1][2], v[b][0][z], v[b][1][z]);
-              }
-#pragma unroll
-              for (int e = 0; e < 2; ++e) out[e] = fmaf(x[e], first, fmaf(x[e + 2], second, out[e]));
+              for (int e = 0; e < 2; ++e) o[4 * y + z][e] = fmaf(sum_of(x[e]), first, fmaf(sum_of(x[e + 2]), second, o[4 * y + z][e]));
             }
           }
+        } else {
+          // in fp16, which holds e4m3 values exactly: p in rows 0 to 7, what its rounding left in rows 8 to 15
+#pragma unroll
+          for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t hi[2], lo[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int i = 4 * b + 2 * h + e;
+                const float x = fast_exp2(s[i][0] - now), y = fast_exp2(s[i][1] - now);
+                sum = fmaf(x, inv[i][0], fmaf(y, inv[i][1], sum));
+                hi[e] = pack_half(x, y);
+                const float2 back = unpack_half(hi[e]);
+                lo[e] = pack_half(x - back.x, y - back.y);
+              }
+#pragma unroll
+              for (int y = 0; y < WORDS; ++y) {
+                const uint32_t t0 = w[b][4 * h][y], t1 = w[b][4 * h + 1][y], t2 = w[b][4 * h + 2][y], t3 = w[b][4 * h + 3][y];
+                const uint32_t a01 = __byte_perm(t0, t1, 0x5140), a23 = __byte_perm(t0, t1, 0x7362);
+                const uint32_t b01 = __byte_perm(t2, t3, 0x5140), b23 = __byte_perm(t2, t3, 0x7362);
+                mma_f16(o[4 * y], hi[0], lo[0], hi[1], lo[1], half_pair<0>(a01), half_pair<0>(b01));
+                mma_f16(o[4 * y + 1], hi[0], lo[0], hi[1], lo[1], half_pair<1>(a01), half_pair<1>(b01));
+                mma_f16(o[4 * y + 2], hi[0], lo[0], hi[1], lo[1], half_pair<0>(a23), half_pair<0>(b23));
+                mma_f16(o[4 * y + 3], hi[0], lo[0], hi[1], lo[1], half_pair<1>(a23), half_pair<1>(b23));
+              }
+            }
         }
       }
       __syncwarp();  // the stage may be refilled
@@ -672,7 +698,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         const auto value = [&](int t, int e) {
-          if constexpr (F == kv::kBf16) return o[t][e] + o[t][e + 2];
+          if constexpr (PLACES == 4) return o[t][e] + o[t][e + 2];
           else return o[t][e];
         };
         // where accumulator column n of tile t lies in the head's dimensions
