@@ -40,7 +40,8 @@ constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int BINS = 2048;
 constexpr int LIST = 256;       // tokens of one bin that are ranked directly
 constexpr int SHORT = 256;      // tokens of a short prefix
-constexpr int MEDIUM = 2048;    // tokens of a longer one
+constexpr int MEDIUM = 2048;    // tokens of a longer one, or of one bin
+constexpr int STAGED = BINS * 3 / 2;  // tokens that the bins' memory holds
 constexpr int MOST_BLOCKS = 8;  // of a cluster
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -110,10 +111,10 @@ struct Shared {
   Warp warps[MOST_BLOCKS][WARPS];
   uint32_t warp_top[2][WARPS];
   bool fine;
-  uint32_t count[BINS], low[BINS], high[BINS];  // masses: 2^16 high + low
+  alignas(8) uint32_t count[BINS], low[BINS], high[BINS];  // masses: 2^16 high + low; between uses, what `gather` collects
   unsigned long long list[MEDIUM], bin_list[LIST];
   uint32_t list_mass[SHORT], bin_mass[LIST];
-  uint32_t listed, bin_listed;
+  uint32_t listed, bin_listed, staged, room;
   unsigned long long scan[WARPS];
   uint32_t reduce32[WARPS];
   unsigned long long slice[MOST_BLOCKS];                      // per block of the cluster
@@ -216,25 +217,27 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     const float hi = (float)rate, lo = (float)(rate - (double)hi);
     const bool together = (reinterpret_cast<uintptr_t>(noise - skew) % 16) == 0;
     constexpr int DEPTH = E == 4 ? 8 : 4;  // pieces of a thread in flight: 128 bytes of random numbers
-    // all logits are on their way to shared memory before the first is used
-    for (int i = tid; i < count; i += THREADS)
-      if (inside(i))
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(held + i)), "l"(aligned + from + i) : "memory");
     float reference = -1e30f, best = greedy ? -INFINITY : -1.f, sum = 0.f;  // exponents are taken from `reference`, an integer
     int winner = a.V;
     for (int i0 = tid; i0 < count; i0 += DEPTH * THREADS) {
+      // all of the turn is under way before its first half is used: logits to shared memory, random numbers to registers
       float4 luck[DEPTH][E / 4];
 #pragma unroll
       for (int j = 0; j < DEPTH; ++j) {
         const int i = i0 + j * THREADS;
-        if (!greedy && together && i < count && inside(i)) {
+        if (i < count && inside(i)) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(held + i)), "l"(aligned + from + i) : "memory");
+          if (!greedy && together) {
 #pragma unroll
-          for (int x = 0; x < E / 4; ++x) luck[j][x] = __ldcs(reinterpret_cast<const float4*>(noise + (from + i) * E - skew) + x);
+            for (int x = 0; x < E / 4; ++x) luck[j][x] = __ldcs(reinterpret_cast<const float4*>(noise + (from + i) * E - skew) + x);
+          }
         }
+        if (j == DEPTH / 2 - 1) asm volatile("cp.async.commit_group;" ::: "memory");
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");  // a thread reads what it copied itself
+      asm volatile("cp.async.commit_group;\n cp.async.wait_group 1;" ::: "memory");  // a thread reads what it copied itself
 #pragma unroll
       for (int j = 0; j < DEPTH; ++j) {
+        if (j == DEPTH / 2) asm volatile("cp.async.wait_group 0;" ::: "memory");
         const int i = i0 + j * THREADS, first = (from + i) * E - skew;
         if (i >= count) continue;
         Piece<T> p(inside(i) ? held[i] : end_piece(i));
@@ -524,86 +527,126 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     return sum;
   };
 
-  // The lowest token of the shortest prefix of those at or above `cut` that holds `target` tokens, or (target 0) `share` of
-  // their mass.
-  const auto shorten = [&](auto wide, const auto& tokens, unsigned long long cut, bool masses, double share, unsigned long long target) {
-    constexpr bool WIDE = decltype(wide)::value;
-    const int n = WIDE ? blocks : 1;
-    const auto sync = [&] {
-      if (WIDE) cluster.sync();
-      else __syncthreads();
-    };
-    clear_bins();
-    tokens(cut, [&](unsigned long long number) { put(first_bin(weight, logit_of(number)), logit_of(number), masses); });
-    if (cross(wide, masses, share, target) < target) return cut;  // fewer tokens than top_k
-    Found found = sh.found;
-    const int bin = found.bin;
-    unsigned long long before = found.before, low = cut, high = ~0ull;  // bounds of the bin's tokens, once it has been divided
-    bool divided = false;
-    const auto members = [&](auto f) {
-      tokens(low, [&](unsigned long long number) {
-        if (divided ? number <= high : first_bin(weight, logit_of(number)) == bin) f(number);
-      });
-    };
-    while (found.count > LIST) {
-      if (!divided) {
-        unsigned long long least = ~0ull, most = 0ull;
-        members([&](unsigned long long number) {
-          least = min(least, number);
-          most = max(most, number);
-        });
-        least = block_reduce(least, sh.scan, [](unsigned long long x, unsigned long long y) { return x < y ? x : y; });
-        most = block_reduce(most, sh.scan, better);
-        if (WIDE) {
-          if (tid < n) {
-            *peer(&sh.ends[0][rank], tid) = least;
-            *peer(&sh.ends[1][rank], tid) = most;
-          }
-          cluster.sync();
-          for (int r = 0; r < n; ++r) {
-            least = min(least, sh.ends[0][r]);
-            most = max(most, sh.ends[1][r]);
-          }
-        }
-        low = least;
-        high = most;
-        divided = true;
-      }
-      const int shift = max(0, 64 - __clzll((long long)(high - low)) - 11);  // 2^11 bins
-      clear_bins();
-      members([&](unsigned long long number) { put((int)((high - number) >> shift), logit_of(number), masses); });
-      unsigned long long left = target - before;
-      cross(wide, masses, share, left);
-      found = sh.found;
-      before += found.before;
-      high -= (unsigned long long)found.bin << shift;
-      low = max(low, high - ((1ull << shift) - 1));
-    }
-    // The first block ranks the bin's tokens against one another.
-    members([&](unsigned long long number) {
-      const uint32_t at = atomicAdd(WIDE ? peer(&sh.bin_listed, 0) : &sh.bin_listed, 1u);
-      *(WIDE ? peer(&sh.bin_list[at], 0) : &sh.bin_list[at]) = number;
-      *(WIDE ? peer(&sh.bin_mass[at], 0) : &sh.bin_mass[at]) = masses ? weight.fixed(logit_of(number)) : 1u;
+  // Adds tokens to the first block's list: each block collects its own, and asks for room once.  Returns how many they are.
+  unsigned long long* const staging = reinterpret_cast<unsigned long long*>(sh.count);
+  const auto gather = [&](const auto& each) {
+    if (tid == 0) sh.staged = 0u;
+    __syncthreads();
+    each([&](unsigned long long number) {
+      const uint32_t at = atomicAdd(&sh.staged, 1u);
+      if (at < STAGED) staging[at] = number;
     });
-    sync();
-    if (!WIDE || rank == 0) {
-      constexpr int PARTS = THREADS / LIST;
-      const int mine = tid / PARTS;
-      const unsigned long long me = mine < (int)found.count ? sh.bin_list[mine] : ~0ull;
-      unsigned long long ahead = 0;
-      for (int j = tid % PARTS; j < (int)found.count; j += PARTS)
-        if (sh.bin_list[j] > me) ahead += sh.bin_mass[j];
-      for (int o = PARTS / 2; o > 0; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
-      const unsigned long long last =
-          block_reduce(before + ahead < target ? me : ~0ull, sh.scan, [](unsigned long long x, unsigned long long y) { return x < y ? x : y; });
-      if (tid < n) *(WIDE ? peer(&sh.cut, tid) : &sh.cut) = last;
-      if (tid == 0) sh.bin_listed = 0u;
-    }
-    sync();
-    return sh.cut;
+    __syncthreads();
+    const uint32_t mine = sh.staged;
+    if (tid == 0) sh.room = atomicAdd(peer(&sh.listed, 0), mine);
+    __syncthreads();
+    for (uint32_t i = tid; i < min(mine, (uint32_t)STAGED); i += THREADS)
+      if (sh.room + i < MEDIUM) *peer(&sh.list[sh.room + i], 0) = staging[i];
+    return mine;
   };
+  const auto smaller = [](unsigned long long x, unsigned long long y) { return x < y ? x : y; };
   using Cluster = std::integral_constant<bool, true>;
   using Block = std::integral_constant<bool, false>;
+
+  // Tokens of one bin: those of a bin of the first histogram, or, once that has been divided, those between two bounds.
+  struct Bin {
+    int first;
+    bool divided;
+    unsigned long long low, high;
+  };
+  const auto in_bin = [&](const Bin& bin, unsigned long long number) {
+    return bin.divided ? number <= bin.high : first_bin(weight, logit_of(number)) == bin.first;
+  };
+  // A histogram over the bin's tokens, by their numbers' bits; `bin` becomes the one of its 2048 parts that holds the target.
+  const auto divide = [&](auto wide, const auto& tokens, Bin& bin, Found& found, bool masses, unsigned long long target) {
+    constexpr bool WIDE = decltype(wide)::value;
+    if (!bin.divided) {
+      unsigned long long least = ~0ull, most = 0ull;
+      tokens(bin.low, [&](unsigned long long number) {
+        if (!in_bin(bin, number)) return;
+        least = min(least, number);
+        most = max(most, number);
+      });
+      least = block_reduce(least, sh.scan, smaller);
+      most = block_reduce(most, sh.scan, better);
+      if (WIDE) {
+        if (tid < blocks) {
+          *peer(&sh.ends[0][rank], tid) = least;
+          *peer(&sh.ends[1][rank], tid) = most;
+        }
+        cluster.sync();
+        for (int r = 0; r < blocks; ++r) {
+          least = min(least, sh.ends[0][r]);
+          most = max(most, sh.ends[1][r]);
+        }
+      }
+      bin = Bin{0, true, least, most};
+    }
+    const int shift = max(0, 64 - __clzll((long long)(bin.high - bin.low)) - 11);  // 2^11 bins
+    clear_bins();
+    tokens(bin.low, [&](unsigned long long number) {
+      if (in_bin(bin, number)) put((int)((bin.high - number) >> shift), logit_of(number), masses);
+    });
+    unsigned long long left = target - found.before;
+    cross(wide, masses, 0.0, left);
+    const unsigned long long before = found.before + sh.found.before;
+    found = sh.found;
+    found.before = before;
+    bin.high -= (unsigned long long)found.bin << shift;
+    bin.low = max(bin.low, bin.high - ((1ull << shift) - 1));
+  };
+
+  // The lowest token of the shortest prefix of those at or above `cut` that holds `target` tokens, or that mass, or (target 0)
+  // `share` of their mass; `cut` if there are not so many.  First among the listed ones, by the first block alone:
+  const auto shorten_list = [&](unsigned long long cut, bool masses, double share, unsigned long long target) {
+    clear_bins();
+    listed_tokens(cut, [&](unsigned long long number) { put(first_bin(weight, logit_of(number)), logit_of(number), masses); });
+    if (cross(Block(), masses, share, target) < target) return cut;
+    Found found = sh.found;
+    Bin bin{found.bin, false, cut, ~0ull};
+    while (found.count > LIST) divide(Block(), listed_tokens, bin, found, masses, target);
+    // rank the bin's tokens against one another
+    listed_tokens(bin.low, [&](unsigned long long number) {
+      if (!in_bin(bin, number)) return;
+      const uint32_t at = atomicAdd(&sh.bin_listed, 1u);
+      sh.bin_list[at] = number;
+      sh.bin_mass[at] = masses ? weight.fixed(logit_of(number)) : 1u;
+    });
+    __syncthreads();
+    constexpr int PARTS = THREADS / LIST;
+    const int mine = tid / PARTS;
+    const unsigned long long me = mine < (int)found.count ? sh.bin_list[mine] : ~0ull;
+    unsigned long long ahead = 0;
+    for (int j = tid % PARTS; j < (int)found.count; j += PARTS)
+      if (sh.bin_list[j] > me) ahead += sh.bin_mass[j];
+    for (int o = PARTS / 2; o > 0; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+    const unsigned long long last = block_reduce(found.before + ahead < target ? me : ~0ull, sh.scan, smaller);
+    if (tid == 0) sh.bin_listed = 0u;
+    __syncthreads();
+    return last;
+  };
+  // then among all: the cluster finds the bin, and sends its tokens to the first block.
+  const auto shorten_row = [&](unsigned long long cut, bool masses, double share, unsigned long long target) {
+    if (tid == 0) sh.listed = 0u;
+    clear_bins();
+    all_tokens(cut, [&](unsigned long long number) { put(first_bin(weight, logit_of(number)), logit_of(number), masses); });
+    if (cross(Cluster(), masses, share, target) < target) return cut;
+    Found found = sh.found;
+    Bin bin{found.bin, false, cut, ~0ull};
+    while (found.count > MEDIUM) divide(Cluster(), all_tokens, bin, found, masses, target);
+    gather([&](const auto& f) {
+      all_tokens(bin.low, [&](unsigned long long number) {
+        if (in_bin(bin, number)) f(number);
+      });
+    });
+    cluster.sync();
+    if (rank == 0) {
+      const unsigned long long last = shorten_list(0ull, masses, 0.0, target - found.before);
+      if (tid < blocks) *peer(&sh.cut, tid) = last;
+    }
+    cluster.sync();
+    return sh.cut;
+  };
 
   Sum total;
   // ---- a short prefix: the tokens that reach the threshold, ranked by the first block
@@ -712,68 +755,106 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   }
 
   // ---- a longer one, or all tokens
-  const auto cut_both = [&](auto wide, const auto& tokens, unsigned long long limit) {
-    unsigned long long cut = 1ull << 32;  // all but -inf
-    if (by_count) cut = shorten(wide, tokens, cut, false, 0.0, top_k);
-    if (by_mass) cut = shorten(wide, tokens, cut, true, top_p, by_count ? 0 : limit);
-    return cut;
-  };
-  // The race among the tokens at or above `cut`: (score, lowest index) of the block's best as one ordered number.
-  const auto race = [&](const auto& tokens, unsigned long long cut) {
-    float best_score = -1.f;
-    uint32_t winner = 0xffffffffu;
-    tokens(cut, [&](unsigned long long number) {
-      const float l = logit_of(number), w = weight(l);
-      const uint32_t token = 0xffffffffu - (uint32_t)number;
-      if (l != weight.best && (greedy || !(w >= min_p))) return;
-      const float score = greedy ? 1.f : fmaxf(__fdividef(w, noise[token]), -0.5f);
-      if (score > best_score || (score == best_score && token < winner)) {
-        best_score = score;
-        winner = token;
-      }
-    });
-    return block_reduce(((unsigned long long)key_of(best_score) << 32) | (0xffffffffu - winner), sh.scan, better);
-  };
   double whole = 0.0;
   for (int r = 0; r < blocks; ++r) whole += sh.totals[r];
   const unsigned long long limit = max(1ull, (unsigned long long)ceil((double)top_p * whole * 2147483648.0));
+  float best_score = -1.f;
+  uint32_t winner = 0xffffffffu;
+  const auto enter = [&](float l, float luck, uint32_t token) {  // a token into the race
+    const float w = weight(l);
+    if (l != weight.best && (greedy || !(w >= min_p))) return;
+    const float score = greedy ? 1.f : fmaxf(__fdividef(w, luck), -0.5f);
+    if (score > best_score || (score == best_score && token < winner)) {
+      best_score = score;
+      winner = token;
+    }
+  };
+  const auto best_of_block = [&] {  // (score, lowest index) as one ordered number
+    return block_reduce(((unsigned long long)key_of(best_score) << 32) | (0xffffffffu - winner), sh.scan, better);
+  };
   const auto finish = [&](unsigned long long first) {
     if (tid != 0) return;
     const int token = (int)(0xffffffffu - (uint32_t)first);
     a.token[row] = token;
     a.logprob[row] = (weight.exponent(Piece<T>::one(logits[token])) - __log2f((float)whole)) * LN2;
   };
+  unsigned long long cut = 1ull << 32;  // all but -inf
   if (by_count || by_mass) {
     if (tid == 0) sh.listed = 0u;
     cluster.sync();
-    const unsigned long long least = (unsigned long long)max(lower, 1u) << 32;
-    uint32_t sent = 0;
     unsigned long long sent_mass = 0;
-    all_tokens(least, [&](unsigned long long number) {
-      const uint32_t at = atomicAdd(peer(&sh.listed, 0), 1u);
-      if (at < MEDIUM) *peer(&sh.list[at], 0) = number;
-      ++sent;
-      sent_mass += weight.fixed(logit_of(number));
+    const uint32_t sent = gather([&](const auto& f) {
+      all_tokens((unsigned long long)max(lower, 1u) << 32, [&](unsigned long long number) {
+        f(number);
+        sent_mass += weight.fixed(logit_of(number));
+      });
     });
-    const auto add = [](unsigned long long x, unsigned long long y) { return x + y; };
-    sent_mass = block_reduce(sent_mass, sh.scan, add);
-    const unsigned long long sent_all = block_reduce((unsigned long long)sent, sh.scan, add);
+    sent_mass = block_reduce(sent_mass, sh.scan, [](unsigned long long x, unsigned long long y) { return x + y; });
     if (tid < blocks) {
       *peer(&sh.masses[rank], tid) = sent_mass;
-      *peer(&sh.slice[rank], tid) = sent_all;
+      *peer(&sh.counts[rank], tid) = sent;
     }
     cluster.sync();
-    unsigned long long held_mass = 0, n = 0;
+    unsigned long long held_mass = 0;
+    uint32_t n = 0;
     for (int r = 0; r < blocks; ++r) {
       held_mass += sh.masses[r];
-      n += sh.slice[r];
+      n += sh.counts[r];
     }
-    if (n <= MEDIUM && (by_count ? n >= (unsigned long long)top_k : held_mass >= limit)) {
-      if (rank == 0) finish(race(listed_tokens, cut_both(Block(), listed_tokens, limit)));
+    if (n <= MEDIUM && (by_count ? n >= (uint32_t)top_k : held_mass >= limit)) {
+      if (rank != 0) return;
+      if (by_count) cut = shorten_list(cut, false, 0.0, top_k);
+      if (by_mass) cut = shorten_list(cut, true, top_p, by_count ? 0 : limit);
+      listed_tokens(cut, [&](unsigned long long number) {
+        const uint32_t token = 0xffffffffu - (uint32_t)number;
+        enter(logit_of(number), noise[token], token);
+      });
+      finish(best_of_block());
       return;
     }
+    if (by_count) cut = shorten_row(cut, false, 0.0, top_k);
+    if (by_mass) cut = shorten_row(cut, true, top_p, by_count ? 0 : limit);
   }
-  const unsigned long long first = race(all_tokens, cut_both(Cluster(), all_tokens, limit));
+  if (own_top >= (uint32_t)(cut >> 32)) {
+    // pieces with a token that stays; the random numbers of several are under way together
+    constexpr int DEPTH = E == 4 ? 4 : 2;
+    const bool together = (reinterpret_cast<uintptr_t>(noise - skew) % 16) == 0;
+    for (int i0 = tid; i0 < count; i0 += DEPTH * THREADS) {
+      float luck[DEPTH][E];
+      bool any[DEPTH];
+#pragma unroll
+      for (int j = 0; j < DEPTH; ++j) {
+        const int i = i0 + j * THREADS, first = (from + i) * E - skew;
+        any[j] = false;
+        if (i < count) {
+          const Piece<T> p(held[i]);
+#pragma unroll
+          for (int e = 0; e < E; ++e) any[j] |= rank_of(p.v[e], first + e) >= cut;
+        }
+        if (!any[j]) continue;
+        if (together && inside(i)) {
+#pragma unroll
+          for (int x = 0; x < E / 4; ++x) {
+            const float4 v = *(reinterpret_cast<const float4*>(noise + first) + x);
+            luck[j][4 * x] = v.x, luck[j][4 * x + 1] = v.y, luck[j][4 * x + 2] = v.z, luck[j][4 * x + 3] = v.w;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) luck[j][e] = first + e >= 0 && first + e < a.V ? noise[first + e] : 1.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < DEPTH; ++j) {
+        if (!any[j]) continue;
+        const int i = i0 + j * THREADS, first = (from + i) * E - skew;
+        const Piece<T> p(held[i]);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (rank_of(p.v[e], first + e) >= cut) enter(p.v[e], luck[j][e], (uint32_t)(first + e));
+      }
+    }
+  }
+  const unsigned long long first = best_of_block();
   if (tid == 0) *peer(&sh.slice[rank], 0) = first;
   cluster.sync();
   if (rank == 0) {
