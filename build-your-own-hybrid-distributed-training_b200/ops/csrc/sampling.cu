@@ -51,8 +51,8 @@ __device__ __forceinline__ uint32_t key_of(float l) {
   const uint32_t u = __float_as_uint(l + 0.f);  // -0 + 0 = +0: equal logits have equal keys
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float value_of(uint32_t key) {
-  return key == 0u ? -INFINITY : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+__device__ __forceinline__ float value_of(uint32_t key) {  // keys below that of the lowest number stand for -inf
+  return key <= 0x007fffffu ? -INFINITY : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -438,7 +438,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
 
   // Who looks for a cut: the cluster, among all tokens, or the first block, among those of its list.
   const auto all_tokens = [&](unsigned long long least, auto f) {
+    const float lowest = value_of((uint32_t)(least >> 32));
     visit((uint32_t)(least >> 32), [&](float l, int token) {
+      if (!(l >= lowest)) return;
       const unsigned long long number = rank_of(l, token);
       if (number >= least) f(number);
     });
@@ -553,9 +555,17 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     int first;
     bool divided;
     unsigned long long low, high;
+    float lowest, highest;  // logits that an undivided bin lies between, a bin's width to spare on either side
+  };
+  const auto bin_at = [&](int first, unsigned long long low) {
+    const float width = 1.f / (64.f * LN2 * weight.hi);  // of a bin; not a number where a single logit weighs anything
+    return Bin{first, false, low, ~0ull, first == BINS - 1 ? -INFINITY : weight.best - (first + 2) * width, weight.best - (first - 1) * width};
   };
   const auto in_bin = [&](const Bin& bin, unsigned long long number) {
-    return bin.divided ? number <= bin.high : first_bin(weight, logit_of(number)) == bin.first;
+    if (bin.divided) return number <= bin.high;
+    const float l = logit_of(number);
+    if (l < bin.lowest || l > bin.highest) return false;
+    return first_bin(weight, l) == bin.first;
   };
   // A histogram over the bin's tokens, by their numbers' bits; `bin` becomes the one of its 2048 parts that holds the target.
   const auto divide = [&](auto wide, const auto& tokens, Bin& bin, Found& found, bool masses, unsigned long long target) {
@@ -580,7 +590,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
           most = max(most, sh.ends[1][r]);
         }
       }
-      bin = Bin{0, true, least, most};
+      bin.divided = true;
+      bin.low = least;
+      bin.high = most;
     }
     const int shift = max(0, 64 - __clzll((long long)(bin.high - bin.low)) - 11);  // 2^11 bins
     clear_bins();
@@ -603,7 +615,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     listed_tokens(cut, [&](unsigned long long number) { put(first_bin(weight, logit_of(number)), logit_of(number), masses); });
     if (cross(Block(), masses, share, target) < target) return cut;
     Found found = sh.found;
-    Bin bin{found.bin, false, cut, ~0ull};
+    Bin bin = bin_at(found.bin, cut);
     while (found.count > LIST) divide(Block(), listed_tokens, bin, found, masses, target);
     // rank the bin's tokens against one another
     listed_tokens(bin.low, [&](unsigned long long number) {
@@ -632,7 +644,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     all_tokens(cut, [&](unsigned long long number) { put(first_bin(weight, logit_of(number)), logit_of(number), masses); });
     if (cross(Cluster(), masses, share, target) < target) return cut;
     Found found = sh.found;
-    Bin bin{found.bin, false, cut, ~0ull};
+    Bin bin = bin_at(found.bin, cut);
     while (found.count > MEDIUM) divide(Cluster(), all_tokens, bin, found, masses, target);
     gather([&](const auto& f) {
       all_tokens(bin.low, [&](unsigned long long number) {
@@ -657,7 +669,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     unsigned long long sent_mass = 0;
     visit(0u, [&](float l, int token) {
       total.add(weight(l));
-      if (l >= least) {
+      if (l >= least && l > -INFINITY) {
         const uint32_t at = atomicAdd(peer(&sh.listed, 0), 1u), mass = weight.fixed(l);
         if (at < SHORT) {
           *peer(&sh.list[at], 0) = rank_of(l, token);
