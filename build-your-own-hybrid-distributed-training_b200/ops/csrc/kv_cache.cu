@@ -22,6 +22,19 @@ namespace kv {
 
 constexpr int THREADS = 256;
 
+// Division of row numbers (below 2^31) by the number of heads: the high half of a product, shifted.
+struct Divider {
+  uint32_t by, factor;
+  int shift;  // -1: by one
+  explicit Divider(int d) : by((uint32_t)d) {
+    int log = 0;
+    while ((1ll << log) < d) ++log;
+    shift = log - 1;
+    factor = (uint32_t)((1ull << (31 + log)) / (unsigned)d + 1);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t r) const { return shift < 0 ? r : __umulhi(r, factor) >> shift; }
+};
+
 __device__ __forceinline__ long long slot_of(const void* slots, int wide, int t) {
   return wide ? static_cast<const long long*>(slots)[t] : (long long)static_cast<const int*>(slots)[t];
 }
@@ -70,7 +83,7 @@ __device__ __forceinline__ float4 values_of(uint32_t w) {
 }
 
 template <int F, int D>
-__global__ void __launch_bounds__(THREADS) write_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(THREADS) write_kernel(const __grid_constant__ WriteArgs a, const Divider heads) {
   constexpr int LANES = D / 8, PER_BLOCK = THREADS / LANES;
   const int rows = (int)a.T * a.pool.Hkv, lane = threadIdx.x % LANES;
   // every lane of a warp makes the same number of turns, so the shuffles below always see a full warp
@@ -79,34 +92,45 @@ __global__ void __launch_bounds__(THREADS) write_kernel(const WriteArgs a) {
     uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
     long long at = -1;
     if (r < rows) {
-      const int t = r / a.pool.Hkv, h = r - t * a.pool.Hkv;
+      const int t = (int)heads((uint32_t)r), h = r - t * a.pool.Hkv;
       raw[0] = __ldcs(reinterpret_cast<const uint4*>(a.src[0] + t * a.tok[0] + h * a.head[0] + lane * 8));
       raw[1] = __ldcs(reinterpret_cast<const uint4*>(a.src[1] + t * a.tok[1] + h * a.head[1] + lane * 8));
       at = pool_row(a.pool, slot_of(a.slots, a.wide, t), h);
     }
+    if constexpr (F == kBf16) {
+      if (at >= 0) {
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.pool.k) + at * D + lane * 8) = raw[0];
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.pool.v) + at * D + lane * 8) = raw[1];
+      }
+    } else {
+      // The rows' largest magnitudes as 16 bits each (NaN > infinity > every finite value), the key's and the value's side by
+      // side through one reduction.
+      uint32_t top[2];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      void* const pool = which ? a.pool.v : a.pool.k;
-      if constexpr (F == kBf16) {
-        if (at >= 0) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(pool) + at * D + lane * 8) = raw[which];
-      } else {
+      for (int which = 0; which < 2; ++which) {
+        const uint32_t m = 0x7fff7fffu;
+        top[which] = __vmaxu2(__vmaxu2(raw[which].x & m, raw[which].y & m), __vmaxu2(raw[which].z & m, raw[which].w & m));
+      }
+      uint32_t both = __vmaxu2(__byte_perm(top[0], top[1], 0x5410), __byte_perm(top[0], top[1], 0x7632));
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const float largest = __uint_as_float(which ? both & 0xffff0000u : both << 16);
+        const bool finite = largest < INFINITY;
+        const float scale =
+            finite ? fmaxf(__fmul_rn(largest, F == kInt8 ? 1.0f / 127.0f : 1.0f / 448.0f), kMinScale) : __int_as_float(0x7fc00000);
         const uint32_t u[4] = {raw[which].x, raw[which].y, raw[which].z, raw[which].w};
         float x[8];
-        uint32_t top = 0;  // the largest magnitude as bits: NaN > infinity > every finite value
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           x[2 * j] = __uint_as_float(u[j] << 16);
           x[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-          top = max(top, max((u[j] << 16) & 0x7fffffffu, u[j] & 0x7fff0000u));
         }
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const bool finite = top < 0x7f800000u;
-        const float scale = finite ? fmaxf(__fmul_rn(__uint_as_float(top), F == kInt8 ? 1.0f / 127.0f : 1.0f / 448.0f), kMinScale)
-                                   : __int_as_float(0x7fc00000);
-        const uint2 q = finite ? quantise8<F>(x, __frcp_rn(scale)) : make_uint2(0, 0);
+        uint2 q = quantise8<F>(x, __frcp_rn(scale));
+        if (!finite) q = make_uint2(0, 0);
         if (at >= 0) {
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + at * D + lane * 8) = q;
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(which ? a.pool.v : a.pool.k) + at * D + lane * 8) = q;
           if (lane == 0) (which ? a.pool.v_scale : a.pool.k_scale)[at] = scale;
         }
       }
@@ -115,11 +139,11 @@ __global__ void __launch_bounds__(THREADS) write_kernel(const WriteArgs a) {
 }
 
 template <int F, int D>
-__global__ void __launch_bounds__(THREADS) read_kernel(const ReadArgs a) {
+__global__ void __launch_bounds__(THREADS) read_kernel(const __grid_constant__ ReadArgs a, const Divider heads) {
   constexpr int LANES = D / 8, PER_BLOCK = THREADS / LANES;
   const int rows = (int)a.T * a.pool.Hkv, lane = threadIdx.x % LANES;
   for (int r = blockIdx.x * PER_BLOCK + threadIdx.x / LANES; r < rows; r += gridDim.x * PER_BLOCK) {
-    const int t = r / a.pool.Hkv, h = r - t * a.pool.Hkv;
+    const int t = (int)heads((uint32_t)r), h = r - t * a.pool.Hkv;
     const long long at = pool_row(a.pool, slot_of(a.slots, a.wide, t), h);
     uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
     float scale[2] = {0.f, 0.f};
@@ -164,13 +188,13 @@ static unsigned row_blocks(long long rows, int D, int sms) {
 
 cudaError_t launch_write(const WriteArgs& a, int sms, cudaStream_t stream) {
   const unsigned blocks = row_blocks(a.T * a.pool.Hkv, a.pool.D, sms);
-  by_format(a.pool, [&](auto f, auto d) { write_kernel<decltype(f)::value, decltype(d)::value><<<blocks, THREADS, 0, stream>>>(a); });
+  by_format(a.pool, [&](auto f, auto d) { write_kernel<decltype(f)::value, decltype(d)::value><<<blocks, THREADS, 0, stream>>>(a, Divider(a.pool.Hkv)); });
   return cudaGetLastError();
 }
 
 cudaError_t launch_read(const ReadArgs& a, int sms, cudaStream_t stream) {
   const unsigned blocks = row_blocks(a.T * a.pool.Hkv, a.pool.D, sms);
-  by_format(a.pool, [&](auto f, auto d) { read_kernel<decltype(f)::value, decltype(d)::value><<<blocks, THREADS, 0, stream>>>(a); });
+  by_format(a.pool, [&](auto f, auto d) { read_kernel<decltype(f)::value, decltype(d)::value><<<blocks, THREADS, 0, stream>>>(a, Divider(a.pool.Hkv)); });
   return cudaGetLastError();
 }
 
