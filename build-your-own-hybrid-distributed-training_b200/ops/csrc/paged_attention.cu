@@ -215,6 +215,13 @@ __device__ __forceinline__ unsigned arrive(unsigned* counter) {
   return before;
 }
 
+// Of this block's shared memory, or of what other blocks wrote before they arrived.
+__device__ __forceinline__ float load(const float* p) {
+  float v;
+  asm volatile("ld.relaxed.gpu.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
+
 template <int F, int D>
 __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const __grid_constant__ Args a) {
   using S = Shape<F, D>;
@@ -224,19 +231,17 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
     int item;  // first tile of the row on the line
     int b, row, tile, count, tiles;
   };
-  struct Group {
-    Meta first;
-    int end_tile, from, to;  // pieces [from, to) of the list of all
-    bool whole;
+  struct Job {      // pieces of one row to bring together
+    int from, to;   // of the list of pieces
+    int b, row;
+    int item, tiles;
+    bool begins, whole;  // whether they start with the row's first token, and whether they are all of the row
   };
   struct Shared {
     Meta meta[2 * WARPS];
-    Group groups[WARPS + 1];
+    Job jobs[WARPS + 1];
     int count;
-    uint32_t have;
-    float weight[2 * WARPS][HEADS];
     bool shared_rows;  // whether a row of this block goes on in another one
-    int join_first[2], join_count[2], join_b[2], join_row[2];
   };
   static_assert(sizeof(Shared) <= WARPS * S::BOOK, "shared bookkeeping");
   unsigned char* const rings = smem;
@@ -757,191 +762,109 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
   }
   __syncthreads();
 
-  // ---- pieces of the same row are neighbours: merge them
+  // ---- bring pieces of the same row together: first those of this block, which are neighbours, and then, if this block is the
+  // last to arrive, those that other blocks left of its first and its last row.  One loop does both: the code of the
+  // end of a block is fetched from afar, so that its length costs more than its steps.
+  static_assert(2 * WARPS <= 32, "a lane per piece");
   constexpr int STEP = HEADS * (D + 2);  // floats of a piece
-  const auto piece_of = [&](int i) {
-    return reinterpret_cast<float*>(i % 2 == 0 ? pieces + i / 2 * S::PIECE : rings + i / 2 * S::STAGES * S::STAGE);
-  };
+  const float** const list = reinterpret_cast<const float**>(rings + S::PIECE);  // behind the first warp's piece
   if (warp == 0) {
-    const bool some = lane < 2 * WARPS && sh.meta[lane].count > 0;
-    const int item = some ? sh.meta[lane].item : -1;
+    const Meta mine = sh.meta[lane < 2 * WARPS ? lane : 0];
+    const bool some = lane < 2 * WARPS && mine.count > 0;
     const uint32_t have = __ballot_sync(0xffffffffu, some), before = have & ((1u << lane) - 1);
-    const int previous = __shfl_sync(0xffffffffu, item, before ? 31 - __clz(before) : 0);
-    const bool head = some && (before == 0 || previous != item);
-    const uint32_t heads = __ballot_sync(0xffffffffu, head);
-    if (head) {
-      const uint32_t later = heads & ~((2u << lane) - 1);
-      const int to = later ? __ffs(later) - 1 : 2 * WARPS;
-      const int last = 31 - __clz(have & (to == 32 ? 0xffffffffu : (1u << to) - 1));
-      Group& group = sh.groups[__popc(heads & ((1u << lane) - 1))];
-      group.first = sh.meta[lane];
-      group.end_tile = sh.meta[last].tile + sh.meta[last].count;
-      group.from = lane;
-      group.to = last + 1;
-      group.whole = group.first.tile == 0 && group.end_tile == group.first.tiles;
-    }
+    const int previous = __shfl_sync(0xffffffffu, mine.item, before ? 31 - __clz(before) : 0);
+    const bool head = some && (before == 0 || previous != mine.item);
+    const uint32_t heads = __ballot_sync(0xffffffffu, head), later = heads & ~((2u << lane) - 1);
+    const uint32_t members = have & ~((1u << lane) - 1) & (later ? (1u << (__ffs(later) - 1)) - 1 : 0xffffffffu);
+    const int last = members ? 31 - __clz(members) : lane;
+    const int end = __shfl_sync(0xffffffffu, mine.tile + mine.count, last);
+    const bool whole = mine.tile == 0 && end == mine.tiles;
+    if (some) list[__popc(before)] = reinterpret_cast<const float*>(lane % 2 == 0 ? pieces + lane / 2 * S::PIECE : rings + lane / 2 * S::STAGES * S::STAGE);
+    if (head)
+      sh.jobs[__popc(heads & ((1u << lane) - 1))] =
+          Job{__popc(before), __popc(before) + __popc(members), mine.b, mine.row, mine.item, mine.tiles, mine.tile == 0, whole};
+    const bool shared_rows = __any_sync(0xffffffffu, head && !whole);
     if (lane == 0) {
       sh.count = __popc(heads);
-      sh.have = have;
-      sh.join_count[0] = sh.join_count[1] = 0;
+      sh.shared_rows = shared_rows;
     }
-    const bool whole = !head || sh.groups[__popc(heads & ((1u << lane) - 1))].whole;
-    if (lane == 0) sh.shared_rows = false;
-    __syncwarp();
-    if (!whole) sh.shared_rows = true;
   }
   __syncthreads();
-  const int real_heads = min(group, HEADS);
-  // The results of a row's head h, and whether the group has that head.
-  const auto head_of = [&](int b, int row, int h, long long& head) {
-    const int kv_head = chunks == 1 ? row : row / chunks, in_group = (row - kv_head * chunks) * HEADS + h;
-    head = (long long)b * a.H + (long long)kv_head * group + in_group;
-    return in_group < group;
-  };
-  // Dimension of accumulator place (v = 2 t + e, lane).
-  const auto dim_of = [&](int v, int lane_) {
-    return F == kv::kBf16 ? (v >> 1) * 8 + 2 * (lane_ & 3) + (v & 1) : (2 * (lane_ & 3) + (v & 1)) * NT + (v >> 1);
-  };
-  float* const merged = a.partial + (long long)blockIdx.x * 2 * STEP;
-  // weights of the pieces: a warp per head, a lane per piece
-  static_assert(2 * WARPS <= 32 && WARPS >= HEADS, "one lane per piece, one warp per head");
-  if (warp < real_heads) {
-    const uint32_t have = sh.have;
-    const bool some = (have >> lane) & 1u;
-    const float* p = piece_of(some ? lane : 0);
-    const float mine = some ? p[HEADS * D + warp] : -INFINITY, part = some ? p[HEADS * D + HEADS + warp] : 0.f;
-    int gi = 0;
-    while (some && lane >= sh.groups[gi].to) ++gi;
-    const Group& grp = sh.groups[gi];
-    const uint32_t members = some ? have & (0xffffffffu << grp.from) & (0xffffffffu >> (32 - grp.to)) : 0u;
-    float top = -INFINITY, total = 0.f;
+  for (bool joining = false;; joining = true) {
+    constexpr int VALUES = 4, UNITS = 2 * NT / VALUES;  // a warp takes this many values a lane, of one row, at a time
+    for (int unit = warp; unit < sh.count * UNITS; unit += WARPS) {
+      const Job job = sh.jobs[unit / UNITS];
+      const int v0 = unit % UNITS * VALUES;
+      float top = -INFINITY, total = 0.f, x[VALUES] = {};
+      for (int i = job.from; i < job.to; i += 2) {
+        const float *p = list[i], *q2 = list[min(i + 1, job.to - 1)];
+        const float m0 = load(p + HEADS * D + g), l0 = load(p + HEADS * D + HEADS + g);
+        float m1 = load(q2 + HEADS * D + g);
+        const float l1 = load(q2 + HEADS * D + HEADS + g);
+        float y0[VALUES], y1[VALUES];
 #pragma unroll
-    for (int i = 0; i < 2 * WARPS; ++i) {
-      const float other = __shfl_sync(0xffffffffu, mine, i);
-      if ((members >> i) & 1u) top = fmaxf(top, other);
-    }
-    const float at = top == -INFINITY ? 0.f : top, w = fast_exp2(mine - at);
-    const float weighted = w * part;
+        for (int y = 0; y < VALUES; ++y) {
+          y0[y] = load(p + (v0 + y) * 32 + lane);
+          y1[y] = load(q2 + (v0 + y) * 32 + lane);
+        }
+        if (i + 1 == job.to) m1 = -INFINITY;
+        const float higher = fmaxf(top, fmaxf(m0, m1)), at = higher == -INFINITY ? 0.f : higher;
+        const float keep = fast_exp2(top - at), w0 = fast_exp2(m0 - at), w1 = fast_exp2(m1 - at);
+        top = higher;
+        total = fmaf(w1, l1, fmaf(w0, l0, total * keep));
 #pragma unroll
-    for (int i = 0; i < 2 * WARPS; ++i) {
-      const float other = __shfl_sync(0xffffffffu, weighted, i);
-      if ((members >> i) & 1u) total += other;
-    }
-    if (some) {
-      sh.weight[lane][warp] = w * (!grp.whole ? 1.f : total == 0.f ? 0.f : __fdividef(1.f, total));
-      long long head;
-      if (lane == grp.from && head_of(grp.first.b, grp.first.row, warp, head)) {
-        if (!grp.whole) {
-          float* const out = merged + (grp.first.tile > 0 ? 0 : STEP);
-          out[HEADS * D + warp] = top;
-          out[HEADS * D + HEADS + warp] = total;
-        } else if (a.lse != nullptr) {
-          a.lse[head] = total == 0.f ? -INFINITY : (top + fast_log2(total)) * LN2;
+        for (int y = 0; y < VALUES; ++y) x[y] = fmaf(w1, y1[y], fmaf(w0, y0[y], x[y] * keep));
+      }
+      const int kv_head = chunks == 1 ? job.row : job.row / chunks, in_group = (job.row - kv_head * chunks) * HEADS + g;
+      if (in_group >= group) continue;
+      if (job.whole) {
+        const long long head = (long long)job.b * a.H + (long long)kv_head * group + in_group;
+        const float norm = total == 0.f ? 0.f : __fdividef(1.f, total);
+#pragma unroll
+        for (int y = 0; y < VALUES; ++y) {
+          const int v = v0 + y, d = F == kv::kBf16 ? (v >> 1) * 8 + 2 * c4 + (v & 1) : (2 * c4 + (v & 1)) * NT + (v >> 1);
+          a.out[head * D + d] = __float2bfloat16_rn(x[y] * norm);
+        }
+        if (a.lse != nullptr && v0 == 0 && c4 == 0) a.lse[head] = total == 0.f ? -INFINITY : (top + fast_log2(total)) * LN2;
+      } else {
+        float* const out = a.partial + ((long long)blockIdx.x * 2 + (job.begins ? 1 : 0)) * STEP;
+#pragma unroll
+        for (int y = 0; y < VALUES; ++y) out[(v0 + y) * 32 + lane] = x[y];
+        if (v0 == 0 && c4 == 0) {
+          out[HEADS * D + g] = top;
+          out[HEADS * D + HEADS + g] = total;
         }
       }
     }
-  }
-  __syncthreads();
-  // values: a warp takes VALUES per lane of one group at a time
-  constexpr int VALUES = 4, UNITS = 2 * NT / VALUES;
-  for (int unit = warp; unit < sh.count * UNITS; unit += WARPS) {
-    const Group& grp = sh.groups[unit / UNITS];
-    const int v0 = unit % UNITS * VALUES;
-    float x[VALUES] = {};
-    for (uint32_t m = sh.have & (0xffffffffu << grp.from) & (0xffffffffu >> (32 - grp.to)); m != 0; m &= m - 1) {
-      const int piece = __ffs(m) - 1;
-      const float w = sh.weight[piece][g];
-      const float* p = piece_of(piece) + v0 * 32 + lane;
-#pragma unroll
-      for (int y = 0; y < VALUES; ++y) x[y] = fmaf(w, p[y * 32], x[y]);
-    }
-    long long head;
-    if (!head_of(grp.first.b, grp.first.row, g, head)) continue;
-    if (grp.whole) {
-#pragma unroll
-      for (int y = 0; y < VALUES; ++y) a.out[head * D + dim_of(v0 + y, lane)] = __float2bfloat16_rn(x[y]);
-    } else {
-      float* const out = merged + (grp.first.tile > 0 ? 0 : STEP) + v0 * 32 + lane;
-#pragma unroll
-      for (int y = 0; y < VALUES; ++y) out[y * 32] = x[y];
-    }
-  }
-
-  // ---- rows that cross blocks: the last block to arrive joins them.  A row that goes on behind its first block is that
-  // block's last one, so the block's number names the counter.
-  if (!sh.shared_rows) return;
-  __syncthreads();
-  if (tid == 0) {
-    int joins = 0;
-    for (int gi = 0; gi < sh.count; gi += max(1, sh.count - 1)) {
-      const Group& grp = sh.groups[gi];
-      if (grp.whole) continue;
-      const int b0 = grp.first.item / per_block, b1 = (grp.first.item + grp.first.tiles - 1) / per_block;
-      if (arrive(a.arrived + b0) == (unsigned)(b1 - b0)) {
-        a.arrived[b0] = 0;
-        sh.join_first[joins] = b0;
-        sh.join_count[joins] = b1 - b0 + 1;
-        sh.join_b[joins] = grp.first.b;
-        sh.join_row[joins++] = grp.first.row;
+    if (joining || !sh.shared_rows) return;
+    __syncthreads();
+    // A row that goes on behind its first block is that block's last one, so the block's number names the row's counter.
+    if (warp == 0) {
+      const Job job = sh.jobs[lane == 0 ? 0 : sh.count - 1];
+      int first = 0, n = 0;
+      bool won = false;
+      if (lane < min(2, sh.count) && !job.whole) {
+        first = job.item / per_block;
+        n = (job.item + job.tiles - 1) / per_block - first + 1;
+        won = arrive(a.arrived + first) == (unsigned)(n - 1);
+        if (won) a.arrived[first] = 0;
       }
-    }
-  }
-  __syncthreads();
-  for (int join = 0; join < 2; ++join) {
-    const int n = sh.join_count[join];
-    if (n == 0) break;
-    // the first block's piece is its second, the others' their first
-    const auto part = [&](int j) { return a.partial + ((long long)(sh.join_first[join] + j) * 2 + (j == 0 ? 1 : 0)) * STEP; };
-    float* const weights = reinterpret_cast<float*>(rings);  // [n][HEADS], then the heads' norms, then the copies' sums
-    float* const norms = weights + n * HEADS;
-    float* const sums = norms + HEADS;
-    // a thread takes 4 neighbouring places (of one head); the threads left over take further parts of the list
-    const int quads = 2 * NT * real_heads, copies = S::THREADS / quads;
-    const int quad = tid % quads, copy = tid / quads;
-    const int place = quad / real_heads * 32 + quad % real_heads * 4;
-    float4 ahead = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (copy < copies && copy < n) ahead = __ldcg(reinterpret_cast<const float4*>(part(copy) + place));
-    if (warp < real_heads) {  // one warp per head
-      float top = -INFINITY, total = 0.f;
-      for (int j = lane; j < n; j += 32) {
-        const float m = __ldcg(part(j) + HEADS * D + warp), l = __ldcg(part(j) + HEADS * D + HEADS + warp);
-        const float higher = fmaxf(top, m), at = higher == -INFINITY ? 0.f : higher;
-        weights[j * HEADS + warp] = m;
-        total = total * fast_exp2(top - at) + l * fast_exp2(m - at);
-        top = higher;
-      }
-      const float mine = top;
-      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const float at = top == -INFINITY ? 0.f : top;
-      total *= fast_exp2(mine - at);
-      for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
-      for (int j = lane; j < n; j += 32) weights[j * HEADS + warp] = fast_exp2(weights[j * HEADS + warp] - at);
+      const uint32_t wins = __ballot_sync(0xffffffffu, won);
+      if (won) sh.jobs[lane == 1 && (wins & 1u) ? 1 : 0] = Job{0, n, job.b, job.row, first, n, true, true};
+      __syncwarp();
       if (lane == 0) {
-        norms[warp] = total == 0.f ? 0.f : __fdividef(1.f, total);
-        long long head;
-        if (head_of(sh.join_b[join], sh.join_row[join], warp, head) && a.lse != nullptr)
-          a.lse[head] = total == 0.f ? -INFINITY : (top + fast_log2(total)) * LN2;
+        sh.count = __popc(wins);
+        if (wins == 3u) {  // the second row's pieces lie behind the first's
+          sh.jobs[1].from = sh.jobs[0].to;
+          sh.jobs[1].to += sh.jobs[0].to;
+        }
       }
     }
     __syncthreads();
-    if (copy < copies) {
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int j = copy; j < n; j += copies) {
-        const float w = weights[j * HEADS + quad % real_heads];
-        const float4 v = j == copy ? ahead : __ldcg(reinterpret_cast<const float4*>(part(j) + place));
-        acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
-      }
-      reinterpret_cast<float4*>(sums)[copy * quads + quad] = acc;
-    }
-    __syncthreads();
-    for (int x = tid; x < quads * 4; x += S::THREADS) {
-      float value = 0.f;
-      for (int y = 0; y < copies; ++y) value += sums[y * quads * 4 + x];
-      const int v = x / (4 * real_heads), lane_ = x - v * 4 * real_heads;
-      long long head;
-      if (head_of(sh.join_b[join], sh.join_row[join], lane_ / 4, head))
-        a.out[head * D + dim_of(v, lane_)] = __float2bfloat16_rn(value * norms[lane_ / 4]);
+    for (int j = 0; j < sh.count; ++j) {
+      const Job job = sh.jobs[j];
+      // a row's first block left its piece in its second place, the others in their first
+      for (int x = tid; x < job.tiles; x += S::THREADS) list[job.from + x] = a.partial + ((long long)(job.item + x) * 2 + (x == 0 ? 1 : 0)) * STEP;
     }
     __syncthreads();
   }
