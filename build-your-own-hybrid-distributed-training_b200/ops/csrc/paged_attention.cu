@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
   const int group = a.H / a.pool.Hkv;               // query heads per key/value head
   const int chunks = (group + HEADS - 1) / HEADS;  // rows per key/value head
   const int rows = a.pool.Hkv * chunks;
+  const auto kv_head_of = [&](int row) { return chunks == 1 ? row : row / chunks; };
 
   // ---- this warp's range of the line.  Every warp works it out for itself: sums of the tiles of 32 sequences at a time, a
   // lane for each sum, then the 32 sequences among which the range starts.  Nobody waits for another warp.
@@ -265,45 +266,51 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
     }
     return v;
   };
-  const auto sums = [&](int b0, bool first) {  // of the 1024 sequences from b0 on
-    int mine = 0;
+  if (warp == 0) {  // sequences without tokens have no tiles: their results are written here
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      if (tokens_of(a, b) > 0) continue;
+      for (int i = lane * 8; i < a.H * D; i += 256) *reinterpret_cast<uint4*>(a.out + (long long)b * a.H * D + i) = make_uint4(0, 0, 0, 0);
+      if (a.lse != nullptr)
+        for (int i = lane; i < a.H; i += 32) a.lse[(long long)b * a.H + i] = -INFINITY;
+    }
+  }
+  int line = 0, base = 0, b0 = 0, mine, upto;
+  int per_block = 0, block_from = 0, from = 0, count = 0;
+  for (bool counted = false;;) {
+    mine = 0;  // lane k: the tiles of sequences b0 + 32 k ... + 31
 #pragma unroll 4
     for (int k = 0; k < 32; ++k) {
-      const int b = b0 + 32 * k + lane;
       if (b0 + 32 * k >= a.B) break;
-      const int n = b < a.B ? tokens_of(a, b) : 0;
-      if (first && warp == 0 && n == 0 && b < a.B && b % gridDim.x == blockIdx.x) {  // no tokens, hence no tiles: write the result here
-        for (int i = 0; i < a.H * D; i += 8) *reinterpret_cast<uint4*>(a.out + (long long)b * a.H * D + i) = make_uint4(0, 0, 0, 0);
-        if (a.lse != nullptr)
-          for (int i = 0; i < a.H; ++i) a.lse[(long long)b * a.H + i] = -INFINITY;
-      }
-      const int sum = (int)__reduce_add_sync(0xffffffffu, (uint32_t)tiles_of(n));
+      const int b = b0 + 32 * k + lane;
+      const int sum = (int)__reduce_add_sync(0xffffffffu, b < a.B ? (uint32_t)tiles_of(tokens_of(a, b)) : 0u);
       if (lane == k) mine = sum;
     }
-    return mine;
-  };
-  int mine = sums(0, true), upto = scan(mine);
-  int line = __shfl_sync(0xffffffffu, upto, 31);
-  for (int b0 = 1024; b0 < a.B; b0 += 1024) line += (int)__reduce_add_sync(0xffffffffu, (uint32_t)sums(b0, true));
-  // at least 8 tiles, a tile a warp: fewer, fuller blocks have fewer pieces to join, and rows of a power of two of tiles end with
-  // a block
-  const int per_block = max((int)((line + gridDim.x - 1) / gridDim.x), 8);
-  const int block_from = (int)min((long long)line, (long long)per_block * blockIdx.x);
-  const int block_to = min(line - block_from, per_block) + block_from;
-  if (block_from >= block_to) return;
-  const int per_warp = (block_to - block_from + WARPS - 1) / WARPS;
-  const int from = block_from + warp * per_warp;
-  const int count = max(0, min(per_warp, block_to - from));
+    upto = scan(mine);
+    const int total = __shfl_sync(0xffffffffu, upto, 31);
+    if (!counted) {
+      line += total;
+      b0 += 1024;
+      if (b0 < a.B) continue;
+      counted = true;
+      // at least 8 tiles, a tile a warp: fewer, fuller blocks have fewer pieces to join, and rows of a power of two of tiles end
+      // with a block
+      per_block = max((int)((line + gridDim.x - 1) / gridDim.x), 8);
+      block_from = (int)min((long long)line, (long long)per_block * blockIdx.x);
+      const int block_to = min(line - block_from, per_block) + block_from;
+      if (block_from >= block_to) return;
+      const int per_warp = (block_to - block_from + WARPS - 1) / WARPS;
+      from = block_from + warp * per_warp;
+      count = max(0, min(per_warp, block_to - from));
+      b0 = 0;
+      if (a.B > 1024) continue;  // again from the first 1024, which are no longer at hand
+    }
+    if (count == 0 || from < base + total) break;
+    base += total;
+    b0 += 1024;
+  }
   if (lane < 2) sh.meta[2 * warp + lane].count = 0;
   Cursor start{0, 0, 0, 1, 0};
   if (count > 0) {
-    int base = 0, b0 = 0;
-    while (from >= base + __shfl_sync(0xffffffffu, upto, 31)) {  // beyond these 1024 sequences
-      base += __shfl_sync(0xffffffffu, upto, 31);
-      b0 += 1024;
-      mine = sums(b0, false);
-      upto = scan(mine);
-    }
     const int chunk = __popc(__ballot_sync(0xffffffffu, base + upto <= from));
     base += __shfl_sync(0xffffffffu, upto - mine, chunk);
     b0 += 32 * chunk;
@@ -355,7 +362,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
           const bool in_pool = p >= 0 && p < a.pool.pages;
           bits |= (uint32_t)in_pool << i;
           const long long first =
-              in_pool ? (((long long)p * a.pool.Hkv + load.row / chunks) << a.pool.page_shift) + (token & ((1 << a.pool.page_shift) - 1)) : 0;
+              in_pool ? (((long long)p * a.pool.Hkv + kv_head_of(load.row)) << a.pool.page_shift) + (token & ((1 << a.pool.page_shift) - 1)) : 0;
           const int real = in_pool ? load.n - token : 0;  // rows behind the sequence become zeros: 0 * NaN would not be 0
           const unsigned char* ks = static_cast<const unsigned char*>(a.pool.k) + first * S::ROW;
           const unsigned char* vs = static_cast<const unsigned char*>(a.pool.v) + first * S::ROW;
@@ -383,10 +390,6 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
     };
 
     const Cursor ahead = next_window(load);
-    issue(0);
-    next_page = look_up(ahead);
-#pragma unroll
-    for (int s = 1; s < S::STAGES - 1; ++s) issue(s);
 
     // Per row: q as fragments of the first operand, the output's accumulators, and the softmax's state.
     constexpr int DIGITS = F == kv::kInt8 ? 3 : 2;  // 8 bits: of q
@@ -396,10 +399,17 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
     float o[NT][PLACES], m = -INFINITY, sum = 0.f, up = 1.f;  // up: what scores are multiplied by for the digits of q
     int row_tile = 0;          // the row's first tile in this warp
     bool opened = false, first_row = true;
-    int stage = 0;
     int row_start = from - use.tile;  // first tile of the row on the line
 
-    for (int i = 0; i < count; ++i) {
+    // Turn i uses tile i; turn -1 starts the first tile's copies (from the same code as all others: what is fetched once is
+    // slow) and opens its row meanwhile.
+    static_assert(S::STAGES == 2, "one tile ahead");
+    for (int i = -1; i < count; ++i) {
+      if (i >= 0) {
+        copies_wait<0>();
+        __syncwarp();
+      }
+      issue((i + 1) & 1);
       if (!opened) {
         opened = true;
         row_tile = use.tile;
@@ -410,9 +420,9 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
           o[t][0] = o[t][1] = 0.f;
           if constexpr (PLACES == 4) o[t][2] = o[t][3] = 0.f;
         }
-        const int in_group = (use.row % chunks) * HEADS + g;
+        const int kv_head = kv_head_of(use.row), in_group = (use.row - kv_head * chunks) * HEADS + g;
         const bool real = in_group < group;
-        const __nv_bfloat16* src = a.q + use.b * a.q_seq + ((long long)(use.row / chunks) * group + in_group) * a.q_head;
+        const __nv_bfloat16* src = a.q + use.b * a.q_seq + ((long long)kv_head * group + in_group) * a.q_head;
         // lane (g, c4) holds, of head g, the 16-byte pieces of a key row that it will load: piece 4 j + c4
         if constexpr (F == kv::kBf16) {
 #pragma unroll
@@ -463,13 +473,11 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
         }
       }
 
-      copies_wait<S::STAGES - 2>();
-      __syncwarp();
-      {
-        int next = stage + S::STAGES - 1;
-        if (next >= S::STAGES) next -= S::STAGES;
-        issue(next);
+      if (i < 0) {
+        next_page = look_up(ahead);
+        continue;
       }
+      const int stage = i & 1;
       const uint32_t kb = ring_addr + stage * S::STAGE, vb = kb + S::DATA;
       const uint32_t in_pool = held >> (4 * stage);
       [[maybe_unused]] const float* const stage_scales = reinterpret_cast<const float*>(ring + stage * S::STAGE + 2 * S::DATA);
@@ -696,7 +704,6 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
         }
       }
       __syncwarp();  // the stage may be refilled
-      if (++stage == S::STAGES) stage = 0;
 
       const bool row_ends = use.tile + 1 == use.tiles, last = i + 1 == count;
       if (row_ends || last) {
@@ -709,9 +716,9 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
         // where accumulator column n of tile t lies in the head's dimensions
         const auto dim = [&](int t, int e) { return F == kv::kBf16 ? t * 8 + 2 * c4 + e : (2 * c4 + e) * NT + t; };
         if (row_ends && row_tile == 0) {
-          const int in_group = (use.row % chunks) * HEADS + g;
+          const int kv_head = kv_head_of(use.row), in_group = (use.row - kv_head * chunks) * HEADS + g;
           if (in_group < group) {
-            const long long head = (long long)use.b * a.H + (use.row / chunks) * group + in_group;
+            const long long head = (long long)use.b * a.H + (long long)kv_head * group + in_group;
             const float norm = sum == 0.f ? 0.f : __fdividef(1.f, sum);
             __nv_bfloat16* dst = a.out + head * D;
             if constexpr (F == kv::kBf16) {
@@ -796,26 +803,36 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
       const Job job = sh.jobs[unit / UNITS];
       const int v0 = unit % UNITS * VALUES;
       float top = -INFINITY, total = 0.f, x[VALUES] = {};
-      for (int i = job.from; i < job.to; i += 2) {
-        const float *p = list[i], *q2 = list[min(i + 1, job.to - 1)];
-        const float m0 = load(p + HEADS * D + g), l0 = load(p + HEADS * D + HEADS + g);
-        float m1 = load(q2 + HEADS * D + g);
-        const float l1 = load(q2 + HEADS * D + HEADS + g);
-        float y0[VALUES], y1[VALUES];
+      constexpr int BATCH = 4;  // pieces whose loads are under way together
+      for (int i = job.from; i < job.to; i += BATCH) {
+        float m[BATCH], l[BATCH], v[BATCH][VALUES], higher = top;
 #pragma unroll
-        for (int y = 0; y < VALUES; ++y) {
-          y0[y] = load(p + (v0 + y) * 32 + lane);
-          y1[y] = load(q2 + (v0 + y) * 32 + lane);
+        for (int k = 0; k < BATCH; ++k) {
+          const float* p = list[min(i + k, job.to - 1)];
+          m[k] = load(p + HEADS * D + g);
+          l[k] = load(p + HEADS * D + HEADS + g);
+#pragma unroll
+          for (int y = 0; y < VALUES; ++y) v[k][y] = load(p + (v0 + y) * 32 + lane);
         }
-        if (i + 1 == job.to) m1 = -INFINITY;
-        const float higher = fmaxf(top, fmaxf(m0, m1)), at = higher == -INFINITY ? 0.f : higher;
-        const float keep = fast_exp2(top - at), w0 = fast_exp2(m0 - at), w1 = fast_exp2(m1 - at);
-        top = higher;
-        total = fmaf(w1, l1, fmaf(w0, l0, total * keep));
 #pragma unroll
-        for (int y = 0; y < VALUES; ++y) x[y] = fmaf(w1, y1[y], fmaf(w0, y0[y], x[y] * keep));
+        for (int k = 0; k < BATCH; ++k) {
+          if (i + k >= job.to) m[k] = -INFINITY;
+          higher = fmaxf(higher, m[k]);
+        }
+        const float at = higher == -INFINITY ? 0.f : higher, keep = fast_exp2(top - at);
+        top = higher;
+        total *= keep;
+#pragma unroll
+        for (int y = 0; y < VALUES; ++y) x[y] *= keep;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const float w = fast_exp2(m[k] - at);
+          total = fmaf(w, l[k], total);
+#pragma unroll
+          for (int y = 0; y < VALUES; ++y) x[y] = fmaf(w, v[k][y], x[y]);
+        }
       }
-      const int kv_head = chunks == 1 ? job.row : job.row / chunks, in_group = (job.row - kv_head * chunks) * HEADS + g;
+      const int kv_head = kv_head_of(job.row), in_group = (job.row - kv_head * chunks) * HEADS + g;
       if (in_group >= group) continue;
       if (job.whole) {
         const long long head = (long long)job.b * a.H + (long long)kv_head * group + in_group;
