@@ -3,6 +3,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <map>
 #include <mutex>
@@ -68,18 +69,18 @@ bool vector_rows(const at::Tensor& x) {
   return x.stride(2) == 1 && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
 }
 
-// The attention kernel's scratch.  Calls on one stream follow one another, so they share one buffer
-// per (device, stream); a captured call gets memory of its own graph, since replays may run on any stream.
-std::pair<float*, unsigned*> attention_scratch(const at::Tensor& like, cudaStream_t stream, at::Tensor& keep) {
-  const long long floats = paged::workspace_floats(sms());
-  const long long bytes = floats * 4 + paged::workspace_counters(sms()) * 4;
+// Scratch of the kernels that join what several blocks leave of a row.  Calls on one stream follow one another, so they share
+// one buffer per (device, stream); a captured call gets memory of its own graph, since replays may run on any stream.
+std::pair<float*, unsigned*> join_scratch(const at::Tensor& like, cudaStream_t stream, at::Tensor& keep) {
+  const long long floats = std::max(paged::workspace_floats(sms()), sampling::workspace_floats(sms()));
+  const long long bytes = floats * 4 + std::max(paged::workspace_counters(sms()), sampling::workspace_counters(sms())) * 4;
   const auto split = [&](const at::Tensor& t) {
     char* base = static_cast<char*>(t.data_ptr());
     return std::make_pair(reinterpret_cast<float*>(base), reinterpret_cast<unsigned*>(base + floats * 4));
   };
   const auto fresh = [&] {
     at::Tensor t = at::empty({bytes}, like.options().dtype(at::kByte));
-    check_launch(cudaMemsetAsync(static_cast<char*>(t.data_ptr()) + floats * 4, 0, bytes - floats * 4, stream), "paged_attention scratch");
+    check_launch(cudaMemsetAsync(static_cast<char*>(t.data_ptr()) + floats * 4, 0, bytes - floats * 4, stream), "scratch");
     return t;
   };
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
@@ -182,7 +183,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> paged_attention(at::Tensor q, 
                 reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), with_lse ? lse->data_ptr<float>() : nullptr, (int)B, (int)H,
                 (float)((scale.has_value() ? *scale : 1.0 / std::sqrt((double)p.D)) * 1.4426950408889634), nullptr, nullptr};
   at::Tensor keep;
-  std::tie(a.partial, a.arrived) = attention_scratch(q, stream, keep);
+  std::tie(a.partial, a.arrived) = join_scratch(q, stream, keep);
   check_launch(paged::launch(a, sms(), stream), "paged_attention");
   return {out, lse};
 }
@@ -207,20 +208,25 @@ std::tuple<at::Tensor, at::Tensor> sample_tokens(at::Tensor logits, at::Tensor n
   if (B == 0) return {token, logprob};
   if (V > 1 && logits.stride(1) != 1) logits = logits.contiguous();
   if (V > 1 && noise.stride(1) != 1) noise = noise.contiguous();
-  const sampling::Args a{logits.data_ptr(),
-                         logits.stride(0),
-                         noise.stride(0),
-                         noise.data_ptr<float>(),
-                         per_row<float>(temperature_rows, temperature, logits, at::kFloat, "temperature"),
-                         per_row<float>(top_p_rows, top_p, logits, at::kFloat, "top_p"),
-                         per_row<float>(min_p_rows, min_p, logits, at::kFloat, "min_p"),
-                         per_row<int>(top_k_rows, (double)std::min<int64_t>(top_k, V), logits, at::kInt, "top_k"),
-                         reinterpret_cast<long long*>(token.data_ptr<int64_t>()),
-                         logprob.data_ptr<float>(),
-                         (int)B,
-                         (int)V,
-                         logits.scalar_type() == at::kFloat};
-  check_launch(sampling::launch(a, sms(), at::cuda::getCurrentCUDAStream()), "sample_tokens");
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  sampling::Args a{logits.data_ptr(),
+                   logits.stride(0),
+                   noise.stride(0),
+                   noise.data_ptr<float>(),
+                   per_row<float>(temperature_rows, temperature, logits, at::kFloat, "temperature"),
+                   per_row<float>(top_p_rows, top_p, logits, at::kFloat, "top_p"),
+                   per_row<float>(min_p_rows, min_p, logits, at::kFloat, "min_p"),
+                   per_row<int>(top_k_rows, (double)std::min<int64_t>(top_k, V), logits, at::kInt, "top_k"),
+                   reinterpret_cast<long long*>(token.data_ptr<int64_t>()),
+                   logprob.data_ptr<float>(),
+                   (int)B,
+                   (int)V,
+                   logits.scalar_type() == at::kFloat,
+                   nullptr,
+                   nullptr};
+  at::Tensor keep;
+  if (sampling::streams(a, sms())) std::tie(a.partial, a.arrived) = join_scratch(logits, stream, keep);
+  check_launch(sampling::launch(a, sms(), stream), "sample_tokens");
   return {token, logprob};
 }
 

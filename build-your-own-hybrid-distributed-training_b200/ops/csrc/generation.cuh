@@ -109,8 +109,16 @@ struct Args {
   float* logprob;
   int B, V;
   int wide;  // fp32 logits
+  float* partial;     // where `streams` says so, workspace_floats(): what a block leaves of a row that other blocks share
+  unsigned* arrived;  // likewise workspace_counters(): zero before the first call; every call leaves them zero
 };
 
+// Whether a call takes the kernel for many rows of which nothing is cut (sampling_stream.cu), and the scratch that this one
+// needs on a GPU with this many SMs.
+bool streams(const Args& a, int sms);
+long long workspace_floats(int sms);
+int workspace_counters(int sms);
+cudaError_t launch_stream(const Args& a, int sms, cudaStream_t stream);
 cudaError_t launch(const Args& a, int sms, cudaStream_t stream);
 
 }  // namespace sampling

@@ -12,7 +12,8 @@
 //
 // Bound: memory (the logits once, and the random numbers of the tokens that may be drawn); at a handful of
 // rows, the latency of the steps.  A row belongs to a cluster of blocks, which exchange a few numbers per step
-// through distributed shared memory.  There are three ways through a row, each with fewer steps than the next:
+// through distributed shared memory.  (Many rows of which nothing is cut are streamed by another kernel, see `streams`.)  There
+// are three ways through a row, each with fewer steps than the next:
 //
 // * Nothing to cut (no top_k, top_p or min_p, or T <= 0): one pass over logits and random numbers with a running
 //   reference for the exponentials, rescaled by powers of two, so that no step waits for the maximum.
@@ -29,71 +30,19 @@
 // overflow.  Integer sums do not depend on their order, so neither do the cuts.
 #include <cooperative_groups.h>
 
-#include "generation.cuh"
+#include "sampling.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace ht {
 namespace sampling {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int BINS = 2048;
 constexpr int LIST = 256;       // tokens of one bin that are ranked directly
 constexpr int SHORT = 256;      // tokens of a short prefix
 constexpr int MEDIUM = 2048;    // tokens of a longer one, or of one bin
 constexpr int STAGED = BINS * 3 / 2;  // tokens that the bins' memory holds
 constexpr int MOST_BLOCKS = 8;  // of a cluster
-constexpr float LN2 = 0.6931471805599453f;
-
-// Unsigned keys in the order of the floats; -inf has the lowest one.
-__device__ __forceinline__ uint32_t key_of(float l) {
-  if (!(l > -INFINITY)) return 0u;
-  const uint32_t u = __float_as_uint(l + 0.f);  // -0 + 0 = +0: equal logits have equal keys
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float value_of(uint32_t key) {  // keys below that of the lowest number stand for -inf
-  return key <= 0x007fffffu ? -INFINITY : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-}
-
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// w = 2^((l - best) log2(e) / T); the quotient is carried in two floats, since its rounding error times the distance
-// would show in the weights of unlikely tokens.
-struct Weights {
-  float best, hi, lo, least;
-  bool single;  // only tokens equal to the best weigh anything (best = +inf, or 1 / T beyond fp32)
-  __device__ Weights(float best_, float temperature) : best(best_) {
-    const double rate = 1.4426950408889634 / fmin((double)temperature, 1e30);
-    hi = (float)rate;
-    single = best == INFINITY || hi == INFINITY;
-    lo = single ? 0.f : (float)(rate - (double)hi);
-    least = single ? 0.f : -2048.f / hi;  // further away the weight is zero whatever the correction says
-  }
-  __device__ __forceinline__ float exponent(float l) const {
-    if (single) return l == best ? 0.f : -INFINITY;
-    const float d = l - best;
-    return fmaf(d, hi, fmaxf(d, least) * lo);
-  }
-  __device__ __forceinline__ float operator()(float l) const { return fast_exp2(exponent(l)); }
-  __device__ __forceinline__ uint32_t fixed(float l) const { return (uint32_t)__float2uint_rn((*this)(l)*2147483648.f); }
-};
-
-// A sum of weights that comes out the same in every order (and so for every alignment of the row): multiples of 2^-16,
-// which a thread's few hundred terms add without rounding, and what they leave of each weight (at most 2^-17), whose
-// roundings lie far below the fp32 result.
-struct Sum {
-  float coarse = 0.f, fine = 0.f;
-  __device__ __forceinline__ void add(float w) {
-    const float near = __fadd_rn(__fadd_rn(w, 128.f), -128.f);
-    coarse += near;
-    fine += w - near;
-  }
-  __device__ __forceinline__ double value() const { return (double)coarse + (double)fine; }
-};
 
 struct Found {  // where a running sum over the bins crosses its target
   int bin;
@@ -125,42 +74,6 @@ struct Shared {
   uint32_t counts[MOST_BLOCKS];                               // likewise
   Found found;
   unsigned long long cut;
-};
-
-template <typename V, typename Op>
-__device__ __forceinline__ V block_reduce(V v, V* scratch, Op op) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = v;
-  __syncthreads();
-  v = scratch[threadIdx.x % WARPS];
-#pragma unroll
-  for (int o = WARPS / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-
-// 16 bytes of the row as floats.
-template <typename T>
-struct Piece {
-  static constexpr int E = 16 / sizeof(T);
-  float v[E];
-  static __device__ __forceinline__ float one(T x) {
-    if constexpr (sizeof(T) == 4) return x;
-    else return __bfloat162float(x);
-  }
-  __device__ __forceinline__ explicit Piece(uint4 raw) {
-    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (sizeof(T) == 4) {
-        v[j] = __uint_as_float(u[j]);
-      } else {
-        v[2 * j] = __uint_as_float(u[j] << 16);
-        v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-      }
-    }
-  }
 };
 
 // Bins of 1/64 of the exponent (to base e) for the first 32; everything further away shares the last bin.  Monotone in l,
@@ -907,13 +820,33 @@ static cudaError_t launch_as(const Args& a, int blocks, cudaStream_t stream) {
   return cudaLaunchKernelEx(&config, sample_kernel<T>, a);
 }
 
-cudaError_t launch(const Args& a, int sms, cudaStream_t stream) {
-  // Blocks per row: as many as let two of them share an SM (72 KB of the row each), and more while all of them run at
-  // once and have some tokens for each thread.
-  const int size = a.wide ? 4 : 2;
+// Blocks per row: as many as let two of them share an SM (72 KB of the row each), and more while all of them run at once
+// and have some tokens for each thread.
+static int blocks_per_row(const Args& a, int sms) {
   int blocks = 1;
-  while (blocks < MOST_BLOCKS && (long long)a.V * size > blocks * 73728ll) blocks *= 2;
+  while (blocks < MOST_BLOCKS && (long long)a.V * (a.wide ? 4 : 2) > blocks * 73728ll) blocks *= 2;
   while (blocks < MOST_BLOCKS && (long long)a.B * blocks <= sms && a.V > blocks * 4096) blocks *= 2;
+  return blocks;
+}
+
+// Rows of which nothing is cut, at an ordinary temperature (which the host has to know), are streamed by persistent blocks where
+// clusters of two blocks or more would need a second wave: 64 rows of 128256 in fp32 21.1 us against 23.1, 256 rows 47 against 81,
+// in bf16 128 rows 27.3 against 30.2.  With one wave (32 rows in fp32 15.6 against 11.6 us) or one block per row (512 rows of 32000
+// in bf16 32.0 against 29.5, 1024 of 16384 in fp32 42 against 38.6) clusters are faster.
+bool streams(const Args& a, int sms) {
+  const float t = a.temperature.same;
+  const bool greedy = t <= 0.f, numbers = a.top_k.rows == nullptr && a.top_p.rows == nullptr && a.min_p.rows == nullptr;
+  if (a.temperature.rows != nullptr || !(greedy || (numbers && t > 1e-3f && t < 1e3f))) return false;
+  if (!greedy && ((a.top_k.same > 0 && a.top_k.same < a.V) || !(a.top_p.same >= 1.f) || a.min_p.same > 0.f)) return false;
+  const int blocks = blocks_per_row(a, sms);
+  if (blocks == 1 || (long long)a.B * blocks <= 2ll * sms) return false;
+  // what the streaming kernel counts in 32 bits, and the rows of one block that it can put off
+  return (long long)a.B * (a.V / 4 + 2) < (1ll << 31) && a.B / sms < 1000;
+}
+
+cudaError_t launch(const Args& a, int sms, cudaStream_t stream) {
+  if (streams(a, sms)) return launch_stream(a, sms, stream);
+  const int blocks = blocks_per_row(a, sms);
   return a.wide ? launch_as<float>(a, blocks, stream) : launch_as<__nv_bfloat16>(a, blocks, stream);
 }
 

@@ -1,0 +1,99 @@
+// What the sampling kernels share: orders of floats, weights and their sums, rows in pieces of 16 bytes.
+#pragma once
+
+#include "generation.cuh"
+
+namespace ht {
+namespace sampling {
+
+constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr float LN2 = 0.6931471805599453f;
+
+// Unsigned keys in the order of the floats; -inf has the lowest one.
+__device__ __forceinline__ uint32_t key_of(float l) {
+  if (!(l > -INFINITY)) return 0u;
+  const uint32_t u = __float_as_uint(l + 0.f);  // -0 + 0 = +0: equal logits have equal keys
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t key) {  // keys below that of the lowest number stand for -inf
+  return key <= 0x007fffffu ? -INFINITY : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// w = 2^((l - best) log2(e) / T); the quotient is carried in two floats, since its rounding error times the distance
+// would show in the weights of unlikely tokens.
+struct Weights {
+  float best, hi, lo, least;
+  bool single;  // only tokens equal to the best weigh anything (best = +inf, or 1 / T beyond fp32)
+  __device__ Weights(float best_, float temperature) : best(best_) {
+    const double rate = 1.4426950408889634 / fmin((double)temperature, 1e30);
+    hi = (float)rate;
+    single = best == INFINITY || hi == INFINITY;
+    lo = single ? 0.f : (float)(rate - (double)hi);
+    least = single ? 0.f : -2048.f / hi;  // further away the weight is zero whatever the correction says
+  }
+  __device__ __forceinline__ float exponent(float l) const {
+    if (single) return l == best ? 0.f : -INFINITY;
+    const float d = l - best;
+    return fmaf(d, hi, fmaxf(d, least) * lo);
+  }
+  __device__ __forceinline__ float operator()(float l) const { return fast_exp2(exponent(l)); }
+  __device__ __forceinline__ uint32_t fixed(float l) const { return (uint32_t)__float2uint_rn((*this)(l)*2147483648.f); }
+};
+
+// A sum of weights that comes out the same in every order (and so for every alignment of the row): multiples of 2^-16,
+// which a thread's few hundred terms add without rounding, and what they leave of each weight (at most 2^-17), whose
+// roundings lie far below the fp32 result.
+struct Sum {
+  float coarse = 0.f, fine = 0.f;
+  __device__ __forceinline__ void add(float w) {
+    const float near = __fadd_rn(__fadd_rn(w, 128.f), -128.f);
+    coarse += near;
+    fine += w - near;
+  }
+  __device__ __forceinline__ double value() const { return (double)coarse + (double)fine; }
+};
+
+template <int N = WARPS, typename V, typename Op>
+__device__ __forceinline__ V block_reduce(V v, V* scratch, Op op) {  // of a block of N warps
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = v;
+  __syncthreads();
+  v = scratch[threadIdx.x % N];
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// 16 bytes of the row as floats.
+template <typename T>
+struct Piece {
+  static constexpr int E = 16 / sizeof(T);
+  float v[E];
+  static __device__ __forceinline__ float one(T x) {
+    if constexpr (sizeof(T) == 4) return x;
+    else return __bfloat162float(x);
+  }
+  __device__ __forceinline__ explicit Piece(uint4 raw) {
+    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        v[j] = __uint_as_float(u[j]);
+      } else {
+        v[2 * j] = __uint_as_float(u[j] << 16);
+        v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+      }
+    }
+  }
+};
+
+}  // namespace sampling
+}  // namespace ht

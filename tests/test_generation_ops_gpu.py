@@ -446,6 +446,90 @@ def test_sample_tokens_follows_the_distribution() -> None:
     assert bool(((share - p).abs() <= 5.0 * torch.sqrt(p * (1 - p) / b)).all())
 
 
+# Batches whose rows are streamed by persistent blocks (more than one wave of clusters): shared rows, odd sizes, the largest vocabulary.
+_MANY = [(151, 18500, torch.float32), (77, 50257, torch.float32), (39, 128256, torch.float32), (38, 262144, torch.float32),
+         (75, 128256, torch.bfloat16), (160, 50257, torch.bfloat16), (38, 262143, torch.bfloat16), (700, 20011, torch.float32)]
+
+
+@pytest.mark.parametrize("b, v, dtype", _MANY)
+@pytest.mark.parametrize("filters", [{}, {"temperature": 0.0}, {"temperature": 0.6}, {"temperature": 40.0}, {"temperature": 0.01, "top_k": 1 << 20},
+                                     {"temperature": 0.0, "top_k": 3, "top_p": 0.5}])
+def test_sample_tokens_many_rows(b, v, dtype, filters) -> None:
+    logits, noise = _logits(b, v, dtype, seed=b + v)
+    token = _check_sample(logits, noise, **filters)
+    per_row = torch.full((b,), filters.get("temperature", 1.0), device="cuda")
+    assert torch.equal(token, ops.sample_tokens(logits, noise, **{**filters, "temperature": per_row})[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("filters", [{}, {"temperature": 0.0}, {"temperature": 500.0}])
+def test_sample_tokens_many_rows_masked_infinite_and_nan(dtype, filters) -> None:
+    b, v = 160, 40001
+    logits, noise = _logits(b, v, dtype, seed=21)
+    lowest = torch.finfo(dtype).min
+    logits[0] = -math.inf
+    logits[1] = -math.inf
+    logits[1, 12345] = -5.0
+    logits[2, 1:] = -math.inf
+    logits[3, ::3] = math.nan
+    logits[4] = math.nan
+    logits[5, 7] = math.inf
+    logits[6, 5:] = lowest
+    logits[7] = lowest
+    logits[8] = 3e6 * logits[8]  # too far apart for exponents without a reference
+    logits[9] = logits[9] - 2.0**40
+    logits[10, : v // 2] = -math.inf
+    logits[11, v // 2 :] = lowest
+    logits[12] = lowest
+    logits[12, v - 1] = -1e4
+    logits[b - 1] = -math.inf
+    logits[b - 2, :-1] = -math.inf
+    token = _check_sample(logits, noise, **filters)
+    assert token[0] == -1 and token[4] == -1 and token[b - 1] == -1
+    assert token[1] == 12345 and token[2] == 0 and token[5] == 7 and token[6] < 5 and token[12] == v - 1 and token[b - 2] == v - 1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("filters", [{}, {"temperature": 0.0}])
+def test_sample_tokens_many_rows_ties_and_strides(dtype, filters) -> None:
+    b, v = 160, 40001
+    logits, noise = torch.zeros(b, v + 8, device="cuda", dtype=dtype)[:, 3 : v + 3], torch.ones(b, v + 6, device="cuda")[:, 1 : v + 1]
+    assert torch.equal(_check_sample(logits, noise, **filters), torch.zeros(b, dtype=torch.int64, device="cuda"))  # the first among equals
+    at = torch.randint(1, v - 1, (b,), device="cuda")
+    logits.scatter_(1, at[:, None], 1.0)
+    logits.scatter_(1, at[:, None] + 1, 1.0)
+    assert torch.equal(_check_sample(logits, noise, **filters), at)
+    values, luck = _logits(b, v, dtype, seed=22)
+    want = ops.sample_tokens(values, luck, **filters)
+    logits.copy_(values)
+    noise.copy_(luck)
+    for x, e in ((logits, noise), (values, noise), (logits, luck), (values.t().contiguous().t(), luck)):
+        got = ops.sample_tokens(x, e, **filters)
+        assert torch.equal(got[0], want[0])
+        assert bool(((got[1] - want[1]).abs() <= 4e-6 * (1.0 + want[1].abs())).all())
+
+
+def test_sample_tokens_many_rows_on_streams_and_in_graphs() -> None:
+    inputs = [_logits(b, v, torch.float32, seed=b) for b, v in ((77, 50257), (151, 18500))]
+    want = [ops.sample_tokens(*x) for x in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        got = []
+        for stream, x in zip(streams, inputs, strict=True):
+            with torch.cuda.stream(stream):
+                got.append(ops.sample_tokens(*x))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for gs, ws in zip(got, want, strict=True) for g, w in zip(gs, ws, strict=True))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [ops.sample_tokens(*x) for x in inputs]
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for gs, ws in zip(got, want, strict=True) for g, w in zip(gs, ws, strict=True))
+
+
 # --------------------------------------------------------------------------- refusals
 
 
