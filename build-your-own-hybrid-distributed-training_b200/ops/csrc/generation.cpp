@@ -223,7 +223,8 @@ std::tuple<at::Tensor, at::Tensor> sample_tokens(at::Tensor logits, at::Tensor n
                    (int)V,
                    logits.scalar_type() == at::kFloat,
                    nullptr,
-                   nullptr};
+                   nullptr,
+                   0};
   at::Tensor keep;
   if (sampling::streams(a, sms())) std::tie(a.partial, a.arrived) = join_scratch(logits, stream, keep);
   check_launch(sampling::launch(a, sms(), stream), "sample_tokens");

@@ -90,6 +90,7 @@ cudaError_t launch(const Args& a, int sms, cudaStream_t stream);
 namespace sampling {
 
 constexpr int kMaxVocabulary = 1 << 18;
+constexpr int kMostListed = 2048;  // rows of a batch that the streaming kernel picks its own from
 
 // One value per row, or one for all of them.
 template <typename T>
@@ -111,14 +112,15 @@ struct Args {
   int wide;  // fp32 logits
   float* partial;     // where `streams` says so, workspace_floats(): what a block leaves of a row that other blocks share
   unsigned* arrived;  // likewise workspace_counters(): zero before the first call; every call leaves them zero
+  int streamed;       // set by `launch`: rows that the streaming kernel takes are not this launch's
 };
 
-// Whether a call takes the kernel for many rows of which nothing is cut (sampling_stream.cu), and the scratch that this one
-// needs on a GPU with this many SMs.
+// Whether a call takes the kernel for many rows of which nothing is cut (sampling_stream.cu), for all rows (`whole`) or for those
+// that turn out to be such, and the scratch that it needs on a GPU with this many SMs.
 bool streams(const Args& a, int sms);
 long long workspace_floats(int sms);
 int workspace_counters(int sms);
-cudaError_t launch_stream(const Args& a, int sms, cudaStream_t stream);
+cudaError_t launch_stream(const Args& a, bool whole, int sms, cudaStream_t stream);
 cudaError_t launch(const Args& a, int sms, cudaStream_t stream);
 
 }  // namespace sampling

@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   const bool greedy = !(temperature > 0.f);
   const int top_k = a.top_k[row];
   const float top_p = a.top_p[row], min_p = a.min_p[row];
+  if (a.streamed && ordinary(temperature) && cuts_nothing(top_k, top_p, min_p, a.V)) return;
   const bool by_count = !greedy && top_k > 0 && top_k < a.V, by_mass = !greedy && !(top_p >= 1.f);
   const float* const noise = a.noise + row * a.noise_stride;
 
@@ -829,23 +830,39 @@ static int blocks_per_row(const Args& a, int sms) {
   return blocks;
 }
 
-// Rows of which nothing is cut, at an ordinary temperature (which the host has to know), are streamed by persistent blocks where
-// clusters of two blocks or more would need a second wave: 64 rows of 128256 in fp32 21.1 us against 23.1, 256 rows 47 against 81,
-// in bf16 128 rows 27.3 against 30.2.  With one wave (32 rows in fp32 15.6 against 11.6 us) or one block per row (512 rows of 32000
-// in bf16 32.0 against 29.5, 1024 of 16384 in fp32 42 against 38.6) clusters are faster.
+// Rows of which nothing is cut, at an ordinary temperature, are streamed by persistent blocks where clusters of two blocks or
+// more would need a second wave: 64 rows of 128256 in fp32 21.1 us against 23.1, 256 rows 47 against 81, in bf16 128 rows 27.3
+// against 30.2.  With one wave (32 rows in fp32 15.6 against 11.6 us) or one block per row (512 rows of 32000 in bf16 32.0 against
+// 29.5, 1024 of 16384 in fp32 42 against 38.6) clusters are faster.
+// Where temperature or filters are per row, only the device knows which rows those are: both kernels are launched, and each
+// leaves the other's rows alone.  That pays from four blocks per row and two waves on: 256 rows of 128256 in fp32 58 us against 83,
+// 96 rows 30.7 against 34.1, 192 in bf16 39.9 against 44.3; 64 rows in fp32 25.0 against 23.1, 128 in bf16 32.0 against 30.2.
+// Batches that turn out to be cut lose the time of a launch (256 rows of top-k 1000: 168 -> 172 us).
+static bool whole_stream(const Args& a) {
+  if (a.temperature.rows != nullptr) return false;
+  if (a.temperature.same <= 0.f) return true;
+  return ordinary(a.temperature.same) && a.top_k.rows == nullptr && a.top_p.rows == nullptr && a.min_p.rows == nullptr &&
+         cuts_nothing(a.top_k.same, a.top_p.same, a.min_p.same, a.V);
+}
+
 bool streams(const Args& a, int sms) {
-  const float t = a.temperature.same;
-  const bool greedy = t <= 0.f, numbers = a.top_k.rows == nullptr && a.top_p.rows == nullptr && a.min_p.rows == nullptr;
-  if (a.temperature.rows != nullptr || !(greedy || (numbers && t > 1e-3f && t < 1e3f))) return false;
-  if (!greedy && ((a.top_k.same > 0 && a.top_k.same < a.V) || !(a.top_p.same >= 1.f) || a.min_p.same > 0.f)) return false;
   const int blocks = blocks_per_row(a, sms);
   if (blocks == 1 || (long long)a.B * blocks <= 2ll * sms) return false;
   // what the streaming kernel counts in 32 bits, and the rows of one block that it can put off
-  return (long long)a.B * (a.V / 4 + 2) < (1ll << 31) && a.B / sms < 1000;
+  if (whole_stream(a)) return (long long)a.B * (a.V / 4 + 2) < (1ll << 31) && a.B / sms < 1000;
+  if (blocks < 4 || (long long)a.B * blocks <= 4ll * sms || a.B > kMostListed) return false;
+  return (a.temperature.rows != nullptr || ordinary(a.temperature.same)) &&
+         cuts_nothing(a.top_k.rows != nullptr ? 0 : a.top_k.same, a.top_p.rows != nullptr ? 1.f : a.top_p.same,
+                      a.min_p.rows != nullptr ? 0.f : a.min_p.same, a.V);
 }
 
-cudaError_t launch(const Args& a, int sms, cudaStream_t stream) {
-  if (streams(a, sms)) return launch_stream(a, sms, stream);
+cudaError_t launch(const Args& args, int sms, cudaStream_t stream) {
+  Args a = args;
+  a.streamed = streams(a, sms);
+  if (a.streamed) {
+    const cudaError_t err = launch_stream(a, whole_stream(a), sms, stream);
+    if (err != cudaSuccess || whole_stream(a)) return err;
+  }
   const int blocks = blocks_per_row(a, sms);
   return a.wide ? launch_as<float>(a, blocks, stream) : launch_as<__nv_bfloat16>(a, blocks, stream);
 }

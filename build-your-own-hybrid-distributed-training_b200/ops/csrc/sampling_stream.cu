@@ -76,9 +76,14 @@ __device__ __forceinline__ unsigned arrive(unsigned* counter) {  // publishes th
 struct Small {
   Part parts[2][GROUPS];
   int rows[MOST_ROWS];  // left for the end: infinite or huge logits
-  int count;
+  int count, counts[GROUPS];
   double sums[GROUPS];
   unsigned long long picks[GROUPS];
+};
+
+struct Listed {
+  int row;
+  float temperature;
 };
 
 template <bool GREEDY, typename T>
@@ -89,9 +94,10 @@ struct Ring {
   static constexpr int BYTES = STAGES * UNITS * WIDTH * 16;
 };
 
-template <bool GREEDY, typename T>
+// WHOLE: all rows are this kernel's, at one temperature, whose log2(e) / T is hi + lo.
+template <bool GREEDY, bool WHOLE, typename T>
 __global__ void __launch_bounds__(WIDTH, 1)
-stream_kernel(const __grid_constant__ Args a, int pieces /* of a row's share of the line */, int line, int per_block, float hi, float lo) {
+stream_kernel(const __grid_constant__ Args a, int pieces /* of a row's share of the line */, float hi, float lo) {
   using R = Ring<GREEDY, T>;
   constexpr int E = R::E, PER = R::PER, UNITS = R::UNITS, STAGES = R::STAGES, TURN = PER * WIDTH;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -99,22 +105,45 @@ stream_kernel(const __grid_constant__ Args a, int pieces /* of a row's share of 
   uint4* const ring = reinterpret_cast<uint4*>(smem) + threadIdx.x;
   float* const lucks = reinterpret_cast<float*>(smem) + (PER * WIDTH * 4 + threadIdx.x / 32 * 32 * E);
   Small& sh = *reinterpret_cast<Small*>(smem + R::BYTES);
+  Listed* const listed = reinterpret_cast<Listed*>(smem + R::BYTES + sizeof(Small));  // not if WHOLE
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
 
-  const int from = per_block * blockIdx.x, to = min(line - from, per_block) + from;
   if (tid == 0) sh.count = 0;
+  int rows = a.B;
+  if constexpr (!WHOLE) {  // list this kernel's rows
+    rows = 0;
+    for (int r0 = 0; r0 < a.B; r0 += WIDTH) {
+      const int r = r0 + tid;
+      const float temperature = r < a.B ? a.temperature[r] : 0.f;
+      const bool mine = r < a.B && ordinary(temperature) && cuts_nothing(a.top_k[r], a.top_p[r], a.min_p[r], a.V);
+      const uint32_t same = __ballot_sync(0xffffffffu, mine);
+      if (lane == 0) sh.counts[warp] = __popc(same);
+      __syncthreads();
+      const uint32_t count = sh.counts[lane];
+      const int before = (int)__reduce_add_sync(0xffffffffu, lane < warp ? count : 0u);
+      if (mine) listed[rows + before + __popc(same & ((1u << lane) - 1))] = Listed{r, temperature};
+      rows += (int)__reduce_add_sync(0xffffffffu, count);
+      __syncthreads();
+    }
+  }
+  // a row spans at most 17 blocks: fewer than a warp's lanes, which merge its parts
+  const int line = rows * pieces, per_block = max((int)(((uint32_t)line + gridDim.x - 1) / gridDim.x), (pieces + 15) / 16);
+  const int from = (int)min((long long)line, (long long)per_block * blockIdx.x);
+  if (from >= line) return;
+  const int to = min(line - from, per_block) + from;
 
   // A stretch of a row: pieces i ... end - 1, of which the whole ones (all tokens inside the row) are copied.
   struct Stretch {
-    int row, i, end, skew;
+    int at, row, i, end, skew;  // at: on the line
   };
   const auto row_logits = [&](int row) { return static_cast<const T*>(a.logits) + row * a.row_stride; };
   const auto row_noise = [&](int row) { return a.noise + row * a.noise_stride; };
-  const auto stretch_at = [&](int row, int i) {
-    return Stretch{row, i, min(pieces, to - row * pieces), (int)((reinterpret_cast<uintptr_t>(row_logits(row)) % 16) / sizeof(T))};
+  const auto stretch_at = [&](int at, int i) {
+    const int row = WHOLE ? at : listed[at].row;
+    return Stretch{at, row, i, min(pieces, to - at * pieces), (int)((reinterpret_cast<uintptr_t>(row_logits(row)) % 16) / sizeof(T))};
   };
-  const auto last_one = [&](const Stretch& s) { return s.row * pieces + s.end == to; };
+  const auto last_one = [&](const Stretch& s) { return s.at * pieces + s.end == to; };
 
   const int first_row = from / pieces;
   Stretch use = stretch_at(first_row, from - first_row * pieces);
@@ -165,7 +194,7 @@ stream_kernel(const __grid_constant__ Args a, int pieces /* of a row's share of 
       if (ahead.i >= ahead.end) {
         more = !last_one(ahead);
         if (more) {
-          ahead = stretch_at(ahead.row + 1, 0);
+          ahead = stretch_at(ahead.at + 1, 0);
           open();
         }
       }
@@ -175,11 +204,17 @@ stream_kernel(const __grid_constant__ Args a, int pieces /* of a row's share of 
 
   // Of the warp: the reference, and the best score so far (greedy: logit) with its token.  w / e > score is asked as
   // w > score e, without a division; of a warp's tokens only some ten per row get past that.
-  const float nothing = -1e30f * hi;  // where no token has been seen that can be drawn: their logits lie above -1e30
+  float nothing;  // the reference where no token has been seen that can be drawn: their logits lie above -1e30
   float reference, score;
   uint32_t drawn;
   Pair sums;  // of the thread
   const auto clear = [&] {
+    if constexpr (!WHOLE) {
+      const float temperature = listed[use.at].temperature, most = 1.4426950216293335f;  // of log2(e)
+      hi = most / temperature;
+      lo = (fmaf(-hi, temperature, most) + 1.925963033500011e-8f) / temperature;
+    }
+    nothing = -1e30f * hi;
     reference = nothing;
     score = GREEDY ? -1e30f : -1.f;
     drawn = NOBODY;
@@ -298,8 +333,8 @@ stream_kernel(const __grid_constant__ Args a, int pieces /* of a row's share of 
     if (lane == 0) sh.parts[parity][warp] = Part{reference, sum, drawn == NOBODY ? 0u : key_of(score), drawn};
     __syncthreads();  // the other half of `parts` was read before its readers came here
     if (warp == merger) {
-      const int row_from = use.row * pieces;
-      bool whole = row_from >= from && row_from + pieces <= to;
+      const int row_from = use.at * pieces;
+      bool complete = row_from >= from && row_from + pieces <= to;
       const Part* list = sh.parts[parity];
       int n = GROUPS, step = 1, skip = 0;
       for (;;) {
@@ -314,7 +349,7 @@ stream_kernel(const __grid_constant__ Args a, int pieces /* of a row's share of 
         const uint32_t first = __reduce_max_sync(0xffffffffu, key);
         token = __reduce_min_sync(0xffffffffu, key == first ? token : NOBODY);
         key = first;
-        if (whole) {
+        if (complete) {
           if (lane == 0) {
             // beyond this the products with the rate lose the differences (or a logit is infinite)
             if (fabsf(most) < 1e5f && token != NOBODY) {
@@ -341,11 +376,11 @@ stream_kernel(const __grid_constant__ Args a, int pieces /* of a row's share of 
         n = last_block - first_block + 1;
         step = 2;
         skip = row_from > per_block * first_block;
-        whole = true;
+        complete = true;
       }
     }
     if (last_one(use)) break;
-    use = stretch_at(use.row + 1, 0);
+    use = stretch_at(use.at + 1, 0);
     clear();
     parity ^= 1;
     merger = (merger + 1) % GROUPS;
@@ -369,7 +404,7 @@ stream_kernel(const __grid_constant__ Args a, int pieces /* of a row's share of 
       }
       continue;
     }
-    const Weights weight(value_of(best), GREEDY ? 1.f : a.temperature.same);
+    const Weights weight(value_of(best), GREEDY ? 1.f : a.temperature[row]);
     double total = 0.0;
     unsigned long long pick = 0;
     for (int token = tid; token < a.V; token += WIDTH) {
@@ -393,10 +428,10 @@ stream_kernel(const __grid_constant__ Args a, int pieces /* of a row's share of 
 
 }  // namespace
 
-template <bool GREEDY, typename T>
+template <bool GREEDY, bool WHOLE, typename T>
 static cudaError_t stream_as(const Args& a, int sms, cudaStream_t stream) {
   using R = Ring<GREEDY, T>;
-  const int smem = R::BYTES + (int)sizeof(Small), pieces = (a.V + 2 * R::E - 2) / R::E;
+  const int pieces = (a.V + 2 * R::E - 2) / R::E, fixed = R::BYTES + (int)sizeof(Small);
   // dynamic shared memory beyond 48 KB is opted into once per device
   static unsigned long long opted = 0;
   int device = 0;
@@ -404,20 +439,21 @@ static cudaError_t stream_as(const Args& a, int sms, cudaStream_t stream) {
   if (err != cudaSuccess) return err;
   const unsigned long long bit = 1ull << (device & 63);
   if (!(__atomic_load_n(&opted, __ATOMIC_ACQUIRE) & bit)) {
-    err = cudaFuncSetAttribute(stream_kernel<GREEDY, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    err = cudaFuncSetAttribute(stream_kernel<GREEDY, WHOLE, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               fixed + (WHOLE ? 0 : kMostListed * (int)sizeof(Listed)));
     if (err != cudaSuccess) return err;
     __atomic_fetch_or(&opted, bit, __ATOMIC_RELEASE);
   }
-  const int line = a.B * pieces, per_block = (line + sms - 1) / sms;
   const double rate = 1.4426950408889634 / (GREEDY ? 1.0 : (double)a.temperature.same);
   const float hi = (float)rate, lo = (float)(rate - (double)hi);
-  stream_kernel<GREEDY, T><<<(unsigned)((line + per_block - 1) / per_block), WIDTH, smem, stream>>>(a, pieces, line, per_block, hi, lo);
+  stream_kernel<GREEDY, WHOLE, T><<<(unsigned)sms, WIDTH, fixed + (WHOLE ? 0 : a.B * (int)sizeof(Listed)), stream>>>(a, pieces, hi, lo);
   return cudaGetLastError();
 }
 
-cudaError_t launch_stream(const Args& a, int sms, cudaStream_t stream) {
-  if (a.temperature.same > 0.f) return a.wide ? stream_as<false, float>(a, sms, stream) : stream_as<false, __nv_bfloat16>(a, sms, stream);
-  return a.wide ? stream_as<true, float>(a, sms, stream) : stream_as<true, __nv_bfloat16>(a, sms, stream);
+cudaError_t launch_stream(const Args& a, bool whole, int sms, cudaStream_t stream) {
+  if (!whole) return a.wide ? stream_as<false, false, float>(a, sms, stream) : stream_as<false, false, __nv_bfloat16>(a, sms, stream);
+  if (a.temperature.same > 0.f) return a.wide ? stream_as<false, true, float>(a, sms, stream) : stream_as<false, true, __nv_bfloat16>(a, sms, stream);
+  return a.wide ? stream_as<true, true, float>(a, sms, stream) : stream_as<true, true, __nv_bfloat16>(a, sms, stream);
 }
 
 long long workspace_floats(int sms) { return 2ll * sms * (long long)(sizeof(Part) / sizeof(float)); }

@@ -489,6 +489,23 @@ def test_sample_tokens_many_rows_masked_infinite_and_nan(dtype, filters) -> None
     assert token[1] == 12345 and token[2] == 0 and token[5] == 7 and token[6] < 5 and token[12] == v - 1 and token[b - 2] == v - 1
 
 
+@pytest.mark.parametrize("b, v, dtype", [(151, 50257, torch.float32), (150, 128256, torch.bfloat16), (1500, 36999, torch.float32), (2049, 36999, torch.float32)])
+@pytest.mark.parametrize("share", [0.0, 0.02, 0.5, 1.0])
+def test_sample_tokens_many_rows_with_values_per_row(b, v, dtype, share) -> None:
+    """Rows that are cut, greedy rows and rows of which nothing is cut, of different temperatures, in one batch."""
+    logits, noise = _logits(b, v, dtype, seed=b + 7)
+    gen = torch.Generator(device="cuda").manual_seed(b)
+    plain = torch.rand(b, device="cuda", generator=gen) < share
+    pick = lambda values: torch.tensor(values, device="cuda")[torch.randint(0, len(values), (b,), device="cuda", generator=gen)]  # noqa: E731
+    choose = lambda values, otherwise: torch.where(plain, torch.full_like(pick(values), otherwise), pick(values))  # noqa: E731
+    _check_sample(logits, noise, temperature=torch.where(plain, pick([0.3, 1.0, 2.0, 9.0]), pick([0.0, 0.5, 1.0, 1e-4])),
+                  top_k=choose([0, 7, 900], 0).to(torch.int32), top_p=choose([0.5, 0.95], 1.0), min_p=choose([0.0, 0.1], 0.0))
+    if share == 1.0:
+        temperature = pick([0.3, 1.0, 2.0, 9.0])
+        _check_sample(logits, noise, temperature=temperature)
+        _check_sample(logits, noise, temperature=0.7, top_p=torch.ones(b, device="cuda"), min_p=torch.zeros(b, device="cuda"))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("filters", [{}, {"temperature": 0.0}])
 def test_sample_tokens_many_rows_ties_and_strides(dtype, filters) -> None:
