@@ -574,25 +574,35 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     return sh.cut;
   };
 
-  Sum total;
+  Sums total;
   // ---- a short prefix: the tokens that reach the threshold, ranked by the first block
   threshold = max(threshold, 1u);
   {
     const float least = value_of(threshold);
     uint32_t sent = 0;
     unsigned long long sent_mass = 0;
-    visit(0u, [&](float l, int token) {
-      total.add(weight(l));
-      if (l >= least && l > -INFINITY) {
-        const uint32_t at = atomicAdd(peer(&sh.listed, 0), 1u), mass = weight.fixed(l);
-        if (at < SHORT) {
-          *peer(&sh.list[at], 0) = rank_of(l, token);
-          *peer(&sh.list_mass[at], 0) = mass;
-        }
-        ++sent;
-        sent_mass += mass;
+    const auto send = [&](float l, int token) {
+      if (!(l >= least && l > -INFINITY)) return;
+      const uint32_t at = atomicAdd(peer(&sh.listed, 0), 1u), mass = weight.fixed(l);
+      if (at < SHORT) {
+        *peer(&sh.list[at], 0) = rank_of(l, token);
+        *peer(&sh.list_mass[at], 0) = mass;
       }
-    });
+      ++sent;
+      sent_mass += mass;
+    };
+    for (int i = tid; i < count; i += THREADS) {
+      const Piece<T> p(held[i]);
+      float most = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        total.add(weight.single ? pair(weight(p.v[e]), weight(p.v[e + 1])) : weight(pair(p.v[e], p.v[e + 1])));
+        most = fmaxf(most, fmaxf(p.v[e], p.v[e + 1]));
+      }
+      if (!(most >= least && most > -INFINITY)) continue;
+      const T* const held_tokens = reinterpret_cast<const T*>(held + i);
+      for (int e = 0; e < E; ++e) send(Piece<T>::one(held_tokens[e]), (from + i) * E - skew + e);
+    }
     double of_warp = total.value();
     sent = __reduce_add_sync(0xffffffffu, sent);
     for (int o = 16; o > 0; o >>= 1) {

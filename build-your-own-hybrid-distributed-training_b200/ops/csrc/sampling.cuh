@@ -25,6 +25,31 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+// Two floats in a register pair, on which one instruction works.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float x, float y) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ float low(Pair p) { return __uint_as_float((uint32_t)p); }
+__device__ __forceinline__ float high(Pair p) { return __uint_as_float((uint32_t)(p >> 32)); }
+__device__ __forceinline__ Pair plus(Pair x, Pair y) {
+  Pair p;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(p) : "l"(x), "l"(y));
+  return p;
+}
+__device__ __forceinline__ Pair times(Pair x, Pair y) {
+  Pair p;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(p) : "l"(x), "l"(y));
+  return p;
+}
+__device__ __forceinline__ Pair fma(Pair x, Pair y, Pair z) {
+  Pair p;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(x), "l"(y), "l"(z));
+  return p;
+}
+
 // w = 2^((l - best) log2(e) / T); the quotient is carried in two floats, since its rounding error times the distance
 // would show in the weights of unlikely tokens.
 struct Weights {
@@ -43,20 +68,25 @@ struct Weights {
     return fmaf(d, hi, fmaxf(d, least) * lo);
   }
   __device__ __forceinline__ float operator()(float l) const { return fast_exp2(exponent(l)); }
+  __device__ __forceinline__ Pair operator()(Pair l) const {  // the same, but not if `single`
+    const Pair d = plus(l, pair(-best, -best));
+    const Pair x = fma(d, pair(hi, hi), times(pair(fmaxf(low(d), least), fmaxf(high(d), least)), pair(lo, lo)));
+    return pair(fast_exp2(low(x)), fast_exp2(high(x)));
+  }
   __device__ __forceinline__ uint32_t fixed(float l) const { return (uint32_t)__float2uint_rn((*this)(l)*2147483648.f); }
 };
 
-// A sum of weights that comes out the same in every order (and so for every alignment of the row): multiples of 2^-16,
-// which a thread's few hundred terms add without rounding, and what they leave of each weight (at most 2^-17), whose
-// roundings lie far below the fp32 result.
-struct Sum {
-  float coarse = 0.f, fine = 0.f;
-  __device__ __forceinline__ void add(float w) {
-    const float near = __fadd_rn(__fadd_rn(w, 128.f), -128.f);
-    coarse += near;
-    fine += w - near;
+// A sum of weights, two at a time, that comes out the same in every order (and so for every alignment of the row): multiples
+// of 2^-16, which a thread's few hundred terms add without rounding, and what they leave of each weight (at most 2^-17),
+// whose roundings lie far below the fp32 result.
+struct Sums {
+  Pair coarse = pair(0.f, 0.f), fine = pair(0.f, 0.f);
+  __device__ __forceinline__ void add(Pair w) {
+    const Pair near = plus(plus(w, pair(128.f, 128.f)), pair(-128.f, -128.f));
+    coarse = plus(coarse, near);
+    fine = plus(fine, fma(near, pair(-1.f, -1.f), w));
   }
-  __device__ __forceinline__ double value() const { return (double)coarse + (double)fine; }
+  __device__ __forceinline__ double value() const { return ((double)low(coarse) + (double)high(coarse)) + (double)(low(fine) + high(fine)); }
 };
 
 template <int N = WARPS, typename V, typename Op>

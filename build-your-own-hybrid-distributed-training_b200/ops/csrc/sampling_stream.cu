@@ -25,31 +25,6 @@ constexpr int WIDTH = 1024, GROUPS = WIDTH / 32;  // threads and warps of a bloc
 constexpr int MOST_ROWS = 1024;  // of one block
 constexpr uint32_t NOBODY = 0xffffffffu;  // no token yet
 
-// Two floats in a register pair, on which one instruction works.
-using Pair = unsigned long long;
-__device__ __forceinline__ Pair pair(float x, float y) {
-  Pair p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
-  return p;
-}
-__device__ __forceinline__ float low(Pair p) { return __uint_as_float((uint32_t)p); }
-__device__ __forceinline__ float high(Pair p) { return __uint_as_float((uint32_t)(p >> 32)); }
-__device__ __forceinline__ Pair plus(Pair x, Pair y) {
-  Pair p;
-  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(p) : "l"(x), "l"(y));
-  return p;
-}
-__device__ __forceinline__ Pair times(Pair x, Pair y) {
-  Pair p;
-  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(p) : "l"(x), "l"(y));
-  return p;
-}
-__device__ __forceinline__ Pair fma(Pair x, Pair y, Pair z) {
-  Pair p;
-  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(x), "l"(y), "l"(z));
-  return p;
-}
-
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
