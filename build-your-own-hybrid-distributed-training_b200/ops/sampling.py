@@ -4,7 +4,7 @@
 distributed (``torch.empty(B, V).exponential_()``), the token with the largest ``weight / noise`` among
 those that the filters leave is a draw from their softmax.  The random numbers are the caller's, so a
 draw can be repeated, and no rounding of a long cumulative sum decides it.  The kernel is
-``csrc/sampling.cu``; the reference has no counterpart.
+``csrc/sampling.cu`` and ``csrc/sampling_stream.cu``; the reference has no counterpart.
 """
 
 from __future__ import annotations
