@@ -755,6 +755,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     // pieces with a token that stays; the random numbers of several are under way together
     constexpr int DEPTH = E == 4 ? 4 : 2;
     const bool together = (reinterpret_cast<uintptr_t>(noise - skew) % 16) == 0;
+    // number >= cut, without working the number out
+    const float lowest = value_of((uint32_t)(cut >> 32));
+    const int last = lowest == -INFINITY ? -1 : (int)min(0xffffffffu - (uint32_t)cut, 0x7fffffffu);
+    const auto stays = [&](float l, int token) { return l > lowest || (l == lowest && token <= last); };
     for (int i0 = tid; i0 < count; i0 += DEPTH * THREADS) {
       float luck[DEPTH][E];
       bool any[DEPTH];
@@ -765,7 +769,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
         if (i < count) {
           const Piece<T> p(held[i]);
 #pragma unroll
-          for (int e = 0; e < E; ++e) any[j] |= rank_of(p.v[e], first + e) >= cut;
+          for (int e = 0; e < E; ++e) any[j] |= stays(p.v[e], first + e);
         }
         if (!any[j]) continue;
         if (together && inside(i)) {
@@ -786,7 +790,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
         const Piece<T> p(held[i]);
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          if (rank_of(p.v[e], first + e) >= cut) enter(p.v[e], luck[j][e], (uint32_t)(first + e));
+          if (stays(p.v[e], first + e)) enter(p.v[e], luck[j][e], (uint32_t)(first + e));
       }
     }
   }

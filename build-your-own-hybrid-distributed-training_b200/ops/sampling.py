@@ -3,7 +3,7 @@
 ``sample_tokens`` draws by an exponential race: with ``noise`` independent and exponentially
 distributed (``torch.empty(B, V).exponential_()``), the token with the largest ``weight / noise`` among
 those that the filters leave is a draw from their softmax.  The random numbers are the caller's, so a
-draw can be repeated, and no rounding of a long cumulative sum decides it.  The kernel is
+draw can be repeated, and no rounding of a long cumulative sum decides it.  The kernels are
 ``csrc/sampling.cu`` and ``csrc/sampling_stream.cu``; the reference has no counterpart.
 """
 
