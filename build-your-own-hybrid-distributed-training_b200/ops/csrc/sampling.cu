@@ -97,6 +97,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   const bool greedy = !(temperature > 0.f);
   const int top_k = a.top_k[row];
   const float top_p = a.top_p[row], min_p = a.min_p[row];
+  // This launch may begin before the streaming one, whose results it does not read, has ended; it must not end before that one.
+  if (a.streamed && row == a.B - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (a.streamed && ordinary(temperature) && cuts_nothing(top_k, top_p, min_p, a.V)) return;
   const bool by_count = !greedy && top_k > 0 && top_k < a.V, by_mass = !greedy && !(top_p >= 1.f);
   const float* const noise = a.noise + row * a.noise_stride;
@@ -826,12 +828,14 @@ static cudaError_t launch_as(const Args& a, int blocks, cudaStream_t stream) {
   config.blockDim = dim3(THREADS);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  cudaLaunchAttribute cluster;
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = blocks;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  config.attrs = &cluster;
-  config.numAttrs = 1;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = blocks;
+  attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = a.streamed ? 2 : 1;
   return cudaLaunchKernelEx(&config, sample_kernel<T>, a);
 }
 
@@ -849,9 +853,10 @@ static int blocks_per_row(const Args& a, int sms) {
 // against 30.2.  With one wave (32 rows in fp32 15.6 against 11.6 us) or one block per row (512 rows of 32000 in bf16 32.0 against
 // 29.5, 1024 of 16384 in fp32 42 against 38.6) clusters are faster.
 // Where temperature or filters are per row, only the device knows which rows those are: both kernels are launched, and each
-// leaves the other's rows alone.  That pays from four blocks per row and two waves on: 256 rows of 128256 in fp32 58 us against 83,
-// 96 rows 30.7 against 34.1, 192 in bf16 39.9 against 44.3; 64 rows in fp32 25.0 against 23.1, 128 in bf16 32.0 against 30.2.
-// Batches that turn out to be cut lose the time of a launch (256 rows of top-k 1000: 168 -> 172 us).
+// leaves the other's rows alone; the second begins as SMs get free (256 rows of 128256 in fp32: 54.7 us, 58 after the first's end).
+// That pays from four blocks per row and two waves on: those 256 rows 54.7 us against 83, 96 rows 27.9 against 34.1, 192 in bf16
+// 37.5 against 44.3; 64 rows in fp32 24.1 against 23.1, 128 in bf16 31.1 against 30.2.  Batches that turn out to be cut lose the
+// time of a launch (256 rows of top-k 1000: 165 -> 170 us).
 static bool whole_stream(const Args& a) {
   if (a.temperature.rows != nullptr) return false;
   if (a.temperature.same <= 0.f) return true;

@@ -84,6 +84,7 @@ stream_kernel(const __grid_constant__ Args a, int pieces /* of a row's share of 
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
 
+  if constexpr (!WHOLE) asm volatile("griddepcontrol.launch_dependents;");  // the launch for the other rows takes SMs as they get free
   if (tid == 0) sh.count = 0;
   int rows = a.B;
   if constexpr (!WHOLE) {  // list this kernel's rows
