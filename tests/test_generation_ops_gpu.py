@@ -547,6 +547,32 @@ def test_sample_tokens_many_rows_on_streams_and_in_graphs() -> None:
     assert all(torch.equal(g, w) for gs, ws in zip(got, want, strict=True) for g, w in zip(gs, ws, strict=True))
 
 
+def test_sample_tokens_many_rows_with_values_per_row_in_stream_order() -> None:
+    """Two launches share such a batch: what follows them on the stream, or in a graph, finds both ended."""
+    b, v = 160, 50257
+    logits, noise = _logits(b, v, torch.float32, seed=31)
+    rows = torch.arange(b, device="cuda")
+    for cut in (rows < 0, rows % 2 == 0, rows == b - 1, rows == 0, rows < b - 1, rows >= 0):
+        top_k = torch.where(cut, 40, 0).to(torch.int32)
+        want = [x.clone() for x in ops.sample_tokens(logits, noise, top_k=top_k)]
+        assert torch.equal(want[0], ops.reference_sample_tokens(logits, noise, 1.0, top_k, 1.0, 0.0, compute_dtype=torch.float64)[0])
+        values = torch.empty_like(logits)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            values.copy_(logits)
+            got = ops.sample_tokens(values, noise, top_k=top_k)
+            copies = [x.clone() for x in got]
+            values.fill_(-math.inf)
+        for _ in range(3):
+            graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(copies, want, strict=True))
+        for _ in range(3):
+            values.copy_(logits)
+            got = ops.sample_tokens(values, noise, top_k=top_k)
+            values.fill_(math.nan)
+            assert all(torch.equal(x, y) for x, y in zip(got, want, strict=True))
+
+
 # --------------------------------------------------------------------------- refusals
 
 
