@@ -17,15 +17,21 @@
 //   cp.async; warps never wait for one another before their range is done.
 // * Matrix instructions.  S = Q K^T and O += P V have the 8 heads as rows 0-7 of a tile of 16 rows, the smallest
 //   there is: at these intensities the tensor pipe is far from its limit.  Rows 8-15 are not wasted; they carry
-//   what rounding left over of the same heads' operand.  In bf16 (m16n8k16) P enters as two bf16 terms.  The
-//   dimensions of q and k are summed in the order in which 16-byte loads deliver them, and the tokens of a tile in
+//   what rounding left over of the same heads' operand.  P enters with the 24 bits of an fp32 weight, as three bf16 terms or
+//   four digits of 8 bits, since two of either would move one bf16 output in 600 (bf16) or 60 (int8) to its neighbour.  Where a row
+//   has at most 4 heads the third (and fourth) go to rows 4-7 (and 12-15), whose lanes repeat the scores of rows 0-3: no
+//   further instruction (32 x 4096 bf16 at 32/8 heads 92.2 us, with two terms 91.8; 48 ragged GPT-2 rows 23.8 and 23.4).  With 5
+//   to 8 heads they take a second instruction (32 x 4096 at 32/4 heads: bf16 53.0 and 51.9 us, int8 41.2 and 37.1).
+//   The dimensions of q and k are summed in the order in which 16-byte loads deliver them, and the tokens of a tile in
 //   the order in which score accumulators and the second product's operand agree: no data is moved for either.
 // * 8 bits.  Keys enter the instructions (m16n8k32) as they are held, so q has to be in 8 bits too, as digits, worked
 //   out once per row.  int8: q of a head, scaled by a power of two and rounded to 22 bits, is three signed digits, and
-//   the sums are exact integers (below 2^22, read as floats by starting the accumulators at the bits of 1.5 2^23).
+//   the sums are exact integers (below 2^22, read as floats by starting the accumulators at the bits of 1.5 2^23).  The
+//   third digit has rows 4-7 of at most 4 heads, or a second instruction; with the former 128 x 4097..8192 at 32/8
+//   heads take 272 us, with the latter 293.
 //   e4m3: q is two terms of 4 bits each, which hold all 8 bits of a bf16.  int8 values are used as they are as well,
-//   with rint(65535 p) as two unsigned digits: p is taken relative to the tile's own maximum, so that its digits always
-//   start at the tile's largest weight, and the tile's product is added to the output in fp32.  e4m3 values are
+//   with floor(2^32 p) as four unsigned digits: p is taken relative to the tile's own maximum, so that its
+//   digits always start at the tile's largest weight, and the tile's product is added to the output in fp32.  e4m3 values are
 //   converted to fp16 pairs (one conversion costs what a byte permute does; three e4m3 terms of p per token
 //   cost more: 82 us against 71 on 32 rows of 4096).
 //   A token's key scale multiplies its score.  Its value scale sv joins the exponent: with s'_t = s_t + log2(sv_t) and
@@ -123,6 +129,8 @@ __device__ __forceinline__ void mma_int8(int* c, uint32_t a0, uint32_t a1, uint3
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+
+constexpr float WEIGHT = 4294967040.f;  // the largest float below 2^32: what an int8 tile's largest weight is held as
 
 // An integer accumulator that starts at these bits is, read as a float, 1.5 2^23 plus the sum (below 2^22 in magnitude).
 constexpr int ZERO_BITS = 0x4b400000;
@@ -222,7 +230,8 @@ __device__ __forceinline__ float load(const float* p) {
   return v;
 }
 
-template <int F, int D>
+// TWIN: rows of at most 4 heads (not of e4m3).
+template <int F, int D, bool TWIN>
 __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const __grid_constant__ Args a) {
   using S = Shape<F, D>;
   constexpr int TOK = S::TOK, GROUPS = TOK / 16, NT = D / 8, WARPS = S::WARPS;
@@ -325,6 +334,9 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
   }
   unsigned char* const ring = rings + warp * S::STAGES * S::STAGE;
   const uint32_t ring_addr = smem_addr(ring);
+  // Lanes g >= 4 work out head g - 4 once more, and their rows of the second product's operand take the last of the weights'
+  // three terms.
+  const bool last_term = TWIN && g >= HEADS / 2;  // (of int8: the last two of four)
   [[maybe_unused]] float4* const factors = reinterpret_cast<float4*>(pieces + WARPS * S::PIECE + warp * S::FACTORS);
 
   if (count > 0) {
@@ -392,7 +404,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
     const Cursor ahead = next_window(load);
 
     // Per row: q as fragments of the first operand, the output's accumulators, and the softmax's state.
-    constexpr int DIGITS = F == kv::kInt8 ? 3 : 2;  // 8 bits: of q
+    constexpr int DIGITS = F == kv::kInt8 && !TWIN ? 3 : 2;  // 8 bits: of q, in one lane
     constexpr int QR = F == kv::kBf16 ? D / 8 : DIGITS * (D / 16);
     uint32_t q[QR];
     constexpr int PLACES = F == kv::kInt8 ? 2 : 4;  // of an accumulator; int8 adds up tiles in fp32 itself
@@ -420,7 +432,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
           o[t][0] = o[t][1] = 0.f;
           if constexpr (PLACES == 4) o[t][2] = o[t][3] = 0.f;
         }
-        const int kv_head = kv_head_of(use.row), in_group = (use.row - kv_head * chunks) * HEADS + g;
+        const int kv_head = kv_head_of(use.row), in_group = (use.row - kv_head * chunks) * HEADS + (last_term ? g - HEADS / 2 : g);
         const bool real = in_group < group;
         const __nv_bfloat16* src = a.q + use.b * a.q_seq + ((long long)kv_head * group + in_group) * a.q_head;
         // lane (g, c4) holds, of head g, the 16-byte pieces of a key row that it will load: piece 4 j + c4
@@ -461,9 +473,15 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
               uint32_t y[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) y[e] = (uint32_t)(__float2int_rn(x[4 * r + e] * down) + 0x808080);
-              q[3 * r] = gather_bytes<2>(y[0], y[1], y[2], y[3]) ^ 0x80808080u;
-              q[3 * r + 1] = gather_bytes<1>(y[0], y[1], y[2], y[3]) ^ 0x80808080u;
-              q[3 * r + 2] = gather_bytes<0>(y[0], y[1], y[2], y[3]) ^ 0x80808080u;
+              const uint32_t d0 = gather_bytes<2>(y[0], y[1], y[2], y[3]) ^ 0x80808080u;
+              const uint32_t d1 = gather_bytes<1>(y[0], y[1], y[2], y[3]) ^ 0x80808080u;
+              const uint32_t d2 = gather_bytes<0>(y[0], y[1], y[2], y[3]) ^ 0x80808080u;
+              if constexpr (TWIN) {
+                q[2 * r] = last_term ? d2 : d0;
+                q[2 * r + 1] = last_term ? 0u : d1;
+              } else {
+                q[3 * r] = d0, q[3 * r + 1] = d1, q[3 * r + 2] = d2;
+              }
             } else {
               float y[4] = {x[4 * r] * down, x[4 * r + 1] * down, x[4 * r + 2] * down, x[4 * r + 3] * down};
               q[2 * r] = take_digit(y);
@@ -534,16 +552,19 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
             s[t][e] = fast_exp2(s[t][e] - at);
             sum += s[t][e];
           }
-        // o += p v, the rounding's remainder of p in rows 8 to 15
+        // o += p v, the rounding's remainder of p in rows 8 to 15, what its rounding left in rows 4 to 7 or in a second product
 #pragma unroll
         for (int kk = 0; kk < GROUPS; ++kk) {
-          uint32_t hi[2], lo[2];
+          uint32_t hi[2], lo[2], rest[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float x = s[2 * kk + h][0], y = s[2 * kk + h][1];
             hi[h] = pack_bf16(x, y);
             const float2 back = unpack_bf16(hi[h]);
             lo[h] = pack_bf16(x - back.x, y - back.y);
+            const float2 more = unpack_bf16(lo[h]);
+            rest[h] = pack_bf16(x - back.x - more.x, y - back.y - more.y);
+            if (last_term) hi[h] = rest[h], lo[h] = 0u;
           }
           const int mat = lane / 8, r = kk * 16 + (mat & 1) * 8 + (lane & 7);
           const uint32_t row = vb + r * S::ROW;
@@ -553,6 +574,10 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
             ldmatrix4t(v, row + (((2 * np + (mat >> 1)) ^ (r & 7)) * 16));
             mma_bf16(o[2 * np], hi[0], lo[0], hi[1], lo[1], v[0], v[1]);
             mma_bf16(o[2 * np + 1], hi[0], lo[0], hi[1], lo[1], v[2], v[3]);
+            if constexpr (!TWIN) {
+              mma_bf16(o[2 * np], rest[0], 0u, rest[1], 0u, v[0], v[1]);
+              mma_bf16(o[2 * np + 1], rest[0], 0u, rest[1], 0u, v[2], v[3]);
+            }
           }
         }
       } else {
@@ -564,7 +589,21 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
 #pragma unroll
         for (int i = 0; i < TOK / 8; ++i) {
           const uint32_t row = kb + (place(i) + 4 * (g >> 1) + (g & 1)) * S::ROW;
-          if constexpr (F == kv::kInt8) {
+          if constexpr (F == kv::kInt8 && TWIN) {
+            int x[4] = {ZERO_BITS, ZERO_BITS, ZERO_BITS, ZERO_BITS};
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) {
+              const uint4 k = lds128(row + ((D == 128 ? (j * 4 + c4) ^ ((g & 1) << 2) : c4) * 16));
+              const uint32_t* d = q + 8 * j;
+              mma_int8<true>(x, d[0], d[1], d[2], d[3], k.x, k.y);
+              mma_int8<true>(x, d[4], d[5], d[6], d[7], k.z, k.w);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float part = fmaf(sum_of(x[e]), last_term ? 1.f : 65536.f, 256.f * sum_of(x[e + 2]));  // (no second digit in the latter)
+              s[i][e] = part + __shfl_xor_sync(0xffffffffu, part, 16);
+            }
+          } else if constexpr (F == kv::kInt8) {
             int x[4] = {ZERO_BITS, ZERO_BITS, ZERO_BITS, ZERO_BITS}, y[4] = {ZERO_BITS, ZERO_BITS, ZERO_BITS, ZERO_BITS};
 #pragma unroll
             for (int j = 0; j < D / 64; ++j) {
@@ -632,24 +671,29 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
           const float at = top == -INFINITY ? 0.f : top;  // of this tile
           const float share = fast_exp2(top - now);       // of the tile's weights
           float tile_sum = 0.f;
-          uint32_t p[BLOCKS][2][2];  // digits of the weights of tokens 4 c4 ... and 16 + 4 c4 ...
+          uint32_t p[BLOCKS][2][4];  // digits of the weights of tokens 4 c4 ... and 16 + 4 c4 ..., which a TWIN lane has two of
 #pragma unroll
           for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              uint32_t y[4];  // 2^23 + rint(65535 p): the low bytes are the digits
+              uint32_t y[4];  // bytes are the digits
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int i = 4 * b + 2 * h + e / 2;
                 const float x = fast_exp2(s[i][e % 2] - at);
                 tile_sum = fmaf(x, inv[i][e % 2], tile_sum);
-                y[e] = __float_as_uint(fmaf(x, 65535.f, 8388608.f));
+                y[e] = __float2uint_rz(x * WEIGHT);
               }
-              p[b][h][0] = gather_bytes<1>(y[0], y[1], y[2], y[3]);
-              p[b][h][1] = gather_bytes<0>(y[0], y[1], y[2], y[3]);
+              const auto take = [&](uint32_t pick, uint32_t& higher, uint32_t& lower) {  // two neighbouring bytes of each
+                const uint32_t y01 = __byte_perm(y[0], y[1], pick), y23 = __byte_perm(y[2], y[3], pick);
+                higher = __byte_perm(y01, y23, 0x7632);
+                lower = __byte_perm(y01, y23, 0x5410);
+              };
+              take(last_term ? 0x5140 : 0x7362, p[b][h][0], p[b][h][1]);
+              if constexpr (!TWIN) take(0x5140, p[b][h][2], p[b][h][3]);
             }
           sum = fmaf(share, tile_sum, sum);
-          const float first = share * (256.f / 65535.f), second = share * (1.f / 65535.f);
+          const float unit = share * (1.f / WEIGHT), second = last_term ? unit : 65536.f * unit, first = 256.f * second;
 #pragma unroll
           for (int y = 0; y < WORDS; ++y) {
             uint32_t v[BLOCKS][2][4];  // four tokens' bytes of each of four dimensions
@@ -672,6 +716,13 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
               for (int b = 0; b < BLOCKS; ++b) mma_int8<false>(x, p[b][0][0], p[b][0][1], p[b][1][0], p[b][1][1], v[b][0][z], v[b][1][z]);
 #pragma unroll
               for (int e = 0; e < 2; ++e) o[4 * y + z][e] = fmaf(sum_of(x[e]), first, fmaf(sum_of(x[e + 2]), second, o[4 * y + z][e]));
+              if constexpr (!TWIN) {
+                x[0] = x[1] = x[2] = x[3] = ZERO_BITS;
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) mma_int8<false>(x, p[b][0][2], p[b][0][3], p[b][1][2], p[b][1][3], v[b][0][z], v[b][1][z]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) o[4 * y + z][e] = fmaf(fmaf(sum_of(x[e]), 256.f, sum_of(x[e + 2])), unit, o[4 * y + z][e]);
+              }
             }
           }
         } else {
@@ -709,10 +760,14 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
       if (row_ends || last) {
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        const auto value = [&](int t, int e) {
-          if constexpr (PLACES == 4) return o[t][e] + o[t][e + 2];
-          else return o[t][e];
-        };
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if constexpr (PLACES == 4) o[t][e] += o[t][e + 2];
+            if constexpr (TWIN) o[t][e] += __shfl_xor_sync(0xffffffffu, o[t][e], 16);
+          }
+        const auto value = [&](int t, int e) { return o[t][e]; };
         // where accumulator column n of tile t lies in the head's dimensions
         const auto dim = [&](int t, int e) { return F == kv::kBf16 ? t * 8 + 2 * c4 + e : (2 * c4 + e) * NT + t; };
         if (row_ends && row_tile == 0) {
@@ -890,7 +945,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
 long long workspace_floats(int sms) { return (long long)sms * 2 * HEADS * (128 + 2); }
 int workspace_counters(int sms) { return sms; }
 
-template <int F, int D>
+template <int F, int D, bool TWIN>
 static cudaError_t launch_as(const Args& a, int sms, cudaStream_t stream) {
   using S = Shape<F, D>;
   // dynamic shared memory beyond 48 KB is opted into once per device
@@ -900,17 +955,21 @@ static cudaError_t launch_as(const Args& a, int sms, cudaStream_t stream) {
   if (err != cudaSuccess) return err;
   const unsigned long long bit = 1ull << (device & 63);
   if (!(__atomic_load_n(&opted, __ATOMIC_ACQUIRE) & bit)) {
-    err = cudaFuncSetAttribute(decode_kernel<F, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    err = cudaFuncSetAttribute(decode_kernel<F, D, TWIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (err != cudaSuccess) return err;
     __atomic_fetch_or(&opted, bit, __ATOMIC_RELEASE);
   }
-  decode_kernel<F, D><<<sms, S::THREADS, S::SMEM, stream>>>(a);
+  decode_kernel<F, D, TWIN><<<sms, S::THREADS, S::SMEM, stream>>>(a);
   return cudaGetLastError();
 }
 
 cudaError_t launch(const Args& a, int sms, cudaStream_t stream) {
   cudaError_t err = cudaSuccess;
-  kv::by_format(a.pool, [&](auto f, auto d) { err = launch_as<decltype(f)::value, decltype(d)::value>(a, sms, stream); });
+  kv::by_format(a.pool, [&](auto f, auto d) {
+    constexpr int F = decltype(f)::value, D = decltype(d)::value;
+    if (F != kv::kFp8 && a.H / a.pool.Hkv <= HEADS / 2) err = launch_as<F, D, F != kv::kFp8>(a, sms, stream);
+    else err = launch_as<F, D, false>(a, sms, stream);
+  });
   return err;
 }
 

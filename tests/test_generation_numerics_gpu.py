@@ -1,0 +1,63 @@
+"""How many bits the text-generation kernels carry, and over which magnitudes, against plain statements in 64 bits.
+
+Outputs are bf16, whose rounding hides what a kernel keeps of its weights.  The inputs here cancel, so that the result is small
+next to what was summed and its rounding small as well.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import hybrid_training.ops as ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _one_page_each(b: int, kvh: int, d: int, dtype: torch.dtype) -> tuple[ops.KVPages, torch.Tensor]:
+    """A pool of zeros with one page of 16 tokens for each of ``b`` sequences, and its block table."""
+    pages = ops.KVPages.allocate(b, kvh, 16, d, dtype=dtype, device="cuda")
+    for x in (pages.k, pages.v):
+        x.view(torch.uint8).zero_()
+    return pages, torch.arange(b, dtype=torch.int32, device="cuda")[:, None].contiguous()
+
+
+def _check(q, pages, table, n, scale, relative: float) -> None:
+    """Each output within one rounding to bf16 and ``relative`` of the average magnitude that was summed for it."""
+    got = ops.paged_attention(q, pages, table, n, scale=scale)
+    want = ops.reference_paged_attention(q, pages, table, n, scale=scale, compute_dtype=torch.float64)[0]
+    v = pages.v if pages.v_scale is not None else pages.v.abs()
+    magnitudes = ops.KVPages(pages.k, v if v.dtype == torch.bfloat16 else v.float().abs().to(v.dtype), pages.k_scale, pages.v_scale)
+    summed = ops.reference_paged_attention(q, magnitudes, table, n, scale=scale, compute_dtype=torch.float64)[0]
+    excess = (got.double() - want).abs() - 2.0**-8 * want.abs() - relative * summed
+    assert bool((excess <= 0).all()), float((excess / summed).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.int8])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kvh", [(1, 1), (8, 2), (10, 2), (8, 1), (12, 1)])
+def test_paged_attention_carries_weights_in_full(dtype, d, heads, kvh) -> None:
+    """A token of weight 1 against fifteen of weight 2^-a, whose values cancel it.
+
+    The exponential is right to 2^-22 and a, up to 8, to 2^-24 of itself: 2^-21 of the weight, on half of what is summed.
+    Weights of 16 bits (relative to the largest: 2^-17, to their own magnitude: 2^-18) show at several times the 2^-20 allowed.
+    """
+    b = 64
+    pages, table = _one_page_each(b, kvh, d, dtype)
+    a = 4.0 + 4.0 * torch.rand(b, kvh, device="cuda", generator=torch.Generator(device="cuda").manual_seed(d + heads))
+    if dtype == torch.bfloat16:
+        a = a.bfloat16().float()
+        pages.k[:, :, 1:, 0] = -a[..., None].bfloat16()
+    else:
+        pages.k[:, :, 1:, 0] = -1
+        pages.k_scale.copy_(a[..., None].expand(b, kvh, 16))
+        pages.v_scale.fill_(1.0)
+    c = 127.0 - torch.arange(d, device="cuda") % 64
+    pages.v[:, :, 1:] = -c.to(dtype)
+    pages.v[:, :, 0] = torch.round(15.0 * c * torch.exp2(-a)[..., None]).to(dtype)
+    q = torch.zeros(b, heads, d, device="cuda", dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    n = torch.full((b,), 16, dtype=torch.int32, device="cuda")
+    _check(q, pages, table, n, math.log(2.0), 2.0**-20)
