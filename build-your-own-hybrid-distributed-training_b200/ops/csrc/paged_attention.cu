@@ -30,13 +30,14 @@
 //   third digit has rows 4-7 of at most 4 heads, or a second instruction; with the former 128 x 4097..8192 at 32/8
 //   heads take 272 us, with the latter 293.
 //   e4m3: q is two terms of 4 bits each, which hold all 8 bits of a bf16.  int8 values are used as they are as well,
-//   with floor(2^32 p) as four unsigned digits: p is taken relative to the tile's own maximum, so that its
+//   with floor(2^31 p) as four unsigned digits: p is taken relative to the tile's own maximum, so that its
 //   digits always start at the tile's largest weight, and the tile's product is added to the output in fp32.  e4m3 values are
 //   converted to fp16 pairs (one conversion costs what a byte permute does; three e4m3 terms of p per token
 //   cost more: 82 us against 71 on 32 rows of 4096).
-//   A token's key scale multiplies its score.  Its value scale sv joins the exponent: with s'_t = s_t + log2(sv_t) and
-//   m the maximum of s', p_t = 2^(s'_t - m) <= 1, the output is sum p_t v_t / sum (p_t / sv_t): p stays in range
-//   whatever the scales are.
+//   A token's key scale multiplies its score.  Of its value scale sv = 2^n f, 1 <= f < 2, the power of two joins the
+//   exponent: with s'_t = s_t + n_t, m the maximum of s' rounded up and x_t = 2^(s'_t - m) <= 1, the output is
+//   sum (x_t f_t) v_t / sum (x_t 2^-n_t): weights stay in range whatever the scales are, and nothing is rounded for it.
+// * References m are whole numbers, in all formats: factors between them are powers of two and round nothing.
 // * Joining.  A row inside one warp's range is finished by that warp.  Otherwise warps leave (o, m, sum)
 //   in shared memory, the block merges neighbours, and rows that cross blocks go through a workspace:
 //   the block that arrives last merges the pieces in the order of the tokens, so results do not depend
@@ -130,8 +131,6 @@ __device__ __forceinline__ void mma_int8(int* c, uint32_t a0, uint32_t a1, uint3
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-constexpr float WEIGHT = 4294967040.f;  // the largest float below 2^32: what an int8 tile's largest weight is held as
-
 // An integer accumulator that starts at these bits is, read as a float, 1.5 2^23 plus the sum (below 2^22 in magnitude).
 constexpr int ZERO_BITS = 0x4b400000;
 __device__ __forceinline__ float sum_of(int bits) { return __fadd_rn(__int_as_float(bits), -12582912.f); }
@@ -185,6 +184,14 @@ __device__ __forceinline__ float fast_log2(float x) {
   return y;
 }
 
+// log(2^m sum).  The power of two of the sum joins m, so that the logarithm is that of a number between 1 and 2.  Without a
+// token m is -inf; a sum that is NaN stays so.
+__device__ __forceinline__ float lse_of(float m, float sum) {
+  const uint32_t u = __float_as_uint(sum);
+  const float mantissa = __uint_as_float((u & 0x007fffffu) | 0x3f800000u);
+  return fmaf(sum, 0.f, m + (float)((int)(u >> 23) - 127) + fast_log2(mantissa)) * LN2;
+}
+
 // A place on the line of tiles.  `rows` counts the rows of one sequence.
 struct Cursor {
   int b, row, tile, tiles, n;
@@ -235,6 +242,7 @@ template <int F, int D, bool TWIN>
 __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const __grid_constant__ Args a) {
   using S = Shape<F, D>;
   constexpr int TOK = S::TOK, GROUPS = TOK / 16, NT = D / 8, WARPS = S::WARPS;
+  constexpr uint32_t UNIT = F == kv::kInt8 ? 0x4f000000u : 0x3f800000u;  // what a weight of 1 is held as, 2^31 or 1, in bits
   extern __shared__ __align__(16) unsigned char smem[];
   struct Meta {
     int item;  // first tile of the row on the line
@@ -500,15 +508,19 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
       const uint32_t in_pool = held >> (4 * stage);
       [[maybe_unused]] const float* const stage_scales = reinterpret_cast<const float*>(ring + stage * S::STAGE + 2 * S::DATA);
 
-      // 8 bits: one lane per token works out what its scales do.  A scale of zero (none that kv_cache_write leaves) counts as
-      // the smallest one, NaN stays NaN; masked tokens get a finite score factor and an exponent of -inf.
+      // 8 bits: one lane per token works out what its scales do.  A value scale below the smallest that kv_cache_write leaves
+      // counts as that one; one of 2^127 or more (it leaves at most 2^128 / 127) counts as NaN, which NaN and infinities stay.
+      // Masked tokens get a finite score factor and an exponent of -inf.
       if constexpr (F != kv::kBf16) {
 #pragma unroll
         for (int i = lane; i < TOK; i += 32) {
           const bool real = ((in_pool >> (i / 16)) & 1u) && use.tile * TOK + i < use.n;
           const float ks = stage_scales[i], raw = stage_scales[TOK + i];
           const float vs = raw < kv::kMinScale ? kv::kMinScale : raw;
-          factors[i] = real ? make_float4(ks * a.scale_log2, fast_log2(vs), __fdividef(1.f, vs), 0.f) : make_float4(0.f, -INFINITY, 0.f, 0.f);
+          const uint32_t u = __float_as_uint(vs);  // 2^n f
+          const float n = vs < 0x1p127f ? __uint_as_float(0x4b000000u | (u >> 23)) - (8388608.f + 127.f) : __int_as_float(0x7fc00000);
+          factors[i] = make_float4(real ? ks * a.scale_log2 : 0.f, real ? n : -INFINITY, real ? __uint_as_float(0x7f000000u - (u & 0x7f800000u)) : 0.f,
+                                   __uint_as_float((u & 0x007fffffu) | UNIT));
         }
         __syncwarp();
       }
@@ -536,7 +548,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float higher = fmaxf(m, top);
+        const float higher = fmaxf(m, ceilf(top));
         const float at = higher == -INFINITY ? 0.f : higher;  // nothing but masked tokens so far
         if (__any_sync(0xffffffffu, higher > m)) {
           const float keep = fast_exp2(m - at);
@@ -629,7 +641,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
             for (int e = 0; e < 2; ++e) s[i][e] = fmaf(x[e + 2], 0.0625f, x[e]);
           }
         }
-        float inv[TOK / 8][2], top = -INFINITY;
+        float inv[TOK / 8][2], rest[TOK / 8][2], top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < TOK / 8; ++i)
 #pragma unroll
@@ -637,10 +649,11 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
             const float4 f = factors[place(i) + 4 * c4 + e];
             s[i][e] = fmaf(s[i][e] * up, f.x, f.y);
             inv[i][e] = f.z;
+            rest[i][e] = f.w;
             top = fmaxf(top, s[i][e]);
           }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        top = ceilf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)));
         const float higher = fmaxf(m, top), now = higher == -INFINITY ? 0.f : higher;  // nothing but masked tokens so far
         if (__any_sync(0xffffffffu, higher > m)) {
           const float keep = fast_exp2(m - now);
@@ -682,7 +695,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
                 const int i = 4 * b + 2 * h + e / 2;
                 const float x = fast_exp2(s[i][e % 2] - at);
                 tile_sum = fmaf(x, inv[i][e % 2], tile_sum);
-                y[e] = __float2uint_rz(x * WEIGHT);
+                y[e] = __float2uint_rz(x * rest[i][e % 2]);
               }
               const auto take = [&](uint32_t pick, uint32_t& higher, uint32_t& lower) {  // two neighbouring bytes of each
                 const uint32_t y01 = __byte_perm(y[0], y[1], pick), y23 = __byte_perm(y[2], y[3], pick);
@@ -693,7 +706,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
               if constexpr (!TWIN) take(0x5140, p[b][h][2], p[b][h][3]);
             }
           sum = fmaf(share, tile_sum, sum);
-          const float unit = share * (1.f / WEIGHT), second = last_term ? unit : 65536.f * unit, first = 256.f * second;
+          const float unit = share * 0x1p-31f, second = last_term ? unit : 65536.f * unit, first = 256.f * second;
 #pragma unroll
           for (int y = 0; y < WORDS; ++y) {
             uint32_t v[BLOCKS][2][4];  // four tokens' bytes of each of four dimensions
@@ -737,9 +750,10 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
                 const int i = 4 * b + 2 * h + e;
                 const float x = fast_exp2(s[i][0] - now), y = fast_exp2(s[i][1] - now);
                 sum = fmaf(x, inv[i][0], fmaf(y, inv[i][1], sum));
-                hi[e] = pack_half(x, y);
+                const float px = x * rest[i][0], py = y * rest[i][1];
+                hi[e] = pack_half(px, py);
                 const float2 back = unpack_half(hi[e]);
-                lo[e] = pack_half(x - back.x, y - back.y);
+                lo[e] = pack_half(px - back.x, py - back.y);
               }
 #pragma unroll
               for (int y = 0; y < WORDS; ++y) {
@@ -792,7 +806,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
                   *reinterpret_cast<uint4*>(dst + dim(t, e)) = make_uint4(x[0], x[1], x[2], x[3]);
                 }
             }
-            if (a.lse != nullptr && c4 == 0) a.lse[head] = sum == 0.f ? -INFINITY : (m + fast_log2(sum)) * LN2;
+            if (a.lse != nullptr && c4 == 0) a.lse[head] = lse_of(m, sum);
           }
         } else {
           // A piece of a row.  One of the warp's first row goes to a place of its own, one of a later row ends the
@@ -897,7 +911,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
           const int v = v0 + y, d = F == kv::kBf16 ? (v >> 1) * 8 + 2 * c4 + (v & 1) : (2 * c4 + (v & 1)) * NT + (v >> 1);
           a.out[head * D + d] = __float2bfloat16_rn(x[y] * norm);
         }
-        if (a.lse != nullptr && v0 == 0 && c4 == 0) a.lse[head] = total == 0.f ? -INFINITY : (top + fast_log2(total)) * LN2;
+        if (a.lse != nullptr && v0 == 0 && c4 == 0) a.lse[head] = lse_of(top, total);
       } else {
         float* const out = a.partial + ((long long)blockIdx.x * 2 + (job.begins ? 1 : 0)) * STEP;
 #pragma unroll

@@ -61,3 +61,50 @@ def test_paged_attention_carries_weights_in_full(dtype, d, heads, kvh) -> None:
     q[..., 0] = 1.0
     n = torch.full((b,), 16, dtype=torch.int32, device="cuda")
     _check(q, pages, table, n, math.log(2.0), 2.0**-20)
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("heads,kvh", [(4, 1), (8, 1)])
+def test_paged_attention_value_scales_round_nothing(dtype, heads, kvh) -> None:
+    """Two tokens of equal scores, whose values cancel through unequal scales.
+
+    Equal scores have weights that are powers of two times a scale: two terms of fp16 or digits leave 2^-22 of one of them, so
+    2^-21 allows for twice that.  A logarithm of the scale that joins the exponent would leave 2^-22 of its own magnitude, five
+    times that.
+    """
+    b, d = 512, 64
+    pages, table = _one_page_each(b, kvh, d, dtype)
+    gen = torch.Generator(device="cuda").manual_seed(heads)
+    first = torch.exp2(-3.0 - 20.0 * torch.rand(b, kvh, device="cuda", generator=gen))
+    c = torch.tensor([64.0, 96.0, 112.0, 72.0], device="cuda").repeat(d // 4)
+    pages.v[:, :, 0] = c.to(dtype)
+    pages.v[:, :, 1] = (-(c / 2)).to(dtype)
+    pages.k_scale.fill_(1.0)
+    pages.v_scale[:, :, 0] = first
+    pages.v_scale[:, :, 1] = 2.0 * first * (1.0 + 1e-6 * torch.randn(b, kvh, device="cuda", generator=gen))
+    # the cancelling partner at another power of two and mantissa: a third token takes part of the second's share
+    part = torch.rand(b, kvh, device="cuda", generator=gen)
+    pages.v[:, :, 2] = pages.v[:, :, 1]
+    pages.v_scale[:, :, 2] = pages.v_scale[:, :, 1] * part
+    pages.v_scale[:, :, 1] = pages.v_scale[:, :, 1] * (1.0 - part)
+    q = torch.zeros(b, heads, d, device="cuda", dtype=torch.bfloat16)
+    n = torch.full((b,), 3, dtype=torch.int32, device="cuda")
+    _check(q, pages, table, n, 1.0, 2.0**-21)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("length", [5, 900])
+def test_paged_attention_what_is_not_a_number_stays_so(dtype, length) -> None:
+    """A NaN in a query, a key or a value reaches that head's output, and in a query or a key its log-sum-exp; no other head's."""
+    pages = ops.KVPages.allocate(64, 3, 16, 64, dtype=dtype, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(1024, 3, 64, device="cuda", generator=gen).bfloat16() for _ in range(2))
+    k[3, 1, 5] = math.nan
+    v[4, 2, 7] = math.nan
+    ops.kv_cache_write(pages, k, v, torch.arange(1024, device="cuda"))
+    q = torch.randn(1, 6, 64, device="cuda", generator=gen).bfloat16()
+    q[0, 1, 9] = math.nan
+    table, n = torch.arange(64, dtype=torch.int32, device="cuda")[None].contiguous(), torch.tensor([length], dtype=torch.int32, device="cuda")
+    out, lse = ops.paged_attention(q, pages, table, n, return_lse=True)
+    assert torch.isnan(out[0]).any(-1).tolist() == [False, True, True, True, True, True]
+    assert torch.isnan(lse[0, :4]).tolist() == [False, True, True, True]
