@@ -173,6 +173,12 @@ __device__ __forceinline__ uint32_t half_pair(uint32_t x) {
 }
 __device__ __forceinline__ float2 unpack_bf16(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
 
+// A product that takes numbers below 2^-126 as they are, which the build's fast arithmetic does not.
+__device__ __forceinline__ float times(float x, float y) {
+  float z;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -242,6 +248,9 @@ template <int F, int D, bool TWIN>
 __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const __grid_constant__ Args a) {
   using S = Shape<F, D>;
   constexpr int TOK = S::TOK, GROUPS = TOK / 16, NT = D / 8, WARPS = S::WARPS;
+  // Scores are in units of 2^SHIFT times the key's scale (at most 2^128 / 127) until that multiplies them: digits of the largest
+  // queries are sums up to 2^37 before it does.
+  constexpr int SHIFT = 6;
   constexpr uint32_t UNIT = F == kv::kInt8 ? 0x4f000000u : 0x3f800000u;  // what a weight of 1 is held as, 2^31 or 1, in bits
   extern __shared__ __align__(16) unsigned char smem[];
   struct Meta {
@@ -416,7 +425,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
     constexpr int QR = F == kv::kBf16 ? D / 8 : DIGITS * (D / 16);
     uint32_t q[QR];
     constexpr int PLACES = F == kv::kInt8 ? 2 : 4;  // of an accumulator; int8 adds up tiles in fp32 itself
-    float o[NT][PLACES], m = -INFINITY, sum = 0.f, up = 1.f;  // up: what scores are multiplied by for the digits of q
+    float o[NT][PLACES], m = -INFINITY, sum = 0.f, up = 1.f;  // up: what scores are multiplied by, also for the digits of q
     int row_tile = 0;          // the row's first tile in this warp
     bool opened = false, first_row = true;
     int row_start = from - use.tile;  // first tile of the row on the line
@@ -469,11 +478,15 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
             }
           largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
           largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-          // the power of two that brings the largest magnitude into [1, 2): exact both ways
-          const int exponent = max(-100, min(100, (int)(largest >> 23) - 127));
+          // the power of two that brings the largest magnitude into [1, 2): exact both ways, in two steps, since neither it nor
+          // its reciprocal need be a float of its own
+          const auto power = [](int e) { return __uint_as_float((uint32_t)(127 + e) << 23); };
           constexpr int BITS = F == kv::kInt8 ? 21 : 7;
-          const float down = __uint_as_float((uint32_t)(127 - exponent + BITS) << 23);
-          up = largest < 0x7f800000u ? __uint_as_float((uint32_t)(127 + exponent - BITS) << 23) : __int_as_float(0x7fc00000);
+          const int exponent = max(-126, (int)(largest >> 23) - 127), half = exponent / 2;
+          const float down = power(BITS - half), rest = power(half - exponent);
+          up = largest < 0x7f800000u ? a.scale_log2 * power(half) * power(exponent - half - BITS - SHIFT) : __int_as_float(0x7fc00000);
+#pragma unroll
+          for (int r = 0; r < D / 4; ++r) x[r] = times(x[r], rest);
 #pragma unroll
           for (int r = 0; r < D / 16; ++r) {
             if constexpr (F == kv::kInt8) {
@@ -519,7 +532,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
           const float vs = raw < kv::kMinScale ? kv::kMinScale : raw;
           const uint32_t u = __float_as_uint(vs);  // 2^n f
           const float n = vs < 0x1p127f ? __uint_as_float(0x4b000000u | (u >> 23)) - (8388608.f + 127.f) : __int_as_float(0x7fc00000);
-          factors[i] = make_float4(real ? ks * a.scale_log2 : 0.f, real ? n : -INFINITY, real ? __uint_as_float(0x7f000000u - (u & 0x7f800000u)) : 0.f,
+          factors[i] = make_float4(real ? ks * (float)(1 << SHIFT) : 0.f, real ? n : -INFINITY, real ? __uint_as_float(0x7f000000u - (u & 0x7f800000u)) : 0.f,
                                    __uint_as_float((u & 0x007fffffu) | UNIT));
         }
         __syncwarp();
@@ -542,8 +555,8 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
         for (int t = 0; t < TOK / 8; ++t) {
           const int token = use.tile * TOK + t * 8 + 2 * c4;
           const bool pool_ok = (in_pool >> (t / 2)) & 1u;
-          s[t][0] = pool_ok && token < use.n ? acc[t][0] * a.scale_log2 : -INFINITY;
-          s[t][1] = pool_ok && token + 1 < use.n ? acc[t][1] * a.scale_log2 : -INFINITY;
+          s[t][0] = pool_ok && token < use.n ? times(acc[t][0], a.scale_log2) : -INFINITY;
+          s[t][1] = pool_ok && token + 1 < use.n ? times(acc[t][1], a.scale_log2) : -INFINITY;
           top = fmaxf(top, fmaxf(s[t][0], s[t][1]));
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -603,6 +616,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
           const uint32_t row = kb + (place(i) + 4 * (g >> 1) + (g & 1)) * S::ROW;
           if constexpr (F == kv::kInt8 && TWIN) {
             int x[4] = {ZERO_BITS, ZERO_BITS, ZERO_BITS, ZERO_BITS};
+            const float first = last_term ? up : 65536.f * up;
 #pragma unroll
             for (int j = 0; j < D / 64; ++j) {
               const uint4 k = lds128(row + ((D == 128 ? (j * 4 + c4) ^ ((g & 1) << 2) : c4) * 16));
@@ -612,7 +626,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float part = fmaf(sum_of(x[e]), last_term ? 1.f : 65536.f, 256.f * sum_of(x[e + 2]));  // (no second digit in the latter)
+              const float part = fmaf(sum_of(x[e]), first, 256.f * up * sum_of(x[e + 2]));  // (no second digit in the last lanes)
               s[i][e] = part + __shfl_xor_sync(0xffffffffu, part, 16);
             }
           } else if constexpr (F == kv::kInt8) {
@@ -627,7 +641,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
               mma_int8<true>(y, d[8], 0u, d[11], 0u, k.z, k.w);
             }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) s[i][e] = fmaf(sum_of(x[e]), 65536.f, fmaf(sum_of(x[e + 2]), 256.f, sum_of(y[e])));
+            for (int e = 0; e < 2; ++e) s[i][e] = fmaf(sum_of(x[e]), 65536.f * up, fmaf(sum_of(x[e + 2]), 256.f * up, sum_of(y[e]) * up));
           } else {
             float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -638,7 +652,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
               mma_e4m3(x, d[4], d[5], d[6], d[7], k.z, k.w);
             }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) s[i][e] = fmaf(x[e + 2], 0.0625f, x[e]);
+            for (int e = 0; e < 2; ++e) s[i][e] = fmaf(x[e + 2], 0.0625f * up, x[e] * up);
           }
         }
         float inv[TOK / 8][2], rest[TOK / 8][2], top = -INFINITY;
@@ -647,7 +661,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float4 f = factors[place(i) + 4 * c4 + e];
-            s[i][e] = fmaf(s[i][e] * up, f.x, f.y);
+            s[i][e] = fmaf(s[i][e], f.x, f.y);
             inv[i][e] = f.z;
             rest[i][e] = f.w;
             top = fmaxf(top, s[i][e]);

@@ -108,3 +108,22 @@ def test_paged_attention_what_is_not_a_number_stays_so(dtype, length) -> None:
     out, lse = ops.paged_attention(q, pages, table, n, return_lse=True)
     assert torch.isnan(out[0]).any(-1).tolist() == [False, True, True, True, True, True]
     assert torch.isnan(lse[0, :4]).tolist() == [False, True, True, True]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("factor", [1e-36, 1e-33, 1e-30, 1e-20, 1.0, 1e20, 1e30, 5e30, 1e33, 1e36, 1e37])
+def test_paged_attention_query_magnitudes(dtype, factor) -> None:
+    """Queries of every magnitude that bf16 has, whose scores the scale brings back to a few units.
+
+    One rounding to bf16, and the error of the weights: scores up to 30 in fp32 (2^-19) and, of 8-bit caches, queries to 2^-22
+    (int8) or all of their 8 bits (e4m3).
+    """
+    pages = ops.KVPages.allocate(16, 2, 16, 64, dtype=dtype, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    k, v = (torch.randn(256, 2, 64, device="cuda", generator=gen).bfloat16() for _ in range(2))
+    ops.kv_cache_write(pages, 0.25 * k, v, torch.arange(256, device="cuda"))
+    table = torch.arange(16, dtype=torch.int32, device="cuda").view(2, 8)
+    n = torch.tensor([128, 77], dtype=torch.int32, device="cuda")
+    q = (factor * torch.randn(2, 8, 64, device="cuda", generator=gen)).bfloat16()
+    assert bool(torch.isfinite(q).all())
+    _check(q, pages, table, n, 0.5 / factor, 2.0**-18)
