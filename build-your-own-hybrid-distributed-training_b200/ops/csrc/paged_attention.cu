@@ -36,7 +36,8 @@
 //   cost more: 82 us against 71 on 32 rows of 4096).
 //   A token's key scale multiplies its score.  Of its value scale sv = 2^n f, 1 <= f < 2, the power of two joins the
 //   exponent: with s'_t = s_t + n_t, m the maximum of s' rounded up and x_t = 2^(s'_t - m) <= 1, the output is
-//   sum (x_t f_t) v_t / sum (x_t 2^-n_t): weights stay in range whatever the scales are, and nothing is rounded for it.
+//   sum (x_t f_t) v_t / sum (x_t 2^-n_t): nothing is rounded for it.  n is held within 60 of the largest so far (with a smaller
+//   f), so that weights stay in range whatever the scales are, of rows of zeros next to values of 2^64 and more, too.
 // * References m are whole numbers, in all formats: factors between them are powers of two and round nothing.
 // * Joining.  A row inside one warp's range is finished by that warp.  Otherwise warps leave (o, m, sum)
 //   in shared memory, the block merges neighbours, and rows that cross blocks go through a workspace:
@@ -190,6 +191,20 @@ __device__ __forceinline__ float fast_log2(float x) {
   return y;
 }
 
+// 2^d, d <= 0.  References of 8-bit caches contain value scales, which may lie 2^185 apart, and the sums their inverses: a
+// sum takes the factor in two steps (WIDE), since it may be large where the factor alone is too small for fp32.
+template <bool WIDE>
+struct Factor {
+  float first, second, all;
+  __device__ explicit Factor(float d) {
+    const float part = WIDE ? fmaxf(d, -100.f) : d;
+    first = fast_exp2(part);
+    second = WIDE ? fast_exp2(d - part) : 1.f;
+    all = WIDE ? first * second : first;
+  }
+  __device__ __forceinline__ float operator()(float sum) const { return WIDE ? sum * first * second : sum * first; }
+};
+
 // log(2^m sum).  The power of two of the sum joins m, so that the logarithm is that of a number between 1 and 2.  Without a
 // token m is -inf; a sum that is NaN stays so.
 __device__ __forceinline__ float lse_of(float m, float sum) {
@@ -252,6 +267,9 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
   // queries are sums up to 2^37 before it does.
   constexpr int SHIFT = 6;
   constexpr uint32_t UNIT = F == kv::kInt8 ? 0x4f000000u : 0x3f800000u;  // what a weight of 1 is held as, 2^31 or 1, in bits
+  // Value scales more than 2^RANGE below a bound of those of the row so far count as that, with a smaller f.  The bound
+  // leaves room above the largest, so that it seldom moves.
+  constexpr uint32_t RANGE = 60, SPARE = 4;
   extern __shared__ __align__(16) unsigned char smem[];
   struct Meta {
     int item;  // first tile of the row on the line
@@ -426,6 +444,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
     uint32_t q[QR];
     constexpr int PLACES = F == kv::kInt8 ? 2 : 4;  // of an accumulator; int8 adds up tiles in fp32 itself
     float o[NT][PLACES], m = -INFINITY, sum = 0.f, up = 1.f;  // up: what scores are multiplied by, also for the digits of q
+    [[maybe_unused]] uint32_t least = 0;  // power of two that value scales count as at least, as bits of an exponent
     int row_tile = 0;          // the row's first tile in this warp
     bool opened = false, first_row = true;
     int row_start = from - use.tile;  // first tile of the row on the line
@@ -444,6 +463,7 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
         row_tile = use.tile;
         m = -INFINITY;
         sum = 0.f;
+        least = 0;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           o[t][0] = o[t][1] = 0.f;
@@ -525,15 +545,40 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
       // counts as that one; one of 2^127 or more (it leaves at most 2^128 / 127) counts as NaN, which NaN and infinities stay.
       // Masked tokens get a finite score factor and an exponent of -inf.
       if constexpr (F != kv::kBf16) {
+        bool fits = true;
 #pragma unroll
         for (int i = lane; i < TOK; i += 32) {
           const bool real = ((in_pool >> (i / 16)) & 1u) && use.tile * TOK + i < use.n;
           const float ks = stage_scales[i], raw = stage_scales[TOK + i];
           const float vs = raw < kv::kMinScale ? kv::kMinScale : raw;
-          const uint32_t u = __float_as_uint(vs);  // 2^n f
-          const float n = vs < 0x1p127f ? __uint_as_float(0x4b000000u | (u >> 23)) - (8388608.f + 127.f) : __int_as_float(0x7fc00000);
-          factors[i] = make_float4(real ? ks * (float)(1 << SHIFT) : 0.f, real ? n : -INFINITY, real ? __uint_as_float(0x7f000000u - (u & 0x7f800000u)) : 0.f,
-                                   __uint_as_float((u & 0x007fffffu) | UNIT));
+          const uint32_t u = __float_as_uint(vs), n = u >> 23;  // 2^(n - 127) f
+          const float power = vs < 0x1p127f ? __uint_as_float(0x4b000000u | n) - (8388608.f + 127.f) : __int_as_float(0x7fc00000);
+          factors[i] = make_float4(real ? ks * (float)(1 << SHIFT) : 0.f, real ? power : -INFINITY,
+                                   real ? __uint_as_float(0x7f000000u - (u & 0x7f800000u)) : 0.f, __uint_as_float((u & 0x007fffffu) | UNIT));
+          fits = fits && (!real || n - least <= RANGE);
+        }
+        // With a row's first tile, and then hardly ever: a value scale out of range moves the bound, or is brought within it.
+        // (Asking costs 128 x 4097..8192 int8 8 us of 283; a reduction in every tile 15, exponents with room to spare their
+        // last bits.)
+        if (!__all_sync(0xffffffffu, fits)) {
+          uint32_t largest = 0;
+#pragma unroll
+          for (int i = lane; i < TOK; i += 32) {
+            const float power = factors[i].y;
+            if (power > -127.f) largest = max(largest, (uint32_t)(power + 127.f));  // not masked, not NaN
+          }
+          largest = __reduce_max_sync(0xffffffffu, largest) + SPARE;
+          if (largest > least + RANGE) least = largest - RANGE;
+#pragma unroll
+          for (int i = lane; i < TOK; i += 32) {
+            float4& f = factors[i];
+            const float bound = (float)((int)least - 127);
+            if (f.y > -127.f && f.y < bound) {
+              f.w *= fast_exp2(f.y - bound);
+              f.y = bound;
+              f.z = __uint_as_float((254u - least) << 23);
+            }
+          }
         }
         __syncwarp();
       }
@@ -670,12 +715,12 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
         top = ceilf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)));
         const float higher = fmaxf(m, top), now = higher == -INFINITY ? 0.f : higher;  // nothing but masked tokens so far
         if (__any_sync(0xffffffffu, higher > m)) {
-          const float keep = fast_exp2(m - now);
-          sum *= keep;
+          const Factor<true> keep(m - now);
+          sum = keep(sum);
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < PLACES; ++e) o[t][e] *= keep;
+            for (int e = 0; e < PLACES; ++e) o[t][e] *= keep.all;
           m = higher;
         }
         // lane (g, c4) takes dimensions g NT ... + NT - 1 of the tokens whose weights it has
@@ -902,17 +947,18 @@ __global__ void __launch_bounds__(Shape<F, D>::THREADS, 1) decode_kernel(const _
           if (i + k >= job.to) m[k] = -INFINITY;
           higher = fmaxf(higher, m[k]);
         }
-        const float at = higher == -INFINITY ? 0.f : higher, keep = fast_exp2(top - at);
+        const float at = higher == -INFINITY ? 0.f : higher;
+        const Factor<F != kv::kBf16> keep(top - at);
         top = higher;
-        total *= keep;
+        total = keep(total);
 #pragma unroll
-        for (int y = 0; y < VALUES; ++y) x[y] *= keep;
+        for (int y = 0; y < VALUES; ++y) x[y] *= keep.all;
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
-          const float w = fast_exp2(m[k] - at);
-          total = fmaf(w, l[k], total);
+          const Factor<F != kv::kBf16> w(m[k] - at);
+          total += w(l[k]);
 #pragma unroll
-          for (int y = 0; y < VALUES; ++y) x[y] = fmaf(w, v[k][y], x[y]);
+          for (int y = 0; y < VALUES; ++y) x[y] = fmaf(w.all, v[k][y], x[y]);
         }
       }
       const int kv_head = kv_head_of(job.row), in_group = (job.row - kv_head * chunks) * HEADS + g;

@@ -127,3 +127,31 @@ def test_paged_attention_query_magnitudes(dtype, factor) -> None:
     q = (factor * torch.randn(2, 8, 64, device="cuda", generator=gen)).bfloat16()
     assert bool(torch.isfinite(q).all())
     _check(q, pages, table, n, 0.5 / factor, 2.0**-18)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("exponent", [-100, -60, 0, 40, 62, 64, 70, 90, 120])
+@pytest.mark.parametrize("order", ["mixed", "falling", "rising"])
+@pytest.mark.parametrize("lengths", [[200, 37], [9001]])
+def test_paged_attention_value_magnitudes(dtype, exponent, order, lengths) -> None:
+    """Values of every magnitude next to rows of zeros and of small values, whose weights count as much; in any order.
+
+    One rounding to bf16, and the error of the weights: scores up to 10 in fp32 (2^-21), twice.
+    """
+    total = sum(-(-n // 16) * 16 for n in lengths)
+    pages = ops.KVPages.allocate(total // 16, 2, 16, 64, dtype=dtype, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(exponent + 200)
+    k, v = (torch.randn(total, 2, 64, device="cuda", generator=gen) for _ in range(2))
+    kind = torch.randint(0, 3, (total, 1, 1), device="cuda", generator=gen) if order == "mixed" else torch.arange(total, device="cuda")[:, None, None] * 3 // total
+    if order == "falling":
+        kind = 2 - kind
+    v = torch.where(kind == 0, 0.0, torch.where(kind == 1, v, v * 2.0**exponent))
+    ops.kv_cache_write(pages, (0.25 * k).bfloat16(), v.bfloat16(), torch.arange(total, device="cuda"))
+    table = torch.full((len(lengths), -(-max(lengths) // 16)), -1, dtype=torch.int32, device="cuda")
+    start = 0
+    for i, n in enumerate(lengths):
+        used = -(-n // 16)
+        table[i, :used] = torch.arange(start, start + used, device="cuda")
+        start += used
+    q = torch.randn(len(lengths), 8, 64, device="cuda", generator=gen).bfloat16()
+    _check(q, pages, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), 0.5, 2.0**-20)
