@@ -100,6 +100,14 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   // This launch may begin before the streaming one, whose results it does not read, has ended; it must not end before that one.
   if (a.streamed && row == a.B - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (a.streamed && ordinary(temperature) && cuts_nothing(top_k, top_p, min_p, a.V)) return;
+  // Shared memory of a peer may be written once that block runs.  Every thread announces itself here and asks once, before the
+  // first exchange; the row's loads lie between.
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+  bool asked = false;
+  const auto peers_run = [&] {
+    if (!asked) asm volatile("barrier.cluster.wait;" ::: "memory");
+    asked = true;
+  };
   const bool by_count = !greedy && top_k > 0 && top_k < a.V, by_mass = !greedy && !(top_p >= 1.f);
   const float* const noise = a.noise + row * a.noise_stride;
 
@@ -200,6 +208,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
       pick = better(pick, __shfl_xor_sync(0xffffffffu, pick, o));
     }
     // every warp sends its three numbers to every block, which come to the same conclusion
+    peers_run();
     if (lane < blocks) {
       Warp& to = *peer(&sh.warps[rank][warp], lane);
       to.reference = highest;
@@ -302,6 +311,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     if (above == (blocks == 8 ? 9 : blocks == 4 ? 15 : blocks == 2 ? 23 : 29)) sh.warp_top[1][warp] = own_top;
     if (tid == 0) sh.listed = sh.bin_listed = 0u;
     __syncthreads();
+    peers_run();
     if (warp == 0) {
       uint32_t medians[2];
 #pragma unroll

@@ -155,3 +155,27 @@ def test_paged_attention_value_magnitudes(dtype, exponent, order, lengths) -> No
         start += used
     q = torch.randn(len(lengths), 8, 64, device="cuda", generator=gen).bfloat16()
     _check(q, pages, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), 0.5, 2.0**-20)
+
+
+# --------------------------------------------------------------------------- sampling
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("filters", [{}, {"top_p": 0.9}, {"top_k": 700}, {"temperature": 0.0}])
+def test_sample_tokens_while_the_gpu_is_busy(dtype, filters) -> None:
+    """Clusters whose blocks start when another stream's blocks leave room, with short stretches of a row per block."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    b, v = 9, 33000
+    logits = (2.0 * torch.randn(b, v, device="cuda", generator=gen)).to(dtype)
+    noise = torch.empty(b, v, device="cuda").exponential_(generator=gen).clamp_(min=1e-30)
+    want = ops.reference_sample_tokens(logits, noise, **filters, compute_dtype=torch.float64)[0]
+    x = torch.randn(4096, 4096, device="cuda", generator=gen).bfloat16()
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(other):
+            torch.mm(x, x)
+        got += [ops.sample_tokens(logits, noise, **filters)[0] for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
