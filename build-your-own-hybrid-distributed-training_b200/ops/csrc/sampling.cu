@@ -30,6 +30,8 @@
 // overflow.  Integer sums do not depend on their order, so neither do the cuts.
 #include <cooperative_groups.h>
 
+#include <climits>
+
 #include "sampling.cuh"
 
 namespace cg = cooperative_groups;
@@ -767,9 +769,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     // pieces with a token that stays; the random numbers of several are under way together
     constexpr int DEPTH = E == 4 ? 4 : 2;
     const bool together = (reinterpret_cast<uintptr_t>(noise - skew) % 16) == 0;
-    // number >= cut, without working the number out
+    // number >= cut, without working the number out; -inf never stays (places in front of the row hold it, with indices below 0)
     const float lowest = value_of((uint32_t)(cut >> 32));
-    const int last = lowest == -INFINITY ? -1 : (int)min(0xffffffffu - (uint32_t)cut, 0x7fffffffu);
+    const int last = lowest == -INFINITY ? INT_MIN : (int)min(0xffffffffu - (uint32_t)cut, 0x7fffffffu);
     const auto stays = [&](float l, int token) { return l > lowest || (l == lowest && token <= last); };
     for (int i0 = tid; i0 < count; i0 += DEPTH * THREADS) {
       float luck[DEPTH][E];

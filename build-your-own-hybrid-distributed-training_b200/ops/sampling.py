@@ -66,7 +66,8 @@ def reference_sample_tokens(logits: torch.Tensor, noise: torch.Tensor, temperatu
     keep &= (before < top_p.to(compute_dtype) * mass.sum(-1, keepdim=True)) | (top_p >= 1)
     keep &= (ws >= min_p) & ~greedy & (ranked > -math.inf)
     keep |= rank == 0
-    score = torch.where(keep, ws / torch.gather(noise.to(compute_dtype), 1, order), -1.0)
+    # a random number that is none loses to every other, but still names a token
+    score = torch.where(keep, torch.nan_to_num(ws / torch.gather(noise.to(compute_dtype), 1, order), nan=-0.5, posinf=math.inf), -1.0)
     token = torch.where(score == score.amax(-1, keepdim=True), order, v).amin(-1)
     logprob = torch.gather(x, 1, token.clamp(max=v - 1)[:, None])[:, 0] - torch.log(w.sum(-1))
     return torch.where(empty, -1, token), torch.where(empty, -math.inf, logprob)

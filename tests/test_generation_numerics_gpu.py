@@ -179,3 +179,17 @@ def test_sample_tokens_while_the_gpu_is_busy(dtype, filters) -> None:
         got += [ops.sample_tokens(logits, noise, **filters)[0] for _ in range(3)]
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("skew", [1, 3])
+@pytest.mark.parametrize("filters", [{"temperature": 1e30}, {"temperature": 1e-4}, {"min_p": 0.5, "temperature": 1e30}, {}])
+def test_sample_tokens_names_a_token_whatever_the_random_numbers(dtype, skew, filters) -> None:
+    """Rows at odd offsets without a usable random number: the lowest index of those that may be drawn, never one outside the row."""
+    b, v = 5, 3001
+    room = torch.zeros(b, v + 8, device="cuda", dtype=dtype)
+    logits, noise = room[:, skew : skew + v], torch.full((b, v), math.nan, device="cuda")
+    noise[3, 2000] = 1.0
+    token, logprob = ops.sample_tokens(logits, noise, **filters)
+    assert token.tolist() == [0, 0, 0, 2000, 0]
+    assert bool(((logprob + math.log(v)).abs() <= 1e-5 * math.log(v)).all())
