@@ -30,6 +30,7 @@
 // overflow.  Integer sums do not depend on their order, so neither do the cuts.
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <climits>
 
 #include "sampling.cuh"
@@ -818,12 +819,22 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   }
 }
 
+// Blocks per row: as many as let two of them share an SM (72 KB of the row each), and more while all of them run at once
+// and have some tokens for each thread.
+constexpr long long STRETCH = 73728;
+static int blocks_per_row(const Args& a, int sms) {
+  int blocks = 1;
+  while (blocks < MOST_BLOCKS && (long long)a.V * (a.wide ? 4 : 2) > blocks * STRETCH) blocks *= 2;
+  while (blocks < MOST_BLOCKS && (long long)a.B * blocks <= sms && a.V > blocks * 4096) blocks *= 2;
+  return blocks;
+}
+
 template <typename T>
 static cudaError_t launch_as(const Args& a, int blocks, cudaStream_t stream) {
   constexpr int E = 16 / sizeof(T);
   const int pieces = (a.V + 2 * E - 2) / E, each = (pieces + blocks - 1) / blocks;
   const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)each * 16;
-  // dynamic shared memory beyond 48 KB is opted into once per device, for the largest vocabulary
+  // dynamic shared memory beyond 48 KB is opted into once per device, for the longest stretch of a block
   static unsigned long long opted = 0;
   int device = 0;
   cudaError_t err = cudaGetDevice(&device);
@@ -831,7 +842,7 @@ static cudaError_t launch_as(const Args& a, int blocks, cudaStream_t stream) {
   const unsigned long long bit = 1ull << (device & 63);
   if (!(__atomic_load_n(&opted, __ATOMIC_ACQUIRE) & bit)) {
     err = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)(sizeof(Shared) + 64 + (kMaxVocabulary / MOST_BLOCKS) * sizeof(T)));
+                               (int)(sizeof(Shared) + 64 + std::max<long long>(STRETCH, kMaxVocabulary / MOST_BLOCKS * sizeof(T))));
     if (err != cudaSuccess) return err;
     __atomic_fetch_or(&opted, bit, __ATOMIC_RELEASE);
   }
@@ -849,15 +860,6 @@ static cudaError_t launch_as(const Args& a, int blocks, cudaStream_t stream) {
   config.attrs = attributes;
   config.numAttrs = a.streamed ? 2 : 1;
   return cudaLaunchKernelEx(&config, sample_kernel<T>, a);
-}
-
-// Blocks per row: as many as let two of them share an SM (72 KB of the row each), and more while all of them run at once
-// and have some tokens for each thread.
-static int blocks_per_row(const Args& a, int sms) {
-  int blocks = 1;
-  while (blocks < MOST_BLOCKS && (long long)a.V * (a.wide ? 4 : 2) > blocks * 73728ll) blocks *= 2;
-  while (blocks < MOST_BLOCKS && (long long)a.B * blocks <= sms && a.V > blocks * 4096) blocks *= 2;
-  return blocks;
 }
 
 // Rows of which nothing is cut, at an ordinary temperature, are streamed by persistent blocks where clusters of two blocks or

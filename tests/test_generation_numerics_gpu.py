@@ -193,3 +193,18 @@ def test_sample_tokens_names_a_token_whatever_the_random_numbers(dtype, skew, fi
     token, logprob = ops.sample_tokens(logits, noise, **filters)
     assert token.tolist() == [0, 0, 0, 2000, 0]
     assert bool(((logprob + math.log(v)).abs() <= 1e-5 * math.log(v)).all())
+
+
+@pytest.mark.parametrize("v", [32769, 33320, 33321, 35000, 36800, 36864, 36865])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("filters", [{"top_p": 0.9}, {"top_k": 900}])
+def test_sample_tokens_vocabularies_between_powers_of_two(v, dtype, filters) -> None:
+    """Many rows of vocabularies that are a little more than what a block holds of half as many."""
+    gen = torch.Generator(device="cuda").manual_seed(v)
+    b = 150
+    logits = (2.0 * torch.randn(b, v + 1, device="cuda", generator=gen)).to(dtype)[:, 1:]
+    noise = torch.empty(b, v, device="cuda").exponential_(generator=gen).clamp_(min=1e-30)
+    want, want_logprob = ops.reference_sample_tokens(logits, noise, **filters, compute_dtype=torch.float64)
+    token, logprob = ops.sample_tokens(logits, noise, **filters)
+    assert torch.equal(token, want)
+    assert bool(((logprob.double() - want_logprob).abs() <= 4e-6 * (1.0 + want_logprob.abs())).all())
