@@ -819,21 +819,26 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   }
 }
 
-// Blocks per row: as many as let two of them share an SM (72 KB of the row each), and more while all of them run at once
-// and have some tokens for each thread.
-constexpr long long STRETCH = 73728;
+// Bytes of a row that let two blocks share an SM's 228 KB, of which each block takes another 1 KB.
+constexpr long long STRETCH = (228 * 1024 / 2 - 1024 - (long long)(sizeof(Shared) + 15) / 16 * 16) / 16 * 16;
+// Bytes that a block holds of a row that `blocks` share, at the worst alignment.
+static long long stretch(const Args& a, int blocks) {
+  const long long size = a.wide ? 4 : 2, pieces = (a.V * size + 2 * (16 - size)) / 16;
+  return (pieces + blocks - 1) / blocks * 16;
+}
+
+// Blocks per row: as many as let two of them share an SM (512 rows of 36800 in bf16 57.8 us; with one block of 74 KB per row
+// and SM 65.3), and more while all of them run at once and have some tokens for each thread.
 static int blocks_per_row(const Args& a, int sms) {
   int blocks = 1;
-  while (blocks < MOST_BLOCKS && (long long)a.V * (a.wide ? 4 : 2) > blocks * STRETCH) blocks *= 2;
+  while (blocks < MOST_BLOCKS && stretch(a, blocks) > STRETCH) blocks *= 2;
   while (blocks < MOST_BLOCKS && (long long)a.B * blocks <= sms && a.V > blocks * 4096) blocks *= 2;
   return blocks;
 }
 
 template <typename T>
 static cudaError_t launch_as(const Args& a, int blocks, cudaStream_t stream) {
-  constexpr int E = 16 / sizeof(T);
-  const int pieces = (a.V + 2 * E - 2) / E, each = (pieces + blocks - 1) / blocks;
-  const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)each * 16;
+  const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)stretch(a, blocks);
   // dynamic shared memory beyond 48 KB is opted into once per device, for the longest stretch of a block
   static unsigned long long opted = 0;
   int device = 0;
@@ -865,11 +870,12 @@ static cudaError_t launch_as(const Args& a, int blocks, cudaStream_t stream) {
 // Rows of which nothing is cut, at an ordinary temperature, are streamed by persistent blocks where clusters of two blocks or
 // more would need a second wave: 64 rows of 128256 in fp32 21.1 us against 23.1, 256 rows 47 against 81, in bf16 128 rows 27.3
 // against 30.2.  With one wave (32 rows in fp32 15.6 against 11.6 us) or one block per row (512 rows of 32000 in bf16 32.0 against
-// 29.5, 1024 of 16384 in fp32 42 against 38.6) clusters are faster.
+// 29.5, 1024 of 16384 in fp32 42 against 38.6) clusters are faster.  Where a block fills an SM a wave is half as many: 24 rows of
+// 262144 in fp32 23.0 us streamed against 25.5, 37 rows 26.6 against 40.4.
 // Where temperature or filters are per row, only the device knows which rows those are: both kernels are launched, and each
 // leaves the other's rows alone; the second begins as SMs get free (256 rows of 128256 in fp32: 54.7 us, 58 after the first's end).
 // That pays from four blocks per row and two waves on: those 256 rows 54.7 us against 83, 96 rows 27.9 against 34.1, 192 in bf16
-// 37.5 against 44.3; 64 rows in fp32 24.1 against 23.1, 128 in bf16 31.1 against 30.2.  Batches that turn out to be cut lose the
+// 37.5 against 44.3; 48 of 262144 in fp32 32.8 against 53.6; 64 rows in fp32 24.1 against 23.1, 128 in bf16 31.1 against 30.2.  Batches that turn out to be cut lose the
 // time of a launch (256 rows of top-k 1000: 165 -> 170 us).
 static bool whole_stream(const Args& a) {
   if (a.temperature.rows != nullptr) return false;
@@ -880,10 +886,11 @@ static bool whole_stream(const Args& a) {
 
 bool streams(const Args& a, int sms) {
   const int blocks = blocks_per_row(a, sms);
-  if (blocks == 1 || (long long)a.B * blocks <= 2ll * sms) return false;
+  const long long wave = (stretch(a, blocks) <= STRETCH ? 2ll : 1ll) * sms;  // blocks that run at once
+  if (blocks == 1 || (long long)a.B * blocks <= wave) return false;
   // what the streaming kernel counts in 32 bits, and the rows of one block that it can put off
   if (whole_stream(a)) return (long long)a.B * (a.V / 4 + 2) < (1ll << 31) && a.B / sms < 1000;
-  if (blocks < 4 || (long long)a.B * blocks <= 4ll * sms || a.B > kMostListed) return false;
+  if (blocks < 4 || (long long)a.B * blocks <= 2 * wave || a.B > kMostListed) return false;
   return (a.temperature.rows != nullptr || ordinary(a.temperature.same)) &&
          cuts_nothing(a.top_k.rows != nullptr ? 0 : a.top_k.same, a.top_p.rows != nullptr ? 1.f : a.top_p.same,
                       a.min_p.rows != nullptr ? 0.f : a.min_p.same, a.V);
