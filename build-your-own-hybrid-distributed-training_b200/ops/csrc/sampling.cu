@@ -99,6 +99,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   const float temperature = a.temperature[row];
   const bool greedy = !(temperature > 0.f);
   const int top_k = a.top_k[row];
+  // A NaN as top_p or min_p keeps the most probable token alone: its share is a mass of 1, and no weight is at or above it.
   const float top_p = a.top_p[row], min_p = a.min_p[row];
   // This launch may begin before the streaming one, whose results it does not read, has ended; it must not end before that one.
   if (a.streamed && row == a.B - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   const auto better = [](unsigned long long x, unsigned long long y) { return x > y ? x : y; };
 
   // ---- one pass, where nothing is cut and the temperature is an ordinary one
-  if (!by_count && !by_mass && (greedy || (!(min_p > 0.f) && temperature > 1e-3f && temperature < 1e3f))) {
+  if (!by_count && !by_mass && (greedy || (min_p <= 0.f && temperature > 1e-3f && temperature < 1e3f))) {
     const double rate = 1.4426950408889634 / (greedy ? 1.0 : (double)temperature);
     const float hi = (float)rate, lo = (float)(rate - (double)hi);
     const bool together = (reinterpret_cast<uintptr_t>(noise - skew) % 16) == 0;
@@ -444,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
         sum += sh.slice[r];
       }
     }
-    if (target == 0) target = max(1ull, (unsigned long long)ceil(share * (double)sum));
+    if (target == 0) target = (unsigned long long)ceil(fmax(share * (double)sum, 1.0));
     unsigned long long before = base + upto - of_thread;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
@@ -655,7 +656,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
       held_mass += sh.masses[r];
       n += sh.counts[r];
     }
-    unsigned long long limit = max(1ull, (unsigned long long)ceil((double)top_p * whole * 2147483648.0));
+    unsigned long long limit = (unsigned long long)ceil(fmax((double)top_p * whole * 2147483648.0, 1.0));
     const bool holds = greedy || (by_count ? n >= (uint32_t)top_k : by_mass ? held_mass >= limit : min_p > 0.f && weight(least) < min_p);
     if (n <= SHORT && holds) {
       if (rank != 0) return;
@@ -687,7 +688,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
         if (by_count) {
           const unsigned long long left =
               block_reduce(stays && tid % parts == 0 ? (unsigned long long)my_mass : 0ull, sh.scan, [](unsigned long long x, unsigned long long y) { return x + y; });
-          limit = max(1ull, (unsigned long long)ceil((double)top_p * (double)left));
+          limit = (unsigned long long)ceil(fmax((double)top_p * (double)left, 1.0));
         }
         stays = stays && mass_ahead < limit;
       }
@@ -708,7 +709,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
   // ---- a longer one, or all tokens
   double whole = 0.0;
   for (int r = 0; r < blocks; ++r) whole += sh.totals[r];
-  const unsigned long long limit = max(1ull, (unsigned long long)ceil((double)top_p * whole * 2147483648.0));
+  const unsigned long long limit = (unsigned long long)ceil(fmax((double)top_p * whole * 2147483648.0, 1.0));
   float best_score = -1.f;
   uint32_t winner = 0xffffffffu;
   const auto enter = [&](float l, float luck, uint32_t token) {  // a token into the race

@@ -127,7 +127,7 @@ struct Piece {
 
 // Rows that sampling_stream.cu takes: nothing is cut, and the temperature is an ordinary one.
 __host__ __device__ inline bool cuts_nothing(int top_k, float top_p, float min_p, int V) {
-  return (top_k <= 0 || top_k >= V) && top_p >= 1.f && !(min_p > 0.f);
+  return (top_k <= 0 || top_k >= V) && top_p >= 1.f && min_p <= 0.f;  // false for NaN
 }
 __host__ __device__ inline bool ordinary(float temperature) { return temperature > 1e-3f && temperature < 1e3f; }
 

@@ -81,7 +81,7 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, *, temperature: Num
     smallest prefix of those that holds this share of their probability (1: all), ``min_p`` drops tokens less
     probable than this share of the most probable one.  The most probable token always stays, the lower index wins
     ties, and ``temperature`` 0 takes it without drawing.  Each of the four is a number or one value per row
-    (fp32; ``top_k`` int32).  Returns ``(tokens int64 [B], logprobs fp32 [B])``; the log-probability is that of the whole
+    (fp32; ``top_k`` int32); a NaN among a tensor's values leaves the most probable token.  Returns ``(tokens int64 [B], logprobs fp32 [B])``; the log-probability is that of the whole
     row at this temperature (at 1 where the temperature is 0), before any filter.  Logits of ``-inf`` or NaN cannot
     be drawn; a row without any other gives ``-1`` and ``-inf``.
     """

@@ -208,3 +208,20 @@ def test_sample_tokens_vocabularies_between_powers_of_two(v, dtype, filters) -> 
     token, logprob = ops.sample_tokens(logits, noise, **filters)
     assert torch.equal(token, want)
     assert bool(((logprob.double() - want_logprob).abs() <= 4e-6 * (1.0 + want_logprob.abs())).all())
+
+
+@pytest.mark.parametrize("b, v", [(6, 50), (6, 40001), (160, 40001), (40, 128256)])
+@pytest.mark.parametrize("name", ["temperature", "top_p", "min_p"])
+@pytest.mark.parametrize("filters", [{}, {"top_k": 700}])
+def test_sample_tokens_filters_that_are_not_numbers(b, v, name, filters) -> None:
+    """A row whose value is NaN yields its most probable token, in batches of any size and with any other filter."""
+    gen = torch.Generator(device="cuda").manual_seed(b)
+    logits = 2.0 * torch.randn(b, v, device="cuda", generator=gen)
+    noise = torch.empty(b, v, device="cuda").exponential_(generator=gen).clamp_(min=1e-30)
+    values = torch.full((b,), 0.0 if name == "min_p" else 1.0, device="cuda")
+    values[::2] = math.nan
+    filters = {**filters, name: values}
+    token, logprob = ops.sample_tokens(logits, noise, **filters)
+    want, want_logprob = ops.reference_sample_tokens(logits, noise, **filters, compute_dtype=torch.float64)
+    assert torch.equal(token, want) and torch.equal(token[::2], logits[::2].argmax(-1))
+    assert bool(((logprob.double() - want_logprob).abs() <= 4e-6 * (1.0 + want_logprob.abs())).all())
