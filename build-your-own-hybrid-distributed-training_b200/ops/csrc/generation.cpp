@@ -202,6 +202,7 @@ std::tuple<at::Tensor, at::Tensor> sample_tokens(at::Tensor logits, at::Tensor n
   const auto in_range = [](double x, double most) { return x >= 0.0 && x <= most; };  // false for NaN
   HT_CHECK(in_range(temperature, INFINITY) && top_k >= 0 && in_range(top_p, 1.0) && in_range(min_p, 1.0),
            "temperature and top_k must be 0 or more, top_p and min_p between 0 and 1");
+  check_no_gradient(logits, "sample_tokens");
   const c10::cuda::CUDAGuard guard(logits.device());
   at::Tensor token = at::empty({B}, logits.options().dtype(at::kLong).requires_grad(false));
   at::Tensor logprob = at::empty({B}, logits.options().dtype(at::kFloat).requires_grad(false));

@@ -13,7 +13,7 @@ import math
 
 import torch
 
-from ..errors import ConfigurationError, format_error
+from ..errors import ConfigurationError, UnsupportedFeatureError, format_error
 from ._ext import extension
 
 __all__ = ["reference_sample_tokens", "sample_tokens"]
@@ -24,6 +24,14 @@ _MOST_TOKENS = 1 << 18  # vocabulary of the kernel
 
 def _refuse(problem: str, expected: object, observed: object, resolution: str) -> ConfigurationError:
     return ConfigurationError(format_error("ops.sample_tokens", problem, expected=expected, observed=observed, resolution=resolution))
+
+
+def _no_gradient(logits: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and logits.requires_grad:
+        raise UnsupportedFeatureError(format_error("ops.sample_tokens", "a drawn token has no gradient, and its log-probability here none either",
+                                                   expected="logits that need no gradient", observed="requires_grad=True",
+                                                   resolution="call it under torch.no_grad(); for a log-probability with a gradient take "
+                                                              "torch.log_softmax of the logits at the tokens that it returns"))
 
 
 def _check(logits: torch.Tensor, noise: torch.Tensor, filters: dict[str, Number]) -> None:
@@ -83,7 +91,8 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, *, temperature: Num
     ties, and ``temperature`` 0 takes it without drawing.  Each of the four is a number or one value per row
     (fp32; ``top_k`` int32); a NaN among a tensor's values leaves the most probable token.  Returns ``(tokens int64 [B], logprobs fp32 [B])``; the log-probability is that of the whole
     row at this temperature (at 1 where the temperature is 0), before any filter.  Logits of ``-inf`` or NaN cannot
-    be drawn; a row without any other gives ``-1`` and ``-inf``.
+    be drawn; a row without any other gives ``-1`` and ``-inf``.  Neither result has a gradient: logits that need one are
+    refused outside ``torch.no_grad()``.
     """
     if logits.is_cuda:
         try:
@@ -95,6 +104,8 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, *, temperature: Num
             return extension().sample_tokens(logits, noise, *t, *k, *p, *m)
         except RuntimeError:
             _check(logits, noise, {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p})
+            _no_gradient(logits)
             raise
     _check(logits, noise, {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p})
-    return reference_sample_tokens(logits.detach(), noise, temperature, top_k, top_p, min_p)
+    _no_gradient(logits)
+    return reference_sample_tokens(logits, noise, temperature, top_k, top_p, min_p)

@@ -12,6 +12,7 @@ import pytest
 import torch
 
 import hybrid_training.ops as ops
+from hybrid_training.errors import UnsupportedFeatureError
 
 pytestmark = pytest.mark.gpu
 
@@ -225,3 +226,12 @@ def test_sample_tokens_filters_that_are_not_numbers(b, v, name, filters) -> None
     want, want_logprob = ops.reference_sample_tokens(logits, noise, **filters, compute_dtype=torch.float64)
     assert torch.equal(token, want) and torch.equal(token[::2], logits[::2].argmax(-1))
     assert bool(((logprob.double() - want_logprob).abs() <= 4e-6 * (1.0 + want_logprob.abs())).all())
+
+
+def test_sample_tokens_refuses_logits_that_need_a_gradient() -> None:
+    logits, noise = torch.randn(2, 9, device="cuda", requires_grad=True), torch.ones(2, 9, device="cuda")
+    with pytest.raises(UnsupportedFeatureError):
+        ops.sample_tokens(logits, noise)
+    with torch.no_grad():
+        token, logprob = ops.sample_tokens(logits, noise)
+    assert token.shape == (2,) and not logprob.requires_grad
