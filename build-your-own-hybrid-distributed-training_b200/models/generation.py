@@ -12,8 +12,8 @@
   :func:`~hybrid_training.ops.sample_tokens`.
 
 Every step is stream-ordered; the host waits only where a stop token is asked for.  Tensor parallelism
-works as in training (each rank caches its own key/value heads; give every rank a generator of the
-same seed).  The reference has no generation; its model recomputes whole sequences
+works as in training: each rank caches its own key/value heads, and the tokens that the tensor group's
+first rank draws are everyone's, whatever the other ranks' generators say.  The reference has no generation; its model recomputes whole sequences
 (``src/hybrid_training/models/transformer.py:427-512``).
 """
 
@@ -25,6 +25,7 @@ from dataclasses import dataclass
 import torch
 
 from .. import ops
+from ..distributed.collectives import broadcast
 from ..errors import ConfigurationError, UnsupportedFeatureError, format_error
 from ..ops.attention import attention_window_forward
 from .transformer import TinyTransformer
@@ -174,6 +175,16 @@ def _decode(model: TinyTransformer, cache: GenerationCache, tokens: torch.Tensor
     return _run_layers(model, _embed(model, tokens[None], positions), attend)[0]
 
 
+def _agree(token: torch.Tensor, logprob: torch.Tensor, model: TinyTransformer) -> tuple[torch.Tensor, torch.Tensor]:
+    """The first tensor rank's draws on every rank: one token that differed would mix two texts in every later step."""
+    group = model.plan.tensor_group
+    if group.size == 1:
+        return token, logprob
+    both = torch.stack((token, logprob.view(torch.int32).long()))
+    broadcast(both, group).wait()
+    return both[0], both[1].int().view(torch.float32)
+
+
 @torch.no_grad()
 def generate(model: TinyTransformer, prompts: Sequence[Sequence[int] | torch.Tensor], max_new_tokens: int, *,
              temperature: float | torch.Tensor = 1.0, top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
@@ -182,7 +193,7 @@ def generate(model: TinyTransformer, prompts: Sequence[Sequence[int] | torch.Ten
     """``max_new_tokens`` tokens after each of ``prompts`` (token ids), fewer where ``stop_token`` comes first (it is kept).
 
     ``temperature``, ``top_k``, ``top_p`` and ``min_p`` are those of :func:`~hybrid_training.ops.sample_tokens`, numbers or one value
-    per prompt; ``generator`` (on the model's device) makes a run repeatable.  ``cache_dtype`` is ``torch.bfloat16`` (default on CUDA),
+    per prompt; ``generator`` (on the model's device) makes a run repeatable (with tensor parallelism the first rank's).  ``cache_dtype`` is ``torch.bfloat16`` (default on CUDA),
     ``torch.int8`` or ``torch.float8_e4m3fn``.  ``prefill_chunk`` is a multiple of 128.
     """
     _check_model(model)
@@ -225,7 +236,7 @@ def generate(model: TinyTransformer, prompts: Sequence[Sequence[int] | torch.Ten
     for step in range(max_new_tokens):
         logits = model.output_projection(last)
         noise = torch.empty(logits.shape, dtype=torch.float32, device=device).exponential_(generator=generator)
-        token, logprob = ops.sample_tokens(logits, noise, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        token, logprob = _agree(*ops.sample_tokens(logits, noise, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p), model)
         tokens.append(token)
         logprobs.append(logprob)
         kept.append(active)
