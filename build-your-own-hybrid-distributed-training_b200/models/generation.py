@@ -44,6 +44,11 @@ class GenerationOutput:
     logprobs: list[torch.Tensor]
 
 
+def _to_device(x: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """A copy on ``device`` that the host does not wait for."""
+    return x.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else x.to(device)
+
+
 class GenerationCache:
     """Keys and values of every layer for a batch of sequences, in pages that are handed out up front.
 
@@ -68,7 +73,7 @@ class GenerationCache:
             table[b, :n] = torch.arange(start, start + n, dtype=torch.int32)
             start += n
         self.page_size = page_size
-        self.block_table = table.to(device)
+        self.block_table = _to_device(table, device)
         self.lengths = torch.zeros(len(counts), dtype=torch.int32, device=device)
 
     def slots(self, positions: torch.Tensor, valid: torch.Tensor) -> torch.Tensor:
@@ -219,8 +224,8 @@ def generate(model: TinyTransformer, prompts: Sequence[Sequence[int] | torch.Ten
     prompt = torch.zeros(batch, max(counts), dtype=torch.int64)
     for b, p in enumerate(ids):
         prompt[b, :counts[b]] = p
-    prompt = prompt.to(device)
-    length = torch.tensor(counts, device=device)
+    prompt = _to_device(prompt, device)
+    length = _to_device(torch.tensor(counts), device)
 
     # hidden state of every prompt's last token, from whichever chunk it falls into
     last = None
@@ -232,21 +237,21 @@ def generate(model: TinyTransformer, prompts: Sequence[Sequence[int] | torch.Ten
     cache.lengths.copy_(length)
 
     active = torch.ones(batch, dtype=torch.bool, device=device)
-    tokens, logprobs, kept = [], [], []
+    tokens, logprobs, kept = [], [], []  # kept: with a stop token, who had not met it yet
     for step in range(max_new_tokens):
         logits = model.output_projection(last)
         noise = torch.empty(logits.shape, dtype=torch.float32, device=device).exponential_(generator=generator)
         token, logprob = _agree(*ops.sample_tokens(logits, noise, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p), model)
         tokens.append(token)
         logprobs.append(logprob)
-        kept.append(active)
         if stop_token is not None:
+            kept.append(active)
             active = active & (token != stop_token)
             if not bool(active.any()):
                 break
         if step + 1 < max_new_tokens:
             # a sequence that has stopped stays in the batch; what it computes is not kept
             last = _decode(model, cache, token.clamp(min=0), active, tables)
-    keep = torch.stack(kept).sum(0).tolist()
+    keep = torch.stack(kept).sum(0).tolist() if kept else [max_new_tokens] * batch
     rows, scores = torch.stack(tokens, 1), torch.stack(logprobs, 1)
     return GenerationOutput([rows[b, :n] for b, n in enumerate(keep)], [scores[b, :n] for b, n in enumerate(keep)])
