@@ -5,7 +5,7 @@
 :class:`GenerationCache`, pages of :class:`~hybrid_training.ops.KVPages` (bf16, int8 or fp8):
 
 * the prompts run through the flash kernels, in chunks of ``prefill_chunk`` positions (which bounds the
-  activations); each chunk's keys and values are written to the cache, and a later chunk reads the earlier
+  activations; those that have ended leave the batch); each chunk's keys and values are written to the cache, and a later chunk reads the earlier
   ones back next to its own and attends with a query window;
 * each further token is embedded, projected and written for all sequences at once, attends through
   :func:`~hybrid_training.ops.paged_attention`, and the next one is drawn by
@@ -76,10 +76,11 @@ class GenerationCache:
         self.block_table = _to_device(table, device)
         self.lengths = torch.zeros(len(counts), dtype=torch.int32, device=device)
 
-    def slots(self, positions: torch.Tensor, valid: torch.Tensor) -> torch.Tensor:
-        """Slots ``[B, S]`` of each sequence's tokens at ``positions`` ``[B, S]``; -1 where ``valid`` is false."""
+    def slots(self, positions: torch.Tensor, valid: torch.Tensor, rows: torch.Tensor | None = None) -> torch.Tensor:
+        """Slots ``[B, S]`` of each sequence's (or those of ``rows``) tokens at ``positions`` ``[B, S]``; -1 where ``valid`` is false."""
+        table = self.block_table if rows is None else self.block_table[rows]
         page = torch.div(positions, self.page_size, rounding_mode="floor").clamp(max=max(self.block_table.shape[1] - 1, 0))
-        at = torch.gather(self.block_table.long(), 1, page)
+        at = torch.gather(table.long(), 1, page)
         return torch.where(valid, at * self.page_size + positions % self.page_size, -1)
 
 
@@ -127,15 +128,17 @@ def _run_layers(model: TinyTransformer, hidden: torch.Tensor, attend: Attend) ->
     return model.final_norm(residual, delta, out_dtype=model.compute_dtype)[1]
 
 
-def _prefill(model: TinyTransformer, cache: GenerationCache, tokens: torch.Tensor, counts: torch.Tensor, begin: int, tables: tuple[torch.Tensor, torch.Tensor] | None) -> torch.Tensor:
-    """Runs positions ``[begin, begin + S)`` of right-padded prompts ``tokens`` ``[B, S]`` and caches them; returns the hidden states."""
+def _prefill(model: TinyTransformer, cache: GenerationCache, tokens: torch.Tensor, counts: torch.Tensor, begin: int,
+             tables: tuple[torch.Tensor, torch.Tensor] | None, sequences: torch.Tensor | None) -> torch.Tensor:
+    """Runs positions ``[begin, begin + S)`` of right-padded prompts ``tokens`` ``[B, S]`` of the cache's ``sequences`` (``None``: of
+    all) and caches them; returns the hidden states."""
     b, s = tokens.shape
     attention = model.blocks[0].attention
     h, hkv, d = attention.heads_per_partition, attention.kv_heads_per_partition, attention.head_dim
     positions = torch.arange(begin, begin + s, device=tokens.device)
-    slots = cache.slots(positions.expand(b, s), positions[None] < counts[:, None]).reshape(-1)
+    slots = cache.slots(positions.expand(b, s), positions[None] < counts[:, None], sequences).reshape(-1)
     before = torch.arange(begin, device=tokens.device)
-    earlier = cache.slots(before.expand(b, begin), before[None] < counts[:, None]).reshape(-1)
+    earlier = cache.slots(before.expand(b, begin), before[None] < counts[:, None], sequences).reshape(-1)
     if tables is not None:
         cos, sin = (t[begin:begin + s].contiguous() for t in tables)
 
@@ -227,13 +230,19 @@ def generate(model: TinyTransformer, prompts: Sequence[Sequence[int] | torch.Ten
     prompt = _to_device(prompt, device)
     length = _to_device(torch.tensor(counts), device)
 
-    # hidden state of every prompt's last token, from whichever chunk it falls into
-    last = None
+    # hidden state of every prompt's last token, from the chunk that it falls into
+    ends, order = [], []
     for begin in range(0, max(counts), prefill_chunk):
-        hidden = _prefill(model, cache, prompt[:, begin:begin + prefill_chunk].contiguous(), length, begin, tables)
-        at = length - 1 - begin
-        here = hidden[torch.arange(batch, device=device), at.clamp(0, hidden.shape[1] - 1)]
-        last = here if last is None else torch.where(((at >= 0) & (at < hidden.shape[1]))[:, None], here, last)
+        mine = [b for b in range(batch) if counts[b] > begin]
+        sequences = None if len(mine) == batch else _to_device(torch.tensor(mine), device)
+        chunk, of = (prompt, length) if sequences is None else (prompt[sequences], length[sequences])
+        hidden = _prefill(model, cache, chunk[:, begin:begin + prefill_chunk].contiguous(), of, begin, tables, sequences)
+        ending = [i for i, b in enumerate(mine) if counts[b] <= begin + prefill_chunk]
+        if ending:
+            order += [mine[i] for i in ending]
+            at = torch.tensor([[i, counts[mine[i]] - 1 - begin] for i in ending])
+            ends.append(hidden[tuple(_to_device(at, device).T)])
+    last = torch.cat(ends)[_to_device(torch.tensor(order).argsort(), device)]
     cache.lengths.copy_(length)
 
     active = torch.ones(batch, dtype=torch.bool, device=device)
