@@ -57,9 +57,12 @@ template <int F, int D>
 struct Shape {
   static constexpr int ROW = D * (F == kv::kBf16 ? 2 : 1);  // bytes of one key
   static constexpr int TOK = ROW == 256 ? 16 : ROW == 64 ? 64 : 32;  // tokens of one tile: 8 KB of keys and values
-  // Warps of a block, as many as registers and shared memory take and measured best (10 and 12 instead of 8: 91 against 94 us
-  // on 32 rows of 4096 at D = 128 in bf16, 69 against 73 at D = 64; int8 at D = 128 spills registers with 10: 67 against 59).
-  static constexpr int WARPS = F == kv::kBf16 ? (D == 64 ? 12 : 10) : (D == 64 ? 10 : 8);
+  // Warps of a block.  Heads of 64 leave registers for more than 8, which pays as long as loads are what a warp waits for: bf16
+  // 12 (48 ragged GPT-2 rows 23.8 us, with 10 25.0, with 8 25.3; 32 x 4096 at 32/8 heads 50.0, 50.7, 51.1), int8 10 (48 ragged rows
+  // 24.0 us, with 8 24.7, with 6 28.6; 32 x 4096 43.3, 43.2, 51.4), but e4m3 8 (32 x 4096 47.4 us, with 10 51.5, with 6 59.3).
+  // Heads of 128 take 8: 32 x 4096 at 32/8 and at 32/4 heads bf16 91.0 and 52.0 us (with 10 92.2 and 53.0), int8 61 and 43.1 (10,
+  // where 8 heads spill registers, 62 and 47.8; 6: 70.6 and 51.4), e4m3 70 and 43.2 (10, spilling, 78 and 49.0; 6: 86 and 52).
+  static constexpr int WARPS = D == 128 ? 8 : F == kv::kBf16 ? 12 : F == kv::kInt8 ? 10 : 8;
   static constexpr int DATA = TOK * ROW, SCALES = F == kv::kBf16 ? 0 : TOK * 4;
   static constexpr int STAGE = 2 * (DATA + SCALES);
   static constexpr int STAGES = 2;  // one tile under way while the other is used
