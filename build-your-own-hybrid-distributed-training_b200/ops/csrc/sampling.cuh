@@ -8,6 +8,7 @@ namespace sampling {
 
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr float LN2 = 0.6931471805599453f;
+constexpr float MASS = 0x1p44f;  // what a weight of 1 is held as
 
 // Unsigned keys in the order of the floats; -inf has the lowest one.
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -73,7 +74,10 @@ struct Weights {
     const Pair x = fma(d, pair(hi, hi), times(pair(fmaxf(low(d), least), fmaxf(high(d), least)), pair(lo, lo)));
     return pair(fast_exp2(low(x)), fast_exp2(high(x)));
   }
-  __device__ __forceinline__ uint32_t fixed(float l) const { return (uint32_t)__float2uint_rn((*this)(l)*2147483648.f); }
+  // Masses as integers, which add up to the same in every order: multiples of 2^-44, and, for weights that are known to be at
+  // most 2^-k, of 2^-(31 + k) in half as many bits.
+  __device__ __forceinline__ unsigned long long mass(float l) const { return __float2ull_rn((*this)(l)*MASS); }
+  __device__ __forceinline__ uint32_t mass(float l, int k) const { return __float2uint_rn((*this)(l)*__uint_as_float((uint32_t)(127 + 31 + k) << 23)); }
 };
 
 // A sum of weights, two at a time, that comes out the same in every order (and so for every alignment of the row): multiples

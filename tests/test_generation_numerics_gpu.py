@@ -235,3 +235,36 @@ def test_sample_tokens_refuses_logits_that_need_a_gradient() -> None:
     with torch.no_grad():
         token, logprob = ops.sample_tokens(logits, noise)
     assert token.shape == (2,) and not logprob.requires_grad
+
+
+@pytest.mark.parametrize("v,b", [(128256, 2), (128256, 40), (50257, 6), (20011, 100), (3001, 4)])
+@pytest.mark.parametrize("depth", [10.0, 24.0, 28.0, 30.5, 33.5, 45.0])
+@pytest.mark.parametrize("top_k", [0, 2999])
+def test_sample_tokens_cuts_long_tails_where_their_sum_says(v, b, depth, top_k) -> None:
+    """One likely token and a tail of weights 2^-depth, of which top_p keeps half.
+
+    Row after row, the one token that would win the draw lies a thirtieth of the tail's mass within the cut, or beyond it.  Weights
+    are right to 2^-22 and add up as multiples of 2^-44 or finer, far closer than that; multiples of 2^-31 would keep the
+    whole tail, or none.  top_p is an fp32 number, so the tail has to weigh a few hundred of its last places.
+    """
+    kept_of = v - 1 if top_k == 0 else top_k - 1
+    tail = kept_of * 2.0**-depth
+    if tail < 300 * 2.0**-24:
+        pytest.skip("the tail is lost among top_p's last places")
+    gen = torch.Generator(device="cuda").manual_seed(v)
+    z = -math.log(2.0) * depth + 0.01 * torch.randn(b, v, device="cuda", generator=gen)
+    z.scatter_(1, torch.randint(0, v, (b, 1), device="cuda", generator=gen), 0.0)
+    top_p = (1.0 + 0.5 * tail) / (1.0 + tail)
+    order = torch.sort(z, dim=-1, descending=True, stable=True).indices
+    w = torch.softmax(torch.gather(z, 1, order).double(), -1)
+    if top_k:
+        w[:, top_k:] = 0.0
+    w /= w.sum(-1, keepdim=True)
+    before = torch.cumsum(w, -1) - w
+    edge = float(torch.tensor(top_p, dtype=torch.float32)) + torch.where(torch.arange(b, device="cuda") % 2 == 0, -1.0, 1.0)[:, None] * (1.0 - 1.0 / (1.0 + tail)) / 30.0
+    favourite = torch.gather(order, 1, (before < edge).sum(-1, keepdim=True) - 1)
+    noise = torch.ones(b, v, device="cuda").scatter_(1, favourite, 1e-20)
+    token, _ = ops.sample_tokens(z, noise, top_p=top_p, top_k=top_k)
+    inside = torch.arange(b, device="cuda") % 2 == 0
+    assert torch.equal(token, torch.where(inside, favourite[:, 0], z.argmax(-1)))
+    assert torch.equal(token, ops.reference_sample_tokens(z, noise, top_p=top_p, top_k=top_k, compute_dtype=torch.float64)[0])
