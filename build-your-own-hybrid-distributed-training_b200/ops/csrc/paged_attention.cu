@@ -20,15 +20,15 @@
 //   what rounding left over of the same heads' operand.  P enters with the 24 bits of an fp32 weight, as three bf16 terms or
 //   four digits of 8 bits, since two of either would move one bf16 output in 600 (bf16) or 60 (int8) to its neighbour.  Where a row
 //   has at most 4 heads the third (and fourth) go to rows 4-7 (and 12-15), whose lanes repeat the scores of rows 0-3: no
-//   further instruction (32 x 4096 bf16 at 32/8 heads 92.2 us, with two terms 91.8; 48 ragged GPT-2 rows 23.8 and 23.4).  With 5
-//   to 8 heads they take a second instruction (32 x 4096 at 32/4 heads: bf16 53.0 and 51.9 us, int8 41.2 and 37.1).
+//   further instruction (10 warps, 32 x 4096 bf16 at 32/8 heads 92.2 us, with two terms 91.8; 48 ragged GPT-2 rows 23.8 and 23.4).
+//   With 5 to 8 heads they take a second instruction (32 x 4096 at 32/4 heads: bf16 53.0 and 51.9 us, int8 41.2 and 37.1).
 //   The dimensions of q and k are summed in the order in which 16-byte loads deliver them, and the tokens of a tile in
 //   the order in which score accumulators and the second product's operand agree: no data is moved for either.
 // * 8 bits.  Keys enter the instructions (m16n8k32) as they are held, so q has to be in 8 bits too, as digits, worked
 //   out once per row.  int8: q of a head, scaled by a power of two and rounded to 22 bits, is three signed digits, and
 //   the sums are exact integers (below 2^22, read as floats by starting the accumulators at the bits of 1.5 2^23).  The
-//   third digit has rows 4-7 of at most 4 heads, or a second instruction; with the former 128 x 4097..8192 at 32/8
-//   heads take 272 us, with the latter 293.
+//   third digit has rows 4-7 of at most 4 heads, or a second instruction, which took 128 x 4097..8192 at 32/8 heads from
+//   272 us to 293.
 //   e4m3: q is two terms of 4 bits each, which hold all 8 bits of a bf16.  int8 values are used as they are as well,
 //   with floor(2^31 p) as four unsigned digits: p is taken relative to the tile's own maximum, so that its
 //   digits always start at the tile's largest weight, and the tile's product is added to the output in fp32.  e4m3 values are

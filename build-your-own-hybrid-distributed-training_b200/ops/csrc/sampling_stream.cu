@@ -13,7 +13,12 @@
 // A warp keeps one reference for its exponents, an integer that rises with the largest logit so far, and the
 // best score so far.  At the end of a row, or of the block's part of it, the warps' (reference, sum, best token) are merged by
 // one warp while the others go on; rows that cross blocks go through a workspace, where the block that arrives last
-// merges the parts in their order, so that results do not depend on timing.
+// merges the parts in their order, so that results do not depend on timing.  Rows whose logits leave the range in which one
+// reference serves (beyond 1e5 in the exponent, or infinite) are put off and done by their block one after the other: a batch of
+// nothing else takes 264 us for 256 rows of 128256 in fp32, and 71 for 160 of 50257 in bf16 (ordinary ones 51.5 and 32).
+//
+// Sums of weights are fp32: a thread adds at most some 256 of a row, whose roundings leave 5e-8 of the log-probability, as much
+// as its own rounding.
 #include "sampling.cuh"
 
 namespace ht {
