@@ -36,8 +36,9 @@
 //   cost more: 82 us against 71 on 32 rows of 4096).
 //   A token's key scale multiplies its score.  Of its value scale sv = 2^n f, 1 <= f < 2, the power of two joins the
 //   exponent: with s'_t = s_t + n_t, m the maximum of s' rounded up and x_t = 2^(s'_t - m) <= 1, the output is
-//   sum (x_t f_t) v_t / sum (x_t 2^-n_t): nothing is rounded for it.  n is held within 60 of the largest so far (with a smaller
-//   f), so that weights stay in range whatever the scales are, of rows of zeros next to values of 2^64 and more, too.
+//   sum (x_t f_t) v_t / sum (x_t 2^-n_t): what is rounded for it is s' alone, like the score itself.  n is held within 60 of the
+//   largest so far (with a smaller f), so that weights stay in range whatever the scales are, of rows of zeros next to values
+//   of 2^64 and more, too.
 // * References m are whole numbers, in all formats: factors between them are powers of two and round nothing.
 // * Joining.  A row inside one warp's range is finished by that warp.  Otherwise warps leave (o, m, sum)
 //   in shared memory, the block merges neighbours, and rows that cross blocks go through a workspace:
